@@ -1,0 +1,361 @@
+// eventad_amd/csrc/rmsnorm.hip -- root-mean-square norm of rows with the residual's addition, its gradient, and the form
+// with an 8-bit output.
+//
+//   h = round(x + residual),   r = 1 / sqrt(mean(h^2) + eps),   y = h r w
+//   8 bit: scale = max|y| / 448 per row,  q = e4m3(y / scale)
+//
+// h is rounded to the activations' type before it is used, because it is what the next layer reads and what the backward pass
+// has: norm and gradient are those of the stored sum.  Gradient, with e = dy w:
+//   dh = r (e - h r^2 mean(e h)) + dsum   (the gradient of x and of residual),   dw = sum over rows of dy h r
+//
+// Bound by bytes.  LANES lanes hold a row in registers (ITERS 16-byte pieces each), so every array is read and written once;
+// sums over a row go through DPP / shuffles, over more than a wave through LDS.  Rows too long for registers are read twice.
+#include "seq.h"
+
+struct NormArgs {
+    const void *x, *res; int64_t ldx, ldr;
+    const float* w;
+    void *sum, *y; int64_t lds, ldy;
+    uint8_t* q; int64_t ldq; float* scale;
+    int64_t rows; int channels; float eps;
+    // gradient
+    const void *dy, *dsum; int64_t lddy, ldds;
+    void* dh; int64_t lddh;
+    float* part;                                     // [workgroups][channels]
+};
+
+// sum / maximum over the LANES lanes that share a row
+template <int LANES, typename F> __device__ __forceinline__ F row_sum(F v, F* s) {
+#pragma unroll
+    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) v += __shfl_xor(v, d, 64);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = s[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v += s[i];
+    }
+    return v;
+}
+// (of non-negative doubles as bit patterns: NaN is the largest of all and stays)
+template <int LANES> __device__ __forceinline__ double row_max(double v, double* s) {
+    auto top = [](double p, double q) { return __double_as_longlong(p) > __double_as_longlong(q) ? p : q; };
+#pragma unroll
+    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) v = top(v, __shfl_xor(v, d, 64));
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = s[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v = top(v, s[i]);
+    }
+    return v;
+}
+
+// v rounded towards the odd neighbour, so that a second rounding to fewer bits is the one rounding of v: e4m3 keeps 4 of the
+// 24 bits of a float
+__device__ __forceinline__ float norm_to_odd(double v) {
+    const float f = (float)v;
+    const double back = (double)f;
+    if (back == v || !(fabs(v) < 1e30)) return f;
+    unsigned u = __float_as_uint(f);
+    if (fabs(back) > fabs(v)) --u;                               // towards zero
+    return __uint_as_float(u | 1u);
+}
+
+// y / scale = 448 h w / max|h w| needs no r.  It is formed in float64, where h w is exact, so that a value next to a border
+// of the 8-bit grid falls on the side the definition says.
+__device__ __forceinline__ unsigned norm_e4m3(float h, float w, double inv) {
+    const float f = norm_to_odd((double)h * (double)w * inv);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false) & 0xffu;
+}
+struct NormScale { double inv; float scale; };
+__device__ __forceinline__ NormScale norm_scale(double top, float r) {
+    NormScale s;
+    s.scale = (float)(top * (double)r / 448.0);
+    if (!(s.scale >= 1.17549435e-38f) && s.scale == s.scale) { s.scale = 1.f; s.inv = (double)r; }   // a row of zeros (or next to it)
+    else s.inv = 448.0 / top;
+    return s;
+}
+
+// LOOP: the row does not fit ITERS pieces per lane and is read again for every pass over it.
+template <typename T, int V, int LANES, int ITERS, bool LOOP, bool FP8>
+__global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
+    __shared__ double s_red[4];
+    constexpr int PER = 256 / LANES;
+    const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES, D = a.channels;
+    const bool in = row < a.rows;
+    const int64_t r = in ? row : a.rows - 1;
+    const T* x = (const T*)a.x + r * a.ldx;
+    const T* res = a.res ? (const T*)a.res + r * a.ldr : nullptr;
+    float h[ITERS][V];
+    auto piece = [&](int c, float (&v)[V], bool store) {         // h of the piece at column c
+        seq_load<T, V>(x + c, v);
+        if (res) {
+            float e[V];
+            seq_load<T, V>(res + c, e);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = (float)(T)(v[i] + e[i]);
+            if (store) seq_store<T, V>((T*)a.sum + r * a.lds + c, v);
+        }
+    };
+    float ss = 0.f;
+    if constexpr (LOOP) {
+        for (int c = lane * V; c < D; c += LANES * V) {
+            float v[V];
+            piece(c, v, in);
+#pragma unroll
+            for (int i = 0; i < V; ++i) ss = fmaf(v[i], v[i], ss);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            const int c = (k * LANES + lane) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) h[k][i] = 0.f;
+            if (c < D) piece(c, h[k], in);
+        }
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) ss = fmaf(h[k][i], h[k][i], ss);
+    }
+    ss = row_sum<LANES, float>(ss, (float*)s_red);
+    const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+    NormScale sc = {0.0, 0.f};
+    if constexpr (FP8) {
+        double top = 0.0;
+        auto fold = [&](int c, const float (&v)[V]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double p = fabs((double)v[i] * (double)a.w[c + i]);
+                if (__double_as_longlong(p) > __double_as_longlong(top)) top = p;
+            }
+        };
+        if constexpr (LOOP) { for (int c = lane * V; c < D; c += LANES * V) { float v[V]; piece(c, v, false); fold(c, v); } }
+        else {
+#pragma unroll
+            for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, h[k]); }
+        }
+        top = row_max<LANES>(top, s_red);
+        sc = norm_scale(top, inv);
+        if (in && lane == 0) a.scale[r] = sc.scale;
+    }
+    if (!in) return;
+    auto finish = [&](int c, const float (&v)[V]) {
+        if constexpr (FP8) {
+            uint8_t* q = a.q + r * a.ldq + c;
+            if constexpr (V == 1) *q = (uint8_t)norm_e4m3(v[0], a.w[c], sc.inv);
+            else {
+                unsigned word[V / 4];
+#pragma unroll
+                for (int i = 0; i < V; i += 4) {
+                    word[i / 4] = 0;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) word[i / 4] |= norm_e4m3(v[i + m], a.w[c + i + m], sc.inv) << (8 * m);
+                }
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i) ((unsigned*)q)[i] = word[i];
+            }
+        } else {
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[i] = v[i] * inv * a.w[c + i];
+            seq_store<T, V>((T*)a.y + r * a.ldy + c, y);
+        }
+    };
+    if constexpr (LOOP) { for (int c = lane * V; c < D; c += LANES * V) { float v[V]; piece(c, v, false); finish(c, v); } }
+    else {
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, h[k]); }
+    }
+}
+
+// A workgroup goes over rows blockIdx.x, blockIdx.x + gridDim.x, ... (x PER rows at a time) and keeps its share of dw in
+// registers (LOOP: in its own row of `part`).
+template <typename T, int V, int LANES, int ITERS, bool LOOP>
+__global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
+    __shared__ double s_red[4];
+    __shared__ float s_dw[LANES < 256 ? 256 * V * ITERS : 1];
+    constexpr int PER = 256 / LANES;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, D = a.channels;
+    float dw[ITERS][V];
+#pragma unroll
+    for (int k = 0; k < ITERS; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
+    float* part = a.part + (int64_t)blockIdx.x * D;
+    if constexpr (LOOP) {
+        for (int c = lane * V; c < D; c += LANES * V)
+#pragma unroll
+            for (int i = 0; i < V; ++i) part[c + i] = 0.f;
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * PER; r0 < a.rows; r0 += (int64_t)gridDim.x * PER) {
+        const bool in = r0 + sub < a.rows;
+        const int64_t r = in ? r0 + sub : a.rows - 1;
+        const T* hr = (const T*)a.sum + r * a.lds;
+        const T* gr = (const T*)a.dy + r * a.lddy;
+        const T* sr = a.dsum ? (const T*)a.dsum + r * a.ldds : nullptr;
+        float h[ITERS][V], g[ITERS][V], ss = 0.f, eh = 0.f;
+        auto fold = [&](int c, const float (&hv)[V], const float (&gv)[V]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) { ss = fmaf(hv[i], hv[i], ss); eh = fmaf(gv[i] * a.w[c + i], hv[i], eh); }
+        };
+        if constexpr (LOOP) {
+            for (int c = lane * V; c < D; c += LANES * V) { float hv[V], gv[V]; seq_load<T, V>(hr + c, hv); seq_load<T, V>(gr + c, gv); fold(c, hv, gv); }
+        } else {
+#pragma unroll
+            for (int k = 0; k < ITERS; ++k) {
+                const int c = (k * LANES + lane) * V;
+                if (c < D) { seq_load<T, V>(hr + c, h[k]); seq_load<T, V>(gr + c, g[k]); }
+                else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) { h[k][i] = 0.f; g[k][i] = 0.f; }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, h[k], g[k]); }
+        }
+        ss = row_sum<LANES, float>(ss, (float*)s_red);
+        eh = row_sum<LANES, float>(eh, (float*)s_red);
+        const float inv = 1.f / sqrtf(ss / (float)D + a.eps), m = inv * inv * (eh / (float)D);
+        if (!in) continue;
+        auto finish = [&](int c, const float (&hv)[V], const float (&gv)[V], float (&acc)[V]) {
+            float dh[V], ds[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) ds[i] = 0.f;
+            if (sr) seq_load<T, V>(sr + c, ds);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                dh[i] = fmaf(inv, fmaf(-hv[i], m, gv[i] * a.w[c + i]), ds[i]);
+                acc[i] = fmaf(gv[i] * inv, hv[i], acc[i]);
+            }
+            seq_store<T, V>((T*)a.dh + r * a.lddh + c, dh);
+        };
+        if constexpr (LOOP) {
+            for (int c = lane * V; c < D; c += LANES * V) {
+                float hv[V], gv[V], acc[V];
+                seq_load<T, V>(hr + c, hv); seq_load<T, V>(gr + c, gv);
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] = part[c + i];
+                finish(c, hv, gv, acc);
+#pragma unroll
+                for (int i = 0; i < V; ++i) part[c + i] = acc[i];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, h[k], g[k], dw[k]); }
+        }
+    }
+    if constexpr (!LOOP && LANES == 256) {
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            const int c = (k * LANES + lane) * V;
+            if (c < D)
+#pragma unroll
+                for (int i = 0; i < V; ++i) part[c + i] = dw[k][i];
+        }
+    } else if constexpr (!LOOP) {                                  // the workgroup's PER row groups, added in order
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s_dw[sub * (LANES * ITERS * V) + (k * LANES + lane) * V + i] = dw[k][i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < D; c += 256) {
+            float v = 0.f;
+#pragma unroll
+            for (int g = 0; g < PER; ++g) v += s_dw[g * (LANES * ITERS * V) + c];
+            part[c] = v;
+        }
+    }
+}
+
+static int norm_groups(int64_t rows) { return (int)(rows < 1 ? 1 : rows < 1024 ? rows : 1024); }
+
+template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static void norm_launch3(const NormArgs& a, int groups, hipStream_t st) {
+    constexpr int PER = 256 / LANES;
+    const dim3 grid((unsigned)((a.rows + PER - 1) / PER)), block(256);
+    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP, false>), grid, block, 0, st, a);
+    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP, true>), grid, block, 0, st, a);
+    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_bwd<T, V, LANES, ITERS, LOOP>), dim3(groups), block, 0, st, a);
+}
+// The fewest lanes that hold a row in four pieces each: rows of one wave need no LDS, and short rows share a wave.
+template <int WHAT, typename T, int V> static void norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
+    const int pieces = (a.channels + V - 1) / V;
+    if (pieces <= 16) norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
+    else if (pieces <= 32) norm_launch3<WHAT, T, V, 16, 2, false>(a, groups, st);
+    else if (pieces <= 64) norm_launch3<WHAT, T, V, 64, 1, false>(a, groups, st);
+    else if (pieces <= 128) norm_launch3<WHAT, T, V, 64, 2, false>(a, groups, st);
+    else if (pieces <= 256) norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st);
+    else if (pieces <= 512) norm_launch3<WHAT, T, V, 256, 2, false>(a, groups, st);
+    else if (pieces <= 1024) norm_launch3<WHAT, T, V, 256, 4, false>(a, groups, st);
+    else norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
+}
+template <int WHAT, typename T> static void norm_launch1(const NormArgs& a, bool vec, int groups, hipStream_t st) {
+    constexpr int N = SeqVec<T>::n;
+    if (vec && a.channels % N == 0) norm_launch2<WHAT, T, N>(a, groups, st); else norm_launch2<WHAT, T, 1>(a, groups, st);
+}
+template <int WHAT> static int norm_launch(const NormArgs& a, int dtype, bool vec, int groups, hipStream_t st) {
+    if (dtype == SEQ_F32) norm_launch1<WHAT, float>(a, vec, groups, st);
+    else if (dtype == SEQ_BF16) norm_launch1<WHAT, __bf16>(a, vec, groups, st);
+    else norm_launch1<WHAT, _Float16>(a, vec, groups, st);
+    return evad_last_error();
+}
+static bool norm_shape_ok(int64_t rows, int channels, int dtype) {
+    return rows >= 0 && rows <= 0x7fffff00 && channels >= 1 && channels <= (1 << 24) && dtype >= 0 && dtype <= 2;
+}
+
+extern "C" int eventad_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, void* sum, int64_t lds,
+                                    void* y, int64_t ldy, int64_t rows, int channels, float eps, int dtype, void* stream) {
+    if (!norm_shape_ok(rows, channels, dtype) || !w || !(eps >= 0.f) ||
+        (rows && (!x || !y || ldx < channels || ldy < channels || (residual && (!sum || ldr < channels || lds < channels))))) return EVAD_ERR_ARG;
+    if (!rows) return EVAD_OK;
+    NormArgs a = {};
+    a.x = x; a.ldx = ldx; a.res = residual; a.ldr = ldr; a.w = w; a.sum = sum; a.lds = lds; a.y = y; a.ldy = ldy; a.rows = rows; a.channels = channels; a.eps = eps;
+    const int e = dtype == SEQ_F32 ? 4 : 2;
+    const bool vec = seq_aligned(x, ldx * e) && seq_aligned(y, ldy * e) && (!residual || (seq_aligned(residual, ldr * e) && seq_aligned(sum, lds * e)));
+    return norm_launch<0>(a, dtype, vec, 0, (hipStream_t)stream);
+}
+
+extern "C" int eventad_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, void* sum, int64_t lds,
+                                    uint8_t* q, int64_t ldq, float* scale, int64_t rows, int channels, float eps, int dtype, void* stream) {
+    if (!norm_shape_ok(rows, channels, dtype) || !w || !(eps >= 0.f) ||
+        (rows && (!x || !q || !scale || ldx < channels || ldq < channels || (residual && (!sum || ldr < channels || lds < channels))))) return EVAD_ERR_ARG;
+    if (!rows) return EVAD_OK;
+    NormArgs a = {};
+    a.x = x; a.ldx = ldx; a.res = residual; a.ldr = ldr; a.w = w; a.sum = sum; a.lds = lds; a.q = q; a.ldq = ldq; a.scale = scale;
+    a.rows = rows; a.channels = channels; a.eps = eps;
+    const int e = dtype == SEQ_F32 ? 4 : 2;
+    const bool vec = seq_aligned(x, ldx * e) && (!residual || (seq_aligned(residual, ldr * e) && seq_aligned(sum, lds * e))) &&
+                     ((((uintptr_t)q | (uintptr_t)ldq) & 7) == 0);
+    return norm_launch<1>(a, dtype, vec, 0, (hipStream_t)stream);
+}
+
+extern "C" int eventad_rms_norm_workspace(int64_t rows, int channels, int64_t* bytes) {
+    if (!bytes || !norm_shape_ok(rows, channels, 0)) return EVAD_ERR_ARG;
+    *bytes = ((int64_t)norm_groups(rows) + SEQ_SUM_PARTS) * channels * 4;
+    return EVAD_OK;
+}
+
+extern "C" int eventad_rms_norm_bwd(const void* sum, int64_t lds, const float* w, const void* dy, int64_t lddy, const void* dsum, int64_t ldds,
+                                    void* dh, int64_t lddh, float* dw, void* workspace, int64_t workspace_bytes, int64_t rows, int channels,
+                                    float eps, int dtype, void* stream) {
+    int64_t need = 0;
+    if (!norm_shape_ok(rows, channels, dtype) || !w || !(eps >= 0.f) || !dw || eventad_rms_norm_workspace(rows, channels, &need) != EVAD_OK ||
+        !workspace || workspace_bytes < need ||
+        (rows && (!sum || !dy || !dh || lds < channels || lddy < channels || lddh < channels || (dsum && ldds < channels)))) return EVAD_ERR_ARG;
+    NormArgs a = {};
+    a.sum = (void*)sum; a.lds = lds; a.w = w; a.dy = dy; a.lddy = lddy; a.dsum = dsum; a.ldds = ldds; a.dh = dh; a.lddh = lddh;
+    a.part = (float*)workspace; a.rows = rows; a.channels = channels; a.eps = eps;
+    const int e = dtype == SEQ_F32 ? 4 : 2;
+    const bool vec = seq_aligned(sum, lds * e) && seq_aligned(dy, lddy * e) && seq_aligned(dh, lddh * e) && (!dsum || seq_aligned(dsum, ldds * e));
+    const int groups = norm_groups(rows);
+    const int rc = norm_launch<2>(a, dtype, vec, groups, (hipStream_t)stream);
+    if (rc) return rc;
+    return seq_colsum(a.part, groups, channels, dw, a.part + (int64_t)groups * channels, (hipStream_t)stream);
+}

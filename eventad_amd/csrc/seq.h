@@ -1,0 +1,71 @@
+// eventad_amd/csrc/seq.h -- shared by the sequence operators (seqconv.hip, seqscan.hip, rmsnorm.hip): element types, clip
+// offsets, column sums.
+//
+// Rows of a [rows, channels] array are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1 (i32[clips+1], not
+// decreasing, inside 0..rows); rows in front of the first and behind the last clip belong to none.  Without an array all
+// rows are one clip.  The offsets are read on the device only, so no call waits for the GPU and every launch can be
+// captured; whatever they hold, they are only compared with row numbers that the launch made itself, so wrong offsets give
+// wrong numbers, never an access outside an array.
+#pragma once
+#include "common.h"
+
+#define SEQ_F32 0
+#define SEQ_BF16 1
+#define SEQ_F16 2
+
+typedef float seq_f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 seq_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 seq_b8 __attribute__((ext_vector_type(8)));
+
+// what one 16-byte access of a type holds
+template <typename T> struct SeqVec;
+template <> struct SeqVec<float> { typedef seq_f4 type; static constexpr int n = 4; };
+template <> struct SeqVec<_Float16> { typedef seq_h8 type; static constexpr int n = 8; };
+template <> struct SeqVec<__bf16> { typedef seq_b8 type; static constexpr int n = 8; };
+
+// V elements at p as floats / back, rounded to nearest even: one 16-byte access, or (V = 1) one element
+template <typename T, int V> __device__ __forceinline__ void seq_load(const T* __restrict__ p, float (&out)[V]) {
+    if constexpr (V == 1) out[0] = (float)*p;
+    else {
+        static_assert(V == SeqVec<T>::n, "one 16-byte access");
+        const typename SeqVec<T>::type v = *(const typename SeqVec<T>::type*)p;
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = (float)v[i];
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void seq_store(T* __restrict__ p, const float (&in)[V]) {
+    if constexpr (V == 1) *p = (T)in[0];
+    else {
+        typename SeqVec<T>::type v;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (T)in[i];
+        *(typename SeqVec<T>::type*)p = v;
+    }
+}
+
+#define SEQ_LOG2E 1.4426950408889634f
+#define SEQ_LN2 0.6931471805599453f
+
+__device__ __forceinline__ float seq_exp2(float x) { return __builtin_amdgcn_exp2f(x); }          // v_exp_f32, 1 ulp
+__device__ __forceinline__ float seq_rcp(float x) { return __builtin_amdgcn_rcpf(x); }            // v_rcp_f32, 1 ulp
+__device__ __forceinline__ float seq_sigmoid(float x) { return seq_rcp(1.f + seq_exp2(-SEQ_LOG2E * x)); }
+
+struct SeqClips { const int* start; int n; int rows; };        // start == nullptr: one clip of all rows
+
+__device__ __forceinline__ int seq_start(const SeqClips& c, int s) { return c.start ? c.start[s] : (s ? c.rows : 0); }
+
+// the last s in 0..n with start[s] <= row, or -1: the clip of the row (n: behind the last clip), empty clips skipped
+__device__ __forceinline__ int seq_find(const SeqClips& c, int row) {
+    int lo = -1, hi = c.n + 1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (seq_start(c, mid) <= row) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+static inline bool seq_aligned(const void* p, int64_t row_bytes) { return (((uintptr_t)p | (uintptr_t)row_bytes) & 15) == 0; }
+
+// ---- column sums: out[c] = sum over rows of in[rows][cols], in a fixed order.  `scratch` holds SEQ_SUM_PARTS x cols floats.
+#define SEQ_SUM_PARTS 64
+int seq_colsum(const float* in, int64_t rows, int64_t cols, float* out, float* scratch, hipStream_t st);

@@ -504,6 +504,77 @@ int eventad_incr_pool0(const float* y2, const float* map_nhwc, int map_h, int ma
                        const int32_t* deg, int n_first, int k, int W, int H, float* feat, uint64_t* sums, double* tsum,
                        uint32_t* cnt, int32_t* maxidx, uint32_t* bitmap, uint32_t* counters, void* stream);
 
+/* ---- (L) sequence operators over packed clips (no counterpart in the reference, whose temporal part is the head's GRU) ----- */
+/* A causal convolution, a selective state-space scan and a root-mean-square norm: what a state-space block over a clip's
+ * events or nodes needs beside its matrix products, each with its gradient and its form for one token per clip (the dense
+ * pass and the event-by-event update of groups (B)-(K), for a recurrence over the rows themselves).
+ * Arrays of activations are [rows, channels] with a row stride in elements (ld* >= channels; adjacent channels are adjacent
+ * in memory), of type dtype = 0 float32, 1 bfloat16, 2 float16, all of one call alike; parameters and scan states are
+ * float32, sums are formed in float32.  Rows are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1, clip_start
+ * i32[clips+1] on the device, not decreasing, within 0..rows (NULL with clips = 1: all rows are one clip).  Rows of no
+ * clip are neither read into a result nor counted in a gradient; their outputs and gradients are written as zeros.
+ * Outputs must not overlap inputs unless it says so.  Results are reproducible bit for bit (no float atomics).
+ * workspace: 16-byte aligned device memory of at least the bytes that the *_workspace function of the same shape reports
+ * (host call, nothing is launched); its contents need not survive the call, and calls that may run at the same time need
+ * one each.
+ *
+ * y_t = act(bias + sum_k w[:,k] x_{t-(taps-1)+k}) per channel, w f32[channels,taps], bias f32[channels] (nullable), taps
+ * 1..8, act 0 = none, 1 = x sigmoid(x).  state [clips,taps-1,channels] of type dtype (nullable = zeros) holds the inputs in
+ * front of each clip's first row, oldest first; final_state (nullable) receives the last taps-1 of state ++ rows. */
+int eventad_causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bias, const int32_t* clip_start, int clips,
+                            const void* state, void* final_state, void* y, int64_t ldy, int64_t rows, int channels, int taps,
+                            int act, int dtype, void* stream);
+int eventad_causal_conv_workspace(int64_t rows, int channels, int taps, int64_t* bytes);
+/* Its gradient from dy and dfinal (gradient of final_state, nullable): dx, dstate (nullable), dparams f32[channels*taps
+ * (as w) + channels (bias)]. */
+int eventad_causal_conv_bwd(const void* x, int64_t ldx, const float* w, const float* bias, const int32_t* clip_start, int clips,
+                            const void* state, const void* dy, int64_t lddy, const void* dfinal, void* dx, int64_t lddx,
+                            void* dstate, float* dparams, void* workspace, int64_t workspace_bytes, int64_t rows, int channels,
+                            int taps, int act, int dtype, void* stream);
+/* One row per clip: x, y [clips,channels]; state_out = the state moved on by the row (it may be `state` itself). */
+int eventad_causal_conv_step(const void* x, int64_t ldx, const float* w, const float* bias, const void* state, void* state_out,
+                             void* y, int64_t ldy, int clips, int channels, int taps, int act, int dtype, void* stream);
+/* s_t = delta_t + delta_bias, through log(1 + exp(.)) if softplus = 1;  h_t = exp(s_t A) h_{t-1} + s_t u_t B_t;
+ * y_t = (sum_n C_t[n] h_t[n] + D u_t) * (z ? z_t sigmoid(z_t) : 1).  u, delta, z, y [rows,channels], B, C [rows,n_state]
+ * (ldb, ldc >= n_state), A f32[channels,n_state], D, delta_bias f32[channels], n_state 1..64; z, D, delta_bias nullable.
+ * state / final_state f32[clips,channels,n_state] (nullable): h in front of each clip's first row / behind its last.
+ * checkpoint (nullable, 16-byte aligned): eventad_selective_scan_checkpoint() bytes that the gradient of this call reads. */
+int eventad_selective_scan_workspace(int64_t rows, int channels, int n_state, int backward, int64_t* bytes);
+int eventad_selective_scan_checkpoint(int64_t rows, int channels, int n_state, int64_t* bytes);
+int eventad_selective_scan_fwd(const void* u, int64_t ldu, const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb,
+                               const void* C, int64_t ldc, const float* D, const void* z, int64_t ldz, const float* delta_bias,
+                               const int32_t* clip_start, int clips, const float* state, float* final_state, void* y, int64_t ldy,
+                               float* checkpoint, void* workspace, int64_t workspace_bytes, int64_t rows, int channels, int n_state,
+                               int softplus, int dtype, void* stream);
+/* Its gradient from dy and dfinal (gradient of final_state, nullable), with the inputs and the checkpoint of the forward call:
+ * du, ddelta, dB, dC, dz (if z), dstate (nullable), dparams f32[channels*n_state (A) + channels (D) + channels (delta_bias)]. */
+int eventad_selective_scan_bwd(const void* u, int64_t ldu, const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb,
+                               const void* C, int64_t ldc, const float* D, const void* z, int64_t ldz, const float* delta_bias,
+                               const int32_t* clip_start, int clips, const float* state, const float* checkpoint, const void* dy,
+                               int64_t lddy, const float* dfinal, void* du, int64_t lddu, void* ddelta, int64_t lddd, void* dB,
+                               int64_t lddb, void* dC, int64_t lddc, void* dz, int64_t lddz, float* dstate, float* dparams,
+                               void* workspace, int64_t workspace_bytes, int64_t rows, int channels, int n_state, int softplus,
+                               int dtype, void* stream);
+/* One row per clip: state f32[clips,channels,n_state] -> state_out (it may be `state` itself), y [clips,channels]. */
+int eventad_selective_scan_step(const void* u, int64_t ldu, const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb,
+                                const void* C, int64_t ldc, const float* D, const void* z, int64_t ldz, const float* delta_bias,
+                                const float* state, float* state_out, void* y, int64_t ldy, int clips, int channels, int n_state,
+                                int softplus, int dtype, void* stream);
+/* sum = x + residual, rounded to dtype (residual NULL: sum is not written and x takes its place);
+ * y = sum / sqrt(mean(sum^2) + eps) * w over the channels of a row, w f32[channels]. */
+int eventad_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, void* sum, int64_t lds,
+                         void* y, int64_t ldy, int64_t rows, int channels, float eps, int dtype, void* stream);
+/* The same row y as 8-bit values (e4m3: 3 fraction bits, largest 448): scale[row] = max|y| / 448 (1 for a row of zeros),
+ * q = y / scale rounded to nearest even.  q u8[rows,channels] with row stride ldq, scale f32[rows]. */
+int eventad_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, void* sum, int64_t lds,
+                         uint8_t* q, int64_t ldq, float* scale, int64_t rows, int channels, float eps, int dtype, void* stream);
+int eventad_rms_norm_workspace(int64_t rows, int channels, int64_t* bytes);
+/* Gradient of eventad_rms_norm_fwd: dh = gradient of x and of residual (dsum, nullable: gradient that reaches sum from
+ * elsewhere, added), dw f32[channels].  `sum` is the forward's sum (or x, without a residual). */
+int eventad_rms_norm_bwd(const void* sum, int64_t lds, const float* w, const void* dy, int64_t lddy, const void* dsum, int64_t ldds,
+                         void* dh, int64_t lddh, float* dw, void* workspace, int64_t workspace_bytes, int64_t rows, int channels,
+                         float eps, int dtype, void* stream);
+
 /* ---- (J) streams restricted to a CU set (no counterpart in the reference) ------------------------------------------ */
 /* A default-priority HIP stream whose kernels may only use the CUs whose bit is set in mask (u32[words], bit i = CU i).
  * TrainStep uses a pair of them with disjoint masks for the backbone graph and the head graph. */

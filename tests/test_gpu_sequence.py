@@ -1,0 +1,578 @@
+"""The sequence operators (eventad_amd/sequence.py) against their float64 restatement (oracle/sequence_ref.py).
+
+Tolerances: an output is rounded to its type once, half a step (finfo.eps / 2 relative to the value, 2^-25 absolute for
+float16's subnormals), and float32 arithmetic in front of that may be off by the restatement's bound in units of 2^-24."""
+import pytest
+import torch
+
+from oracle import sequence_ref as R
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+UNIT = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def S():
+    from eventad_amd import sequence
+    return sequence
+
+
+def close(name, got, want, units):
+    """got within half a step of its type plus units x 2^-24 of want (both tensors, float64 on the CPU)."""
+    g = got.detach().double().cpu()
+    assert g.shape == want.shape, (name, g.shape, want.shape)
+    tol = torch.finfo(got.dtype).eps / 2 * want.abs() * (1 + 2.0 ** -7) + 1.01 * UNIT * units
+    if got.dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    if got.dtype == torch.float32:
+        tol = tol + 1e-37                                        # (subnormal results are flushed)
+    over = (g - want).abs() - tol
+    assert bool((over <= 0).all()), "%s: %d of %d entries off, worst by %.3g at %s: got %r want %r" % (
+        name, int((~(over <= 0)).sum()), over.numel(), float(over.max()), int(over.argmax()), float(g.reshape(-1)[int(over.argmax())]),
+        float(want.reshape(-1)[int(over.argmax())]))
+
+
+def rnd(gen, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=gen) * scale).to(dtype).cuda()
+
+
+def starts_of(bounds):
+    return None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device="cuda")
+
+
+def leaf(t):
+    return None if t is None else t.clone().requires_grad_()
+
+
+# clip bounds by name; the last entry may be short of the rows (rows behind the last clip), the first above 0
+def bounds_of(kind, rows):
+    return {"one": None, "all": [0, rows], "three": [0, rows // 3, rows // 2, rows], "empties": [0, 0, 0, rows // 2, rows // 2, rows, rows],
+            "gaps": [min(2, rows), rows // 2, rows // 2, max(min(2, rows), rows - 3)], "singles": list(range(rows + 1)),
+            "tiles": sorted({0, min(16, rows), min(63, rows), min(64, rows), min(65, rows), min(128, rows), rows})}[kind]
+
+
+# ---------------------------------------------------------------------------------------------------- causal convolution
+def conv_units(K, rows):
+    return K + 16, K + 16 + rows                                 # per row: K products and the activation; sums over the rows
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,channels,taps,kind,silu,state,bias", [
+    (1, 1, 1, "one", True, False, True), (1, 8, 4, "all", True, True, True), (2, 16, 4, "singles", True, True, True),
+    (33, 8, 4, "three", True, True, True), (70, 24, 3, "empties", False, True, False), (131, 40, 4, "tiles", True, False, True),
+    (64, 7, 2, "gaps", True, True, True), (97, 16, 8, "three", True, True, False), (40, 5, 6, "singles", False, True, True),
+    (200, 64, 5, "tiles", True, True, True), (65, 16, 7, "gaps", True, False, True), (32, 8, 1, "empties", True, True, True)])
+def test_causal_conv_and_gradient(S, dtype, rows, channels, taps, kind, silu, state, bias):
+    gen, dt = torch.Generator().manual_seed(rows * 31 + channels), DTYPES[dtype]
+    b = bounds_of(kind, rows)
+    clips = 1 if b is None else len(b) - 1
+    x, w = rnd(gen, rows, channels, dtype=dt), rnd(gen, channels, taps)
+    bs = rnd(gen, channels) if bias else None
+    st = rnd(gen, clips, taps - 1, channels, dtype=dt) if state else None
+    dy, df = rnd(gen, rows, channels, dtype=dt), rnd(gen, clips, taps - 1, channels, dtype=dt)
+    act = "silu" if silu else None
+    want = R.conv(x, w, bs, b, st, silu, dy, df)
+    row_units, sum_units = conv_units(taps, rows)
+    with torch.no_grad():
+        y, final = S.causal_conv(x, w, bs, starts_of(b), st, act, True)
+        assert torch.equal(y, S.causal_conv(x, w, bs, starts_of(b), st, act))
+    close("y", y, want["y"][0], row_units * want["y"][1])
+    assert torch.equal(final.double().cpu(), want["final"][0])    # copies
+    L = [leaf(t) for t in (x, w, bs, st)]
+    y2, f2 = S.causal_conv(L[0], L[1], L[2], starts_of(b), L[3], act, True)
+    assert torch.equal(y2, y) and torch.equal(f2, final)
+    grads = torch.autograd.grad([y2, f2], [t for t in L if t is not None], [dy, df])
+    names = [k for k, t in zip(("x", "weight", "bias", "state"), L) if t is not None]
+    for k, g in zip(names, grads):
+        close("d" + k, g, want[k][0], (sum_units if k in ("weight", "bias") else row_units + taps) * want[k][1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("clips,channels,taps", [(1, 1, 1), (1, 8, 4), (6, 256, 4), (5, 13, 3), (33, 40, 8), (3, 16, 2)])
+def test_causal_conv_step(S, dtype, clips, channels, taps):
+    gen, dt = torch.Generator().manual_seed(clips), DTYPES[dtype]
+    x, w, bs, st = rnd(gen, clips, channels, dtype=dt), rnd(gen, channels, taps), rnd(gen, channels), rnd(gen, clips, taps - 1, channels, dtype=dt)
+    want = R.conv(x, w, bs, list(range(clips + 1)), st, True)
+    kept, out = st.clone(), torch.empty_like(st)
+    y = S.causal_conv_step(x, w, st, bs, state_out=out)
+    assert torch.equal(st, kept)
+    close("y", y, want["y"][0], (taps + 16) * want["y"][1])
+    assert torch.equal(out.double().cpu(), want["final"][0])
+    assert torch.equal(S.causal_conv_step(x, w, st, bs), y) and torch.equal(st, out)          # in place
+
+
+# -------------------------------------------------------------------------------------------------------- selective scan
+def scan_inputs(gen, rows, channels, N, dt, clips, D=True, z=True, bias=True, state=True, decay=1.0):
+    return dict(u=rnd(gen, rows, channels, dtype=dt), delta=rnd(gen, rows, channels, dtype=dt),
+                A=-torch.exp(rnd(gen, channels, N)) * decay, B=rnd(gen, rows, N, dtype=dt), C=rnd(gen, rows, N, dtype=dt),
+                D=rnd(gen, channels) if D else None, z=rnd(gen, rows, channels, dtype=dt) if z else None,
+                delta_bias=rnd(gen, channels) - 2.0 if bias else None, state=rnd(gen, clips, channels, N) if state else None)
+
+
+SCAN_CASES = [  # rows, channels, states, clips, softplus, which of D z bias state
+    (1, 1, 1, "one", True, "Dzbs"), (1, 3, 16, "all", True, "Dzbs"), (5, 16, 4, "singles", True, "zbs"), (15, 17, 16, "three", True, "Dbs"),
+    (16, 64, 16, "gaps", True, "Dzb"), (17, 70, 5, "empties", True, "Dzbs"), (64, 20, 16, "one", True, "Dzbs"), (65, 66, 16, "tiles", True, "Dzbs"),
+    (200, 33, 16, "tiles", True, "Dzbs"), (200, 65, 16, "all", True, "zb"), (197, 16, 13, "empties", True, "Dzbs"), (150, 9, 24, "three", True, "Dzbs"),
+    (130, 40, 32, "tiles", True, "Dzb"), (131, 18, 64, "three", True, "Dzbs"), (66, 5, 33, "gaps", True, "s"), (140, 12, 16, "gaps", True, ""),
+    (90, 8, 8, "all", False, "Dzs"), (260, 4, 1, "one", True, "Dzbs")]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,channels,N,kind,softplus,given", SCAN_CASES)
+def test_selective_scan_and_gradient(S, dtype, rows, channels, N, kind, softplus, given):
+    gen, dt = torch.Generator().manual_seed(rows * 17 + channels * 3 + N), DTYPES[dtype]
+    b = bounds_of(kind, rows)
+    clips = 1 if b is None else len(b) - 1
+    a = scan_inputs(gen, rows, channels, N, dt, clips, "D" in given, "z" in given, "b" in given, "s" in given)
+    if not softplus:
+        a["delta"] = (a["delta"].abs() * 0.3).to(dt)
+    dy, df = rnd(gen, rows, channels, dtype=dt), rnd(gen, clips, channels, N)
+    want = R.scan(softplus=softplus, clip_start=b, dy=dy, dfinal=df, **a)
+    with torch.no_grad():
+        y, final = S.selective_scan(delta_softplus=softplus, clip_start=starts_of(b), return_state=True, **a)
+        assert torch.equal(y, S.selective_scan(delta_softplus=softplus, clip_start=starts_of(b), **a))
+    close("y", y, *want["y"])
+    close("final", final, *want["final"])
+    L = {k: leaf(t) for k, t in a.items()}
+    y2, f2 = S.selective_scan(delta_softplus=softplus, clip_start=starts_of(b), return_state=True, **L)
+    assert torch.equal(y2, y) and torch.equal(f2, final)
+    have = [k for k, t in L.items() if t is not None]
+    first = torch.autograd.grad([y2, f2], [L[k] for k in have], [dy, df], retain_graph=True)
+    for k, g in zip(have, first):
+        close("d" + k, g, *want[k])
+    for g, again in zip(first, torch.autograd.grad([y2, f2], [L[k] for k in have], [dy, df])):
+        assert torch.equal(g, again)                             # reproducible bit for bit
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("clips,channels,N", [(1, 1, 1), (6, 256, 16), (5, 13, 5), (3, 33, 24), (2, 7, 64), (17, 20, 8)])
+def test_selective_scan_step(S, dtype, clips, channels, N):
+    gen, dt = torch.Generator().manual_seed(clips + N), DTYPES[dtype]
+    a = scan_inputs(gen, clips, channels, N, dt, clips)
+    want = R.scan(clip_start=list(range(clips + 1)), **a)
+    st = a.pop("state")
+    kept, out = st.clone(), torch.empty_like(st)
+    y = S.selective_scan_step(state=st, state_out=out, **a)
+    assert torch.equal(st, kept)
+    close("y", y, *want["y"])
+    close("state", out, *want["final"])
+    assert torch.equal(S.selective_scan_step(state=st, **a), y) and torch.equal(st, out)       # in place
+
+
+def test_scan_extreme_steps_and_decays(S):
+    """Steps from underflow to saturation of softplus, decays that vanish in one row, states that never decay (A = 0)."""
+    gen = torch.Generator().manual_seed(3)
+    rows, ch, N = 80, 6, 16
+    a = scan_inputs(gen, rows, ch, N, torch.float32, 1)
+    a["delta"] = torch.linspace(-90.0, 40.0, rows * ch).view(rows, ch)[torch.randperm(rows, generator=gen)].contiguous().cuda()
+    a["A"][:, 0] = 0.0
+    a["A"][:, 1] = -1e4
+    dy = rnd(gen, rows, ch)
+    want = R.scan(dy=dy, **a)
+    L = {k: leaf(t) for k, t in a.items()}
+    y = S.selective_scan(**L)
+    close("y", y, *want["y"])
+    for k, g in zip(L, torch.autograd.grad(y, list(L.values()), dy)):
+        close("d" + k, g, *want[k])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 1e30])
+def test_rows_of_no_clip_are_not_looked_at(S, value):
+    """Whatever stands in rows in front of the first and behind the last clip: zeros come out, and no gradient sees them."""
+    gen = torch.Generator().manual_seed(4)
+    rows, ch, N, b = 90, 20, 16, [5, 40, 70]
+    a = scan_inputs(gen, rows, ch, N, torch.float32, 2)
+    x, w, bs = rnd(gen, rows, ch), rnd(gen, ch, 4), rnd(gen, ch)
+    dy = rnd(gen, rows, ch)
+    dead = torch.ones(rows, dtype=torch.bool)
+    dead[5:70] = False
+    dead = dead.cuda()
+    results = []
+    for fill in (0.0, value):
+        t = {k: (v.clone() if v is not None else None) for k, v in a.items()}
+        for k in ("u", "delta", "B", "C", "z"):
+            t[k][dead] = fill
+        xx, g = x.clone(), dy.clone()
+        xx[dead], g[dead] = fill, fill
+        L = {k: leaf(v) for k, v in t.items()}
+        y, f = S.selective_scan(clip_start=starts_of(b), return_state=True, **L)
+        C = [leaf(v) for v in (xx, w, bs)]
+        yc = S.causal_conv(C[0], C[1], C[2], starts_of(b))
+        r = [y, f, yc] + list(torch.autograd.grad(y, list(L.values()), g)) + list(torch.autograd.grad(yc, C, g))
+        results.append(r)
+        assert bool((y[dead] == 0).all()) and bool((yc[dead] == 0).all())
+    for p, q in zip(*results):
+        assert torch.equal(p, q)
+
+
+def test_no_rows_and_only_empty_clips(S):
+    st, cs = torch.randn(3, 4, 16, device="cuda"), torch.randn(3, 2, 4, device="cuda")
+    e = lambda n: torch.empty(0, n, device="cuda")
+    b = starts_of([0, 0, 0, 0])
+    L = [leaf(t) for t in (e(4), e(4), -torch.ones(4, 16, device="cuda"), e(16), e(16), st)]
+    y, f = S.selective_scan(*L[:5], clip_start=b, state=L[5], return_state=True)
+    assert y.shape == (0, 4) and torch.equal(f, st)
+    g = torch.autograd.grad(f, L, st, allow_unused=True)
+    assert torch.equal(g[5], st) and bool((g[2] == 0).all())
+    C = [leaf(t) for t in (e(4), torch.ones(4, 3, device="cuda"), cs)]
+    y, f = S.causal_conv(C[0], C[1], clip_start=b, state=C[2], return_state=True)
+    assert y.shape == (0, 4) and torch.equal(f, cs)
+    g = torch.autograd.grad(f, C, cs)
+    assert torch.equal(g[2], cs) and bool((g[1] == 0).all())
+    n = [leaf(e(4)), leaf(torch.ones(4, device="cuda"))]
+    y = S.rms_norm(*n)
+    assert y.shape == (0, 4) and bool((torch.autograd.grad(y, n, y)[1] == 0).all())
+    q, s = S.rms_norm_fp8(e(4), torch.ones(4, device="cuda"))
+    assert q.shape == (0, 4) and s.shape == (0,)
+    assert S.causal_conv_step(e(4), torch.ones(4, 3, device="cuda"), torch.empty(0, 2, 4, device="cuda")).shape == (0, 4)
+    assert S.selective_scan_step(e(4), e(4), -torch.ones(4, 16, device="cuda"), e(16), e(16), torch.empty(0, 4, 16, device="cuda")).shape == (0, 4)
+
+
+# ------------------------------------------------------------------------------------------------------------- RMS norm
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,channels,residual", [(1, 1, True), (3, 7, True), (6, 256, True), (5, 128, False), (37, 64, True), (2, 1000, True),
+                                                    (9, 2048, True), (3, 4104, True), (3, 5000, True), (2, 8192, False), (2, 9000, True), (2, 1027, True),
+                                                    (1100, 24, True), (1, 20001, True)])
+def test_rms_norm_and_gradient(S, dtype, rows, channels, residual):
+    gen, dt = torch.Generator().manual_seed(rows + channels), DTYPES[dtype]
+    x, w = rnd(gen, rows, channels, dtype=dt), rnd(gen, channels) + 1.0
+    res = rnd(gen, rows, channels, dtype=dt, scale=2.0) if residual else None
+    dy, ds = rnd(gen, rows, channels, dtype=dt), rnd(gen, rows, channels, dtype=dt)
+    want = R.norm(x.cpu(), w, None if res is None else res.cpu(), 1e-5, dy, ds if residual else None)
+    units = 2 * (channels / 16 + 24)                             # additions in sequence of a sum over the row
+    with torch.no_grad():
+        r = S.rms_norm(x, w, res, 1e-5)
+    y, total = r if residual else (r, None)
+    close("y", y, want["y"][0], units * want["y"][1])
+    if residual:
+        assert torch.equal(total.double().cpu(), want["sum"][0])
+    L = [leaf(x), leaf(w), leaf(res)]
+    r = S.rms_norm(L[0], L[1], L[2], 1e-5)
+    outs = list(r) if residual else [r]
+    grads = torch.autograd.grad(outs, [t for t in L if t is not None], [dy, ds][:len(outs)])
+    close("dx", grads[0], want["h"][0], units * want["h"][1])
+    close("dweight", grads[1], want["weight"][0], (units + rows) * want["weight"][1])
+    if residual:
+        assert torch.equal(grads[2], grads[0])
+        only = torch.autograd.grad(S.rms_norm(L[0], L[1], L[2], 1e-5)[1], L[2], ds)[0]         # only the sum is used
+        assert torch.equal(only, ds)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,channels,residual", [(1, 1, True), (3, 7, True), (6, 256, True), (37, 64, False), (9, 2048, True), (3, 4104, True), (2, 9000, True),
+                                                    (3, 1030, True)])
+def test_rms_norm_fp8_is_the_nearest_value(S, dtype, rows, channels, residual):
+    gen, dt = torch.Generator().manual_seed(rows + channels), DTYPES[dtype]
+    x, w = rnd(gen, rows, channels, dtype=dt), rnd(gen, channels)
+    res = rnd(gen, rows, channels, dtype=dt) if residual else None
+    x[0] = 0.0                                                   # a row of zeros (with a residual: of the residual alone)
+    if res is not None and rows > 1:
+        res[0] = 0.0
+    want = R.norm(x.cpu(), w, None if res is None else res.cpu(), 1e-6)
+    r = S.rms_norm_fp8(x, w, res)
+    assert r[0].dtype == torch.float8_e4m3fn and r[1].dtype == torch.float32
+    assert torch.equal(r[0].double().cpu(), want["q"])           # every value on the side the definition says
+    close("scale", r[1], want["scale"][0], (channels / 16 + 28) * want["scale"][0])
+    if residual:
+        assert torch.equal(r[2].double().cpu(), want["sum"][0])
+
+
+def test_rms_norm_fp8_keeps_nan(S):
+    x = torch.randn(4, 64, device="cuda")
+    x[1, 3] = float("nan")
+    q, s = S.rms_norm_fp8(x, torch.ones(64, device="cuda"))
+    assert bool(torch.isnan(s[1])) and bool(torch.isnan(q[1].float()).all())
+    assert not bool(torch.isnan(s[[0, 2, 3]]).any()) and not bool(torch.isnan(q[[0, 2, 3]].float()).any())
+
+
+# -------------------------------------------------------------------------------------------------- how they are called
+def block_weights(gen, D, E, N, K, rank):
+    return dict(norm=rnd(gen, D, scale=0.1) + 1.0, w_in=rnd(gen, D, 2 * E, scale=D ** -0.5), conv=rnd(gen, E, K, scale=K ** -0.5), conv_b=rnd(gen, E, scale=0.1),
+                w_x=rnd(gen, E, rank + 2 * N, scale=E ** -0.5), w_dt=rnd(gen, rank, E, scale=rank ** -0.5), dt_b=rnd(gen, E) - 2.0,
+                A=-torch.exp(rnd(gen, E, N)), D=rnd(gen, E), w_out=rnd(gen, E, D, scale=E ** -0.5))
+
+
+def block(S, p, x, res, starts=None, states=None, step=False):
+    """norm(+residual) -> projection -> convolution -> step sizes, B, C -> scan with its gate -> projection; the operators read
+    slices of the projections' outputs."""
+    N, E = p["A"].shape[1], p["A"].shape[0]
+    h, res = S.rms_norm(x, p["norm"], residual=res)
+    xz = h @ p["w_in"]
+    u, z = xz[:, :E], xz[:, E:]
+    if step:
+        u = S.causal_conv_step(u, p["conv"], states[0], p["conv_b"])
+    else:
+        u, cs = S.causal_conv(u, p["conv"], p["conv_b"], starts, None if states is None else states[0], return_state=True)
+    dbc = u @ p["w_x"]
+    rank = dbc.shape[1] - 2 * N
+    dt, Bm, Cm = dbc[:, :rank] @ p["w_dt"], dbc[:, rank:rank + N], dbc[:, rank + N:]
+    if step:
+        y, new = S.selective_scan_step(u, dt, p["A"], Bm, Cm, states[1], p["D"], z, p["dt_b"]), states
+    else:
+        y, ss = S.selective_scan(u, dt, p["A"], Bm, Cm, p["D"], z, p["dt_b"], True, starts, None if states is None else states[1], True)
+        new = [cs, ss]
+    return y @ p["w_out"], res, new
+
+
+def test_block_of_prompts_single_tokens_and_appended_rows_agree(S):
+    gen = torch.Generator().manual_seed(8)
+    D, E, N, K, rank, lens = 24, 40, 16, 4, 5, [37, 1, 80, 0, 20]
+    p = block_weights(gen, D, E, N, K, rank)
+    b = [0]
+    for n in lens:
+        b.append(b[-1] + n)
+    x, res = rnd(gen, b[-1], D), rnd(gen, b[-1], D)
+    with torch.no_grad():
+        whole, wres, wst = block(S, p, x, res, starts_of(b))
+        # each clip's first part as a prompt, the rest appended: by several rows at once, then row by row
+        cut = [n // 2 for n in lens]
+        idx = torch.cat([torch.arange(b[i], b[i] + cut[i]) for i in range(5)]).cuda()
+        cb = [0]
+        for n in cut:
+            cb.append(cb[-1] + n)
+        part, _, st = block(S, p, x[idx], res[idx], starts_of(cb))
+        rest = [n - c for n, c in zip(lens, cut)]
+        more = [max(0, r - 3) for r in rest]
+        idx2 = torch.cat([torch.arange(b[i] + cut[i], b[i] + cut[i] + more[i]) for i in range(5)]).cuda()
+        mb = [0]
+        for n in more:
+            mb.append(mb[-1] + n)
+        part2, _, st = block(S, p, x[idx2], res[idx2], starts_of(mb), st)
+        got = torch.empty_like(whole)
+        got[idx], got[idx2] = part, part2
+        for k in range(3):
+            live = [i for i in range(5) if cut[i] + more[i] + k < lens[i]]
+            rows = torch.tensor([b[i] + cut[i] + more[i] + k for i in live]).cuda()
+            sub = [s[live].contiguous() for s in st]
+            y, _, _ = block(S, p, x[rows], res[rows], states=sub, step=True)
+            got[rows] = y
+            for s, t in zip(st, sub):
+                s[live] = t
+    scale = float(whole.abs().max())
+    assert float((got - whole).abs().max()) < 1e-4 * scale       # different orders of float32 sums over <= 80 rows
+    for s, t in zip(st, wst):
+        assert float((s - t).abs().max()) < 1e-4 * float(t.abs().max())
+
+
+def test_block_gradients_against_differences(S):
+    gen = torch.Generator().manual_seed(9)
+    p = {k: leaf(v) for k, v in block_weights(gen, 12, 20, 16, 4, 3).items()}
+    x, res, b = rnd(gen, 50, 12), rnd(gen, 50, 12), [0, 20, 20, 47]
+    c1, c2 = rnd(gen, 50, 12), rnd(gen, 50, 12)
+    loss = lambda q: sum((o.double() * c.double()).sum() for o, c in zip(block(S, q, x, res, starts_of(b))[:2], (c1, c2)))
+    grads = torch.autograd.grad(loss(p), list(p.values()))
+    for (k, t), g in zip(p.items(), grads):
+        v = rnd(gen, *t.shape) * (t.detach().abs().mean() + 0.1)
+        with torch.no_grad():
+            q = {n: w.detach().clone() for n, w in p.items()}
+            q[k] = t.detach() + 1e-2 * v
+            up = loss(q)
+            q[k] = t.detach() - 1e-2 * v
+            slope = float(up - loss(q)) / 2e-2
+        want = float((g.double() * v.double()).sum())
+        # second-order differences of a smooth function at 1e-2 of the weights' size, and float32 losses divided by the step
+        assert abs(slope - want) < 2e-2 * (abs(want) + float((g.double() * v.double()).norm())) + 1e-3, (k, slope, want)
+
+
+def test_strides_orders_and_alignment(S):
+    """Slices of wider rows, rows that start off a 16-byte border, transposed and broadcast arrays give what copies give."""
+    gen = torch.Generator().manual_seed(10)
+    rows, ch, N, b = 70, 24, 16, [0, 30, 70]
+    for dt in DTYPES.values():
+        wide = rnd(gen, rows, 3 * ch + 2 * N + 5, dtype=dt)
+        for off in (0, 1, 8):
+            u, z, d = wide[:, off:off + ch], wide[:, off + ch:off + 2 * ch], wide[:, off + ch + 3:off + 2 * ch + 3]
+            Bm, Cm = wide[:, 2 * ch + off - 1 if off else 0:][:, :N], wide[:, 5:5 + N]
+            A, D = -torch.exp(rnd(gen, ch, N)), rnd(gen, ch)
+            view, flat = (u, d, A, Bm, Cm, D, z), tuple(t.contiguous().clone() for t in (u, d, A, Bm, Cm, D, z))
+            dy = rnd(gen, rows, 2 * ch, dtype=dt)[:, ch:]
+            outs = []
+            for t in (view, flat, tuple(v.t().contiguous().t() if v.dim() == 2 else v for v in flat)):
+                L = [v.detach().requires_grad_() for v in t]
+                y = S.selective_scan(*L, clip_start=starts_of(b))
+                outs.append([y] + list(torch.autograd.grad(y, L, dy)))
+            for o in outs[1:]:
+                for p, q in zip(outs[0], o):
+                    assert torch.equal(p, q)
+            w, res = rnd(gen, ch, 4), wide[:, 7:7 + ch]
+            outs = []
+            for xs, rs in ((u, res), (u.contiguous().clone(), res.contiguous().clone())):
+                L = [xs.detach().requires_grad_(), w.detach().requires_grad_(), rs.detach().requires_grad_(), D.detach().requires_grad_()]
+                y = S.causal_conv(L[0], L[1], clip_start=starts_of(b))
+                n, t = S.rms_norm(L[0], L[3], L[2])
+                q = S.rms_norm_fp8(xs, D, rs)
+                outs.append([y, n, t, q[0].float(), q[1]] + list(torch.autograd.grad(y, L[:2], dy)) + list(torch.autograd.grad([n, t], [L[0], L[3], L[2]], [dy, dy])))
+            # the 16-byte and the one-element form of the norm add a row in different orders
+            for i, (p, q) in enumerate(zip(*outs)):
+                p, q = p.detach(), q.detach()
+                if i in (0, 5) and dt == torch.float16:
+                    # the last fused multiply-add may be rounded to float16 at once or through float32: both are the rounding of
+                    # numbers 2^-24 apart, hence equal or neighbours, at most eps |q| apart (2^-24 among the subnormals)
+                    assert bool(((p.float() - q.float()).abs() <= torch.finfo(dt).eps * q.float().abs() + 2.0 ** -24).all()), i
+                elif i in (0, 2, 5, 6):
+                    assert torch.equal(p, q), i
+                else:
+                    assert float((p.float() - q.float()).abs().max()) <= 4 * torch.finfo(dt).eps * float(q.float().abs().max()), i
+        row = rnd(gen, 1, ch, dtype=dt).expand(rows, ch)         # one row for all
+        assert torch.equal(S.causal_conv(row, w, clip_start=starts_of(b)), S.causal_conv(row.contiguous(), w, clip_start=starts_of(b)))
+
+
+def test_captured_calls_replay_and_two_graphs_do_not_share(S):
+    gen = torch.Generator().manual_seed(11)
+    rows, ch, N = 200, 32, 16
+    bounds = [[0, 60, 60, 200], [3, 100, 130, 190]]
+    a = scan_inputs(gen, rows, ch, N, torch.float32, 3, state=False)
+    names = [k for k, t in a.items() if t is not None]
+    static = {k: a[k].clone() for k in names}
+    w, starts = rnd(gen, ch, 4), starts_of(bounds[0])
+    dy = rnd(gen, rows, ch)
+
+    def once():
+        L = {k: t.detach().requires_grad_() for k, t in static.items()}
+        u = S.causal_conv(L["u"], w, clip_start=starts)
+        n, t = S.rms_norm(u, L["D"], residual=L["u"])
+        y = S.selective_scan(n, L["delta"], L["A"], L["B"], L["C"], L["D"], L["z"], L["delta_bias"], clip_start=starts)
+        return [y, t] + list(torch.autograd.grad([y, t], [L[k] for k in names], [dy, dy]))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once()
+    side.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = once()
+        graphs.append((g, out))
+    for it in range(4):
+        for k in names:
+            static[k].copy_(a[k] * (1.0 + 0.1 * it))
+        starts.copy_(starts_of(bounds[it % 2]))
+        want = [t.clone() for t in once()]
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            for p, q in zip(out, want):
+                assert torch.equal(p, q), it
+
+
+def test_two_streams_at_once(S):
+    gen = torch.Generator().manual_seed(12)
+    sets = [scan_inputs(gen, 3000, 48, 16, torch.float32, 1) for _ in range(2)]
+    with torch.no_grad():
+        want = [S.selective_scan(return_state=True, **a) for a in sets]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in sets]
+        got = []
+        for _ in range(5):
+            for st, a in zip(streams, sets):
+                with torch.cuda.stream(st):
+                    got.append(S.selective_scan(return_state=True, **a))
+        torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g[0], want[i % 2][0]) and torch.equal(g[1], want[i % 2][1])
+
+
+def test_long_clip_against_float64_doubling(S):
+    """60001 rows in many chunks, three clips, few channels."""
+    gen = torch.Generator().manual_seed(13)
+    rows, ch, N, b = 60001, 8, 16, [0, 20000, 20017, 60001]
+    a = scan_inputs(gen, rows, ch, N, torch.float32, 3, decay=0.2)
+    a["delta_bias"] -= 3.0
+    dy = rnd(gen, rows, ch)
+    L = {k: leaf(t) for k, t in a.items()}
+    y, f = S.selective_scan(clip_start=starts_of(b), return_state=True, **L)
+    got = dict(zip(L, torch.autograd.grad(y, list(L.values()), dy)))
+    u, A, B, C, z = (a[k].double() for k in ("u", "A", "B", "C", "z"))
+    raw = a["delta"].double() + a["delta_bias"].double()
+    s = torch.nn.functional.softplus(raw)
+
+    def doubled(p, q):
+        d = 1
+        while d < rows:
+            q = torch.cat([q[:d], q[d:] + p[d:] * q[:-d]])
+            p = torch.cat([p[:d], p[d:] * p[:-d]])
+            d *= 2
+        return q
+    p, q = torch.exp(s[:, :, None] * A), (s * u)[:, :, None] * B[:, None]
+    for i in range(3):
+        q[b[i]] += p[b[i]] * a["state"][i].double()
+    chain = p.clone()
+    chain[torch.tensor(b[:3]).cuda()] = 0.0
+    h = doubled(chain, q)
+    gate = torch.nn.functional.silu(z)
+    pre = (h * C[:, None]).sum(2) + a["D"].double() * u
+    d = dy.double() * gate
+    back = torch.cat([chain[1:], torch.zeros_like(chain[:1])])
+    g = doubled(back.flip(0), (d[:, :, None] * C[:, None]).flip(0)).flip(0)
+    before = torch.cat([torch.zeros_like(h[:1]), h[:-1]])
+    for i in range(3):
+        before[b[i]] = a["state"][i].double()
+    flow = g * p * before
+    dd = (u * (g * B[:, None]).sum(2) + (flow * A).sum(2)) * torch.sigmoid(raw)
+    want = dict(u=a["D"].double() * d + s * (g * B[:, None]).sum(2), delta=dd, A=(flow * s[:, :, None]).sum(0), B=(g * (s * u)[:, :, None]).sum(1),
+                C=(h * d[:, :, None]).sum(1), D=(d * u).sum(0), delta_bias=dd.sum(0),
+                state=torch.stack([(g[b[i]] * p[b[i]]) for i in range(3)]))
+    # memories of up to a few hundred rows, 2^-24 x (a few tens of units per row) each
+    ok = lambda name, v, w: float((v.double() - w).norm()) <= 3e-5 * float(w.norm()) or pytest.fail("%s: %.3g" % (name, float((v.double() - w).norm() / w.norm())))
+    ok("y", y, pre * gate)
+    ok("final", f, torch.stack([h[b[i + 1] - 1] for i in range(3)]))
+    for k, v in want.items():
+        ok(k, got[k], v)
+
+
+def test_offsets_past_32_bits(S):
+    """Arrays of more than 2^31 elements: the last rows equal those of a call on their own."""
+    rows, ch, tail = 70000, 32768, 20
+    b = [0, rows - tail, rows]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(rows, ch, dtype=torch.bfloat16, device="cuda")
+    x.zero_()
+    x[-tail:].normal_(generator=gen)
+    last = x[-tail:].clone()
+    w, nw = torch.randn(ch, 4, device="cuda", generator=gen), torch.rand(ch, device="cuda", generator=gen)
+    A = -torch.rand(ch, 4, device="cuda", generator=gen)
+    B = torch.randn(rows, 4, device="cuda", generator=gen).bfloat16()
+    with torch.no_grad():
+        assert torch.equal(S.causal_conv(x, w, clip_start=starts_of(b))[-tail:], S.causal_conv(last, w))
+        y = S.rms_norm(x, nw)
+        assert torch.equal(y[-tail:], S.rms_norm(last, nw))
+        del y
+        y = S.selective_scan(x, x, A, B, B, clip_start=starts_of(b))
+        assert torch.equal(y[-tail:], S.selective_scan(last, last, A, B[-tail:].contiguous(), B[-tail:].contiguous()))
+
+
+def test_refusals(S):
+    x, w, st = torch.zeros(4, 8, device="cuda"), torch.zeros(8, 4, device="cuda"), torch.zeros(4, 3, 8, device="cuda")
+    A, Bm, hs = torch.zeros(8, 16, device="cuda"), torch.zeros(4, 16, device="cuda"), torch.zeros(4, 8, 16, device="cuda")
+    b = starts_of([0, 2, 4])
+    bad = [lambda: S.causal_conv(x.double(), w), lambda: S.causal_conv(x, w.half()), lambda: S.causal_conv(x, w[:4]), lambda: S.causal_conv(x, torch.zeros(8, 9, device="cuda")),
+           lambda: S.causal_conv(x[0], w), lambda: S.causal_conv(x, w, activation="relu"), lambda: S.causal_conv(x, w, clip_start=b.long()),
+           lambda: S.causal_conv(x, w, clip_start=b.cpu()), lambda: S.causal_conv(x, w, clip_start=b[:1]), lambda: S.causal_conv(x, w, clip_start=b, state=st),
+           lambda: S.causal_conv(x, w, clip_start=b, state=st[:2].half()), lambda: S.causal_conv(x, w, bias=torch.zeros(7, device="cuda")), lambda: S.causal_conv(x, w.cpu()),
+           lambda: S.causal_conv_step(x, w, st.transpose(0, 1).contiguous().transpose(0, 1)), lambda: S.causal_conv_step(x, w, st[:3]), lambda: S.causal_conv_step(x, w, None),
+           lambda: S.causal_conv_step(x.clone().requires_grad_(), w, st), lambda: S.causal_conv_step(x, w, torch.zeros(5, 3, 8, device="cuda")[:4], state_out=st.half()),
+           lambda: S.selective_scan(x, x.half(), A, Bm, Bm), lambda: S.selective_scan(x, x, A.half(), Bm, Bm), lambda: S.selective_scan(x, x, A, Bm[:3], Bm),
+           lambda: S.selective_scan(x, x, A, Bm, Bm[:, :8]), lambda: S.selective_scan(x, x, torch.zeros(8, 65, device="cuda"), Bm, Bm), lambda: S.selective_scan(x, x, A, Bm, Bm, z=x[:, :7]),
+           lambda: S.selective_scan(x, x, A, Bm, Bm, D=torch.zeros(8, 1, device="cuda")), lambda: S.selective_scan(x, x, A, Bm, Bm, state=hs), lambda: S.selective_scan(x, x, A, Bm, Bm.cpu()),
+           lambda: S.selective_scan_step(x, x, A, Bm, Bm, hs.half()), lambda: S.selective_scan_step(x, x, A, Bm, Bm, hs.transpose(1, 2).contiguous().transpose(1, 2)),
+           lambda: S.selective_scan_step(x, x, A.clone().requires_grad_(), Bm, Bm, hs), lambda: S.rms_norm(x, w), lambda: S.rms_norm(x, None), lambda: S.rms_norm(x, torch.ones(8, device="cuda"), eps=-1.0),
+           lambda: S.rms_norm(x, torch.ones(8, device="cuda"), residual=x.half()), lambda: S.rms_norm(x, torch.ones(8, device="cuda"), residual=x[:2]),
+           lambda: S.rms_norm_fp8(x.clone().requires_grad_(), torch.ones(8, device="cuda")), lambda: S.rms_norm(x[:, :0], torch.ones(0, device="cuda"))]
+    for i, f in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            f()
+            pytest.fail("refusal %d did not happen" % i)
+    big = torch.zeros(8 * 3 * 8 + 4, device="cuda")              # state_out that overlaps the state
+    with pytest.raises(RuntimeError, match="overlaps"):
+        S.causal_conv_step(x, w, big[:96].view(4, 3, 8), state_out=big[4:100].view(4, 3, 8))
+    # a state that a pending gradient needs may not be moved on behind autograd's back
+    s0 = hs.clone().requires_grad_()
+    s1 = (s0 * 1.0)
+    y = S.selective_scan(x, x, A, Bm, Bm, clip_start=starts_of([0, 1, 2, 3, 4]), state=s1)
+    with torch.no_grad():
+        S.selective_scan_step(x, x, A, Bm, Bm, s1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
