@@ -24,6 +24,7 @@
 #include "seq.h"
 
 #define SCAN_TILE 16
+#define SCAN_KEEP 8                  // rows per checkpoint: the backward pass holds that many rows in registers
 #define SCAN_MAX_STATE 64
 
 struct ScanArgs {
@@ -33,7 +34,7 @@ struct ScanArgs {
     const float *A, *D, *bias, *state;
     float* final_state;
     void* y; int64_t ldy;
-    float* ckpt;                                     // [tiles][channels][4 LPC]: the state in front of every 16th row
+    float* ckpt;                                     // [rows / 8][channels][4 LPC]: the state in front of every 8th row
     float* carry; float* span; int* flag;            // per chunk: [channels][4 LPC] end state, [channels] sum of s, 1 = stands alone
     int rows, channels, n_state, chunk_rows, chunks, softplus;
     // gradient
@@ -49,8 +50,12 @@ template <int CTRL> __device__ __forceinline__ float seq_dpp(float v) {
 }
 // value of lane Q of the quad, in all four lanes
 template <int Q> __device__ __forceinline__ float quad_bcast(float v) { return seq_dpp<Q * 0x55>(v); }
+// (as a register of its own: a multiplication with a DPP operand issues at 0.6 of the rate of a plain one -- 31 against 50 T
+// lane operations per second -- and every broadcast value is used four times)
 __device__ __forceinline__ float quad_bcast(float v, int q) {
-    return q == 0 ? quad_bcast<0>(v) : q == 1 ? quad_bcast<1>(v) : q == 2 ? quad_bcast<2>(v) : quad_bcast<3>(v);
+    float b = q == 0 ? quad_bcast<0>(v) : q == 1 ? quad_bcast<1>(v) : q == 2 ? quad_bcast<2>(v) : quad_bcast<3>(v);
+    asm("" : "+v"(b));
+    return b;
 }
 // sum over the LPC lanes of a channel, in all of them: xor 1, xor 2 (quad_perm), then the mirrored half and whole row of 16
 template <int LPC> __device__ __forceinline__ float chan_sum(float v) {
@@ -61,19 +66,32 @@ template <int LPC> __device__ __forceinline__ float chan_sum(float v) {
     return v;
 }
 
-// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], with log1p(e) = 2 artanh(r), r = e / (2 + e) <= 1/3, as its
-// series to r^15 (next term 2 r^17 / 17 < 1e-9): relative accuracy for small e too, where log(1 + e) has none left.
+// Four rows' partial sums v[0..3] in the LPC lanes of a channel -> the sum of row q in every lane with quad position q: the
+// quads are folded first (mirrored half rows and rows: the lane order inside a quad does not matter to the sum), then a quad
+// exchanges halves twice, which takes 9 operations for four rows instead of 12 for a sum in all lanes and a select.
+template <int LPC> __device__ __forceinline__ float quad_rows(float (&v)[4], int q) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (LPC >= 8) v[i] += seq_dpp<0x141>(v[i]);
+        if constexpr (LPC >= 16) v[i] += seq_dpp<0x140>(v[i]);
+    }
+    const bool odd = q & 1, high = q & 2;
+    const float a = (odd ? v[1] : v[0]) + seq_dpp<0xB1>(odd ? v[0] : v[1]);
+    const float b = (odd ? v[3] : v[2]) + seq_dpp<0xB1>(odd ? v[2] : v[3]);
+    return (high ? b : a) + seq_dpp<0x4E>(high ? a : b);
+}
+
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], with log1p(e) = 2 artanh(r), r = e / (2 + e) <= 1/3: relative
+// accuracy for small e too, where log(1 + e) has none left.  artanh(r) / r is a polynomial of degree 4 in r^2 fitted to
+// [0, 1/9] (relative error 4e-9; its series needs r^14 for as much).
 __device__ __forceinline__ float scan_softplus(float x) {
     const float e = seq_exp2(-SEQ_LOG2E * fabsf(x));
     const float r = e * seq_rcp(2.f + e), q = r * r;
-    float p = fmaf(q, 1.f / 15.f, 1.f / 13.f);
-    p = fmaf(q, p, 1.f / 11.f);
-    p = fmaf(q, p, 1.f / 9.f);
-    p = fmaf(q, p, 1.f / 7.f);
-    p = fmaf(q, p, 1.f / 5.f);
-    p = fmaf(q, p, 1.f / 3.f);
+    float p = fmaf(q, 0.14089167f, 0.13980302f);
+    p = fmaf(q, p, 0.20012455f);
+    p = fmaf(q, p, 0.33333158f);
     p = fmaf(q, p, 1.f);
-    return fmaxf(x, 0.f) + 2.f * r * p;
+    return fmaf(2.f * r, p, fmaxf(x, 0.f));
 }
 
 // lane's place in its workgroup
@@ -96,22 +114,65 @@ __device__ __forceinline__ void scan_store4(float* __restrict__ row, int j, int 
     for (int i = 0; i < 4; ++i) if (4 * j + i < N) row[4 * j + i] = v[i];
 }
 
-// B and C of the 16 rows from t0 into LDS as floats, zero for rows outside [lo, hi) and states >= N
-template <typename T, int LPC>
-__device__ __forceinline__ void scan_stage(const ScanArgs& a, int t0, int lo, int hi, float* __restrict__ sB, float* __restrict__ sC) {
-    constexpr int N4 = 4 * LPC;
+// The same number, which the compiler takes for a new one: what is read or computed from it is neither moved out of
+// a loop nor turned into a pointer per access that the loop carries along (16 rows of B and C alone are 128 registers, the
+// addresses of a tile's rows 60).
+__device__ __forceinline__ int scan_again(int v) { asm volatile("" : "+v"(v)); return v; }
+
+// base is the same for the whole wave, off in bytes: one scalar base and one 32-bit offset per access
+template <typename T> __device__ __forceinline__ T& scan_at(T* base, unsigned off) { return *(T*)((char*)base + off); }
+template <typename T> __device__ __forceinline__ const T& scan_at(const T* base, unsigned off) { return *(const T*)((const char*)base + off); }
+
+// B (and C) of a tile on their way to LDS as floats: requested a tile ahead, written when the rows in front are done.  A
+// thread takes one state of every (256 / N4)th row; rows of no clip and states >= N become zero.
+template <typename T, int LPC> struct ScanStage {
+    static constexpr int N4 = 4 * LPC, PER = SCAN_TILE * N4 / 256, STEP = 256 / N4;
+    T v[PER];
+    __device__ __forceinline__ void load(const void* base, int64_t ld, int t0, int rows, int N) {
+        const int r = scan_again(threadIdx.x) / N4, n = threadIdx.x % N4;
+        const T* p = (const T*)base + (int64_t)t0 * ld;
+        const bool full = t0 + SCAN_TILE <= rows;
 #pragma unroll
-    for (int e = threadIdx.x; e < SCAN_TILE * N4; e += 256) {
-        const int r = t0 + e / N4, n = e % N4;
-        float b = 0.f, c = 0.f;
-        if (r >= lo && r < hi && n < a.n_state) {
-            b = (float)((const T*)a.B)[(int64_t)r * a.ldb + n];
-            if (sC) c = (float)((const T*)a.C)[(int64_t)r * a.ldc + n];
+        for (int i = 0; i < PER; ++i) {
+            v[i] = (T)0.f;
+            if (n < N && (full || t0 + r + i * STEP < rows)) v[i] = scan_at(p, (unsigned)((r + i * STEP) * (int)ld + n) * sizeof(T));
         }
-        sB[e] = b;
-        if (sC) sC[e] = c;
+    }
+    __device__ __forceinline__ void store(float* __restrict__ s, int t0, int lo, int hi) const {
+        const bool clean = t0 >= lo && t0 + SCAN_TILE <= hi;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int r = t0 + threadIdx.x / N4 + i * STEP;
+            s[threadIdx.x + 256 * i] = clean || (r >= lo && r < hi) ? (float)v[i] : 0.f;
+        }
+    }
+};
+// A lane's element of four rows of a tile: rows t0 + 4 k + q, channel d (at = q ld + d, in bytes)
+template <typename T> __device__ __forceinline__ void scan_fetch(const void* base, int64_t ld, unsigned at, int t0, int q, int rows, T (&v)[4]) {
+    const T* p = (const T*)base + (int64_t)t0 * ld;
+    const unsigned step = 4 * (unsigned)ld * sizeof(T);
+    at = scan_again(at);
+    if (t0 + SCAN_TILE <= rows) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = scan_at(p, at + k * step);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { v[k] = (T)0.f; if (t0 + 4 * k + q < rows) v[k] = scan_at(p, at + k * step); }
     }
 }
+
+// B or C of a pair of rows, read from LDS a pair ahead (and, with a scheduling barrier behind the reads, not more: the
+// registers would cost waves in flight)
+template <int N4> struct ScanPair {
+    const float* p; seq_f4 v[2][2];
+    __device__ __forceinline__ ScanPair(const float* at, int k = 0) : p(at) { read(k); }
+    __device__ __forceinline__ void read(int k) {
+        v[k & 1][0] = *(const seq_f4*)(p + 2 * k * N4);
+        v[k & 1][1] = *(const seq_f4*)(p + (2 * k + 1) * N4);
+    }
+    __device__ __forceinline__ void ahead(int k) { if (k >= 0 && k < SCAN_TILE / 2) read(k); }
+    __device__ __forceinline__ seq_f4 row(int i) const { return v[(i >> 1) & 1][i & 1]; }
+};
 
 // The walk over the clips' ends while rows go up (all values are the same in the whole workgroup).
 struct ScanWalk { int s, next; };
@@ -123,141 +184,151 @@ __device__ __forceinline__ ScanWalk scan_walk(const SeqClips& c, int row) {
 }
 
 // WHAT 0: outputs.  WHAT 1: the chunk's end state for the chunks behind it.
+//
+// A chunk is walked in pieces, the rows that a tile and a clip have in common.  A piece runs through all 16 rows of its
+// tile as straight-line code, with step and input 0 for rows outside it, which leave the state as it is: the usual tile is one
+// piece, a clip's end inside a tile costs one more, and there is no branch between two rows that would keep the reads
+// of B and C from being requested ahead.
 template <typename T, int LPC, int WHAT>
-__global__ __launch_bounds__(256) void k_scan_fwd(ScanArgs a) {
+__global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     constexpr int N4 = 4 * LPC;
     __shared__ __attribute__((aligned(16))) float sB[2][SCAN_TILE * N4], sC[2][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y;
     const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
-    const int lo = max(0, seq_start(a.clips, 0)), hi = min(a.rows, seq_start(a.clips, n));       // rows that belong to a clip
     float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
     scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
-    const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
+    const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = WHAT == 0 && a.D ? a.D[L.d] : 0.f;
+    auto entry = [&](int s) {                                    // the state in front of clip s
+#pragma unroll
+        for (int m = 0; m < 4; ++m) h[m] = 0.f;
+        if (a.state && s >= 0 && s < n) scan_load4(a.state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
+    };
+    auto leave = [&](int s) {                                    // h is the state behind clip s
+        if (a.final_state && s >= 0 && s < n && L.in) scan_store4(a.final_state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
+    };
 
-    int from = c0;
-    ScanWalk w;
-    bool alone = false;
+    ScanWalk w = scan_walk(a.clips, WHAT == 1 ? c1 - 1 : c0);
+    const int first = w.s >= 0 ? seq_start(a.clips, w.s) : 0;
+    int at = c0;                                                 // first row of the next piece
     if constexpr (WHAT == 1) {
-        // only the rows since the last clip start of the chunk matter, and none if the next chunk starts a clip of its own
-        w = scan_walk(a.clips, c1 - 1);
-        const int first = w.s >= 0 ? seq_start(a.clips, w.s) : 0;
-        alone = w.s < 0 || w.s >= n || w.next <= c1 || first >= c0;
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.flag[chunk] = alone ? 1 : 0;
-        if (w.s < 0 || w.s >= n || w.next <= c1) {
-            if (L.in) {
-                const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-                scan_store4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, zero);
-            }
+        // only the rows since the last clip start of the chunk matter, and none if the next chunk starts with a clip of its own
+        const bool none = w.s < 0 || w.s >= n || w.next <= c1;
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.flag[chunk] = none || first >= c0;
+        if (none) {
+            if (L.in) scan_store4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
             return;
         }
-        if (first >= c0) {
-            from = first;
-            if (a.state) scan_load4(a.state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h);
-        }
+        if (first >= c0) { at = first; entry(w.s); }
         w.next = 0x7fffffff;
     } else {
-        w = scan_walk(a.clips, c0);
-        if (a.final_state && L.in) {                             // empty clips at the chunk's first row keep their state
-            for (int e = w.s - 1; e >= 0 && seq_start(a.clips, e) == c0; --e) {
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (a.state) scan_load4(a.state + ((size_t)e * a.channels + L.d) * N, L.j, N, v);
-                scan_store4(a.final_state + ((size_t)e * a.channels + L.d) * N, L.j, N, v);
-            }
-        }
-        if (w.s >= 0 && w.s < n) {
-            if (seq_start(a.clips, w.s) == c0) { if (a.state) scan_load4(a.state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h); }
-            else if (chunk > 0) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
-        }
+        if (a.final_state)                                       // empty clips at the chunk's first row keep their state
+            for (int e = w.s - 1; e >= 0 && seq_start(a.clips, e) == c0; --e) { entry(e); leave(e); }
+        if (w.s >= 0 && w.s < n && first < c0 && chunk > 0) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
+        else entry(w.s);
     }
     if (c1 <= c0) return;
-    const int tile0 = from / SCAN_TILE * SCAN_TILE;
+    const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));           // rows that belong to a clip
+    const unsigned at_u = (unsigned)(L.q * (int)a.ldu + L.d) * sizeof(T), at_d = (unsigned)(L.q * (int)a.ldd + L.d) * sizeof(T);
+    const unsigned at_z = (unsigned)(L.q * (int)a.ldz + L.d) * sizeof(T), at_y = (unsigned)(L.q * (int)a.ldy + L.d) * sizeof(T);
     float span = 0.f;
     T ru[4], rd[4], rz[4];
+    ScanStage<T, LPC> stB, stC;
     auto fetch = [&](int t0) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t r = min(t0 + 4 * k + L.q, a.rows - 1);
-            ru[k] = ((const T*)a.u)[r * a.ldu + L.d];
-            rd[k] = ((const T*)a.delta)[r * a.ldd + L.d];
-            if (WHAT == 0 && a.z) rz[k] = ((const T*)a.z)[r * a.ldz + L.d];
-        }
+        scan_fetch<T>(a.u, a.ldu, at_u, t0, L.q, a.rows, ru);
+        scan_fetch<T>(a.delta, a.ldd, at_d, t0, L.q, a.rows, rd);
+        if (WHAT == 0 && a.z) scan_fetch<T>(a.z, a.ldz, at_z, t0, L.q, a.rows, rz);
+        stB.load(a.B, a.ldb, t0, a.rows, N);
+        if (WHAT == 0) stC.load(a.C, a.ldc, t0, a.rows, N);
     };
-    fetch(tile0);
-    scan_stage<T, LPC>(a, tile0, max(lo, from), min(hi, c1), sB[0], WHAT == 0 ? sC[0] : nullptr);
+    int t0 = at / SCAN_TILE * SCAN_TILE, buf = 0;
+    fetch(t0);
+    stB.store(sB[0], t0, lo, hi);
+    if (WHAT == 0) stC.store(sC[0], t0, lo, hi);
     __syncthreads();
-    int buf = 0;
-    for (int t0 = tile0; t0 < c1; t0 += SCAN_TILE, buf ^= 1) {
-        float st[4], x[4], u[4], gate[4], ys[4];
+    for (; t0 < c1; t0 += SCAN_TILE, buf ^= 1) {
+        float st[4], u[4], gate[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int r = t0 + 4 * k + L.q;
-            const bool live = r >= max(lo, from) && r < min(hi, c1);
-            u[k] = live ? (float)ru[k] : 0.f;
+            u[k] = (float)ru[k];
             const float raw = (float)rd[k] + bias;
-            st[k] = live ? (a.softplus ? scan_softplus(raw) : raw) : 0.f;      // a row of no clip leaves the state as it is
-            x[k] = st[k] * u[k];
-            span += st[k];
+            st[k] = a.softplus ? scan_softplus(raw) : raw;
             gate[k] = 1.f;
-            if (WHAT == 0 && a.z) { const float z = (float)rz[k]; gate[k] = live ? z * seq_sigmoid(z) : 0.f; }
-            ys[k] = 0.f;
+            if (WHAT == 0 && a.z) { const float z = (float)rz[k]; gate[k] = z * seq_sigmoid(z); }
         }
         const bool more = t0 + SCAN_TILE < c1;
-        if (more) {
-            fetch(t0 + SCAN_TILE);
-            scan_stage<T, LPC>(a, t0 + SCAN_TILE, lo, min(hi, c1), sB[buf ^ 1], WHAT == 0 ? sC[buf ^ 1] : nullptr);
-        }
-        if (WHAT == 0 && a.ckpt && L.in) *(seq_f4*)(a.ckpt + ((size_t)(t0 / SCAN_TILE) * a.channels + L.d) * N4 + 4 * L.j) = seq_f4{h[0], h[1], h[2], h[3]};
+        if (more) fetch(t0 + SCAN_TILE);
+        auto keep = [&](int row) {                               // the state in front of the row, for the backward pass
+            if (WHAT == 0 && a.ckpt && L.in) *(seq_f4*)(a.ckpt + ((size_t)(row / SCAN_KEEP) * a.channels + L.d) * N4 + 4 * L.j) = seq_f4{h[0], h[1], h[2], h[3]};
+        };
+        keep(t0);
+        T* py = (T*)a.y + (int64_t)t0 * a.ldy;
+        const int t1 = min(t0 + SCAN_TILE, c1);
+        do {                                                     // the tile's pieces: rows at .. end-1
+            const int end = min(t1, w.next);
+            const float *tB = sB[buf] + scan_again(4 * L.j), *tC = sC[buf] + scan_again(4 * L.j);
+            const bool whole = at == t0 && end == t0 + SCAN_TILE, live = at >= lo && at < hi;    // (of a clip, or of none)
+            float s4[4], x4[4], ys[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int i = 4 * k + q;
-                if (WHAT == 0 && t0 + i >= w.next && w.s < n && t0 + i < c1) {     // a clip ended in front of this row
-                    const int p = t0 + i;
-                    if (a.final_state && w.s >= 0 && L.in) scan_store4(a.final_state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h);
-                    ++w.s;
-                    while (w.s < n && seq_start(a.clips, w.s + 1) <= p) {
-                        if (a.final_state && L.in) {
-                            float v[4] = {0.f, 0.f, 0.f, 0.f};
-                            if (a.state) scan_load4(a.state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, v);
-                            scan_store4(a.final_state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, v);
-                        }
-                        ++w.s;
-                    }
-                    w.next = w.s < n ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, w.s + 1)) : 0x7fffffff;
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) h[m] = 0.f;
-                    if (a.state && w.s < n) scan_load4(a.state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h);
-                }
-                const float sb = quad_bcast(st[k], q), xb = quad_bcast(x[k], q);
-                const seq_f4 b4 = *(const seq_f4*)(sB[buf] + i * N4 + 4 * L.j);
-                float acc = 0.f;
-                if constexpr (WHAT == 0) {
-                    const seq_f4 c4 = *(const seq_f4*)(sC[buf] + i * N4 + 4 * L.j);
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) {
-                        h[m] = fmaf(seq_exp2(sb * A2[m]), h[m], xb * b4[m]);
-                        acc = fmaf(c4[m], h[m], acc);
-                    }
-                    acc = chan_sum<LPC>(acc);
-                    ys[k] = L.q == q ? acc : ys[k];
-                } else {
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) h[m] = fmaf(seq_exp2(sb * A2[m]), h[m], xb * b4[m]);
-                }
-            }
-        }
-        if constexpr (WHAT == 0) {
-            if (L.in && L.j < 4) {
+            for (int k = 0; k < 4; ++k) { s4[k] = st[k]; x4[k] = st[k] * u[k]; }
+            if (!whole || !live) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int r = t0 + 4 * k + L.q;
-                    if (r < c1) ((T*)a.y)[(int64_t)r * a.ldy + L.d] = (T)(r >= lo && r < hi ? fmaf(Dd, u[k], ys[k]) * gate[k] : 0.f);
+                    const bool mine = live && r >= at && r < end;
+                    s4[k] = mine ? s4[k] : 0.f; x4[k] = mine ? x4[k] : 0.f;
                 }
             }
+            ScanPair<N4> gB(tB), gC(WHAT == 0 ? tC : tB);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float acc[4];
+                if constexpr (WHAT == 1) span += s4[k];
+                if (k == 2 && at <= t0 + SCAN_KEEP && end > t0 + SCAN_KEEP) keep(t0 + SCAN_KEEP);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (q % 2 == 0) {
+                        gB.ahead(2 * k + q / 2 + 1);
+                        if constexpr (WHAT == 0) gC.ahead(2 * k + q / 2 + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    const float sb = quad_bcast(s4[k], q), xb = quad_bcast(x4[k], q);
+                    const seq_f4 b4 = gB.row(4 * k + q), c4 = gC.row(4 * k + q);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        h[m] = fmaf(seq_exp2(sb * A2[m]), h[m], xb * b4[m]);
+                        if constexpr (WHAT == 0) acc[q] = m ? fmaf(c4[m], h[m], acc[q]) : c4[0] * h[0];
+                    }
+                }
+                if constexpr (WHAT == 0) ys[k] = quad_rows<LPC>(acc, L.q);
+            }
+            if constexpr (WHAT == 0) {
+                const unsigned oy = scan_again(at_y);
+                if (L.in && L.j < 4) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = t0 + 4 * k + L.q;
+                        const float y = fmaf(Dd, u[k], ys[k]) * gate[k];
+                        if (whole || (r >= at && r < end)) scan_at(py, oy + 4 * k * (unsigned)a.ldy * sizeof(T)) = (T)(live ? y : 0.f);
+                    }
+                }
+                if (end >= w.next && w.s < n) {                  // a clip ended with the piece
+                    leave(w.s);
+                    if (end < c1 || c1 == a.rows) {              // (clips that start with the next chunk are its own)
+                        ++w.s;
+                        while (w.s < n && seq_start(a.clips, w.s + 1) <= end) { entry(w.s); leave(w.s); ++w.s; }
+                        w.next = w.s < n ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, w.s + 1)) : 0x7fffffff;
+                        if (end < c1) entry(w.s);
+                    }
+                }
+            }
+            at = end;
+        } while (at < t1);
+        if (more) {
+            stB.store(sB[buf ^ 1], t0 + SCAN_TILE, lo, hi);
+            if (WHAT == 0) stC.store(sC[buf ^ 1], t0 + SCAN_TILE, lo, hi);
         }
         __syncthreads();
     }
@@ -267,15 +338,6 @@ __global__ __launch_bounds__(256) void k_scan_fwd(ScanArgs a) {
             span += seq_dpp<0xB1>(span);
             span += seq_dpp<0x4E>(span);
             if (L.j == 0) a.span[(size_t)chunk * a.channels + L.d] = span;
-        }
-    } else if (a.final_state && L.in && w.next <= c1 && w.s < n) {                 // a clip ends with the chunk
-        if (w.s >= 0) scan_store4(a.final_state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h);
-        if (c1 == a.rows) {                                                        // empty clips behind the last row
-            for (int e = w.s + 1; e < n; ++e) {
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (a.state) scan_load4(a.state + ((size_t)e * a.channels + L.d) * N, L.j, N, v);
-                scan_store4(a.final_state + ((size_t)e * a.channels + L.d) * N, L.j, N, v);
-            }
         }
     }
 }
@@ -308,7 +370,7 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
 
 // The adjoint of a chunk by itself: what its rows contribute to dL/dh in front of its first row.
 template <typename T, int LPC>
-__global__ __launch_bounds__(256) void k_scan_adj(ScanArgs a) {
+__global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
     constexpr int N4 = 4 * LPC;
     __shared__ __attribute__((aligned(16))) float sC[2][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
@@ -329,49 +391,52 @@ __global__ __launch_bounds__(256) void k_scan_adj(ScanArgs a) {
     }
     const int to = min(w.next, c1);                                                // rows [c0, to)
     if (ends && a.dfinal) scan_load4(a.dfinal + ((size_t)w.s * a.channels + L.d) * N, L.j, N, g);
+    const unsigned at_d = (unsigned)(L.q * (int)a.ldd + L.d) * sizeof(T), at_y = (unsigned)(L.q * (int)a.lddy + L.d) * sizeof(T), at_z = (unsigned)(L.q * (int)a.ldz + L.d) * sizeof(T);
     float span = 0.f;
     T rd[4], ry[4], rz[4];
+    ScanStage<T, LPC> stC;
     auto fetch = [&](int t0) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t r = max(0, min(t0 + 4 * k + L.q, a.rows - 1));
-            rd[k] = ((const T*)a.delta)[r * a.ldd + L.d];
-            ry[k] = ((const T*)a.dy)[r * a.lddy + L.d];
-            if (a.z) rz[k] = ((const T*)a.z)[r * a.ldz + L.d];
-        }
-    };
-    auto stage = [&](int t0, float* s) {
-        for (int e = threadIdx.x; e < SCAN_TILE * N4; e += 256) {
-            const int r = t0 + e / N4, m = e % N4;
-            s[e] = r < to && m < N ? (float)((const T*)a.C)[(int64_t)r * a.ldc + m] : 0.f;
-        }
+        scan_fetch<T>(a.delta, a.ldd, at_d, t0, L.q, a.rows, rd);
+        scan_fetch<T>(a.dy, a.lddy, at_y, t0, L.q, a.rows, ry);
+        if (a.z) scan_fetch<T>(a.z, a.ldz, at_z, t0, L.q, a.rows, rz);
+        stC.load(a.C, a.ldc, t0, a.rows, N);
     };
     int t0 = (to - 1) / SCAN_TILE * SCAN_TILE, buf = 0;
     fetch(t0);
-    stage(t0, sC[0]);
+    stC.store(sC[0], t0, c0, to);
     __syncthreads();
     for (; t0 >= c0; t0 -= SCAN_TILE, buf ^= 1) {
         float st[4], dy[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const bool live = t0 + 4 * k + L.q < to;
             const float raw = (float)rd[k] + bias;
-            st[k] = live ? (a.softplus ? scan_softplus(raw) : raw) : 0.f;
-            dy[k] = live ? (float)ry[k] : 0.f;
-            if (a.z && live) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
-            span += st[k];
+            st[k] = a.softplus ? scan_softplus(raw) : raw;
+            dy[k] = (float)ry[k];
+            if (a.z) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
         }
-        if (t0 - SCAN_TILE >= c0) { fetch(t0 - SCAN_TILE); stage(t0 - SCAN_TILE, sC[buf ^ 1]); }
+        if (t0 + SCAN_TILE > to) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { const bool live = t0 + 4 * k + L.q < to; st[k] = live ? st[k] : 0.f; dy[k] = live ? dy[k] : 0.f; }
+        }
+        const bool more = t0 - SCAN_TILE >= c0;
+        if (more) fetch(t0 - SCAN_TILE);
+        ScanPair<N4> gC(sC[buf] + 4 * L.j, SCAN_TILE / 2 - 1);
 #pragma unroll
         for (int k = 3; k >= 0; --k) {
+            span += st[k];
 #pragma unroll
             for (int q = 3; q >= 0; --q) {
+                if (q % 2 == 1) {
+                    gC.ahead(2 * k + q / 2 - 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 const float sb = quad_bcast(st[k], q), db = quad_bcast(dy[k], q);
-                const seq_f4 c4 = *(const seq_f4*)(sC[buf] + (4 * k + q) * N4 + 4 * L.j);
+                const seq_f4 c4 = gC.row(4 * k + q);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) g[m] = seq_exp2(sb * A2[m]) * fmaf(c4[m], db, g[m]);
             }
         }
+        if (more) stC.store(sC[buf ^ 1], t0 - SCAN_TILE, c0, to);
         __syncthreads();
     }
     if (L.in) {
@@ -406,188 +471,192 @@ template <int LPC> __device__ __forceinline__ void wave_fold(float (&b)[4], cons
     }
 }
 
+// The gradient of a chunk, from its last row to its first, in pieces like the forward's.  A piece takes its tile in halves: forward
+// from the checkpoint, with e_t = exp(s_t A) and e_t h_{t-1} of the 8 rows kept in registers, then back with the adjoint.
 template <typename T, int LPC>
-__global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs a) {
+__global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     constexpr int N4 = 4 * LPC, W = 2 * N4;
-    __shared__ __attribute__((aligned(16))) float sB[2][SCAN_TILE * N4], sC[2][SCAN_TILE * N4], red[4][SCAN_TILE * W];
+    __shared__ __attribute__((aligned(16))) float sB[2][SCAN_TILE * N4], sC[2][SCAN_TILE * N4], red[4][(SCAN_TILE + 1) * W];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
-    const int lo = max(0, seq_start(a.clips, 0)), hi = min(a.rows, seq_start(a.clips, n));
     float A2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
     scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
-    auto empty = [&](int e) {                                     // an empty clip passes the gradient of its state on
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (a.dfinal) scan_load4(a.dfinal + ((size_t)e * a.channels + L.d) * N, L.j, N, v);
-        scan_store4(a.dstate + ((size_t)e * a.channels + L.d) * N, L.j, N, v);
+    auto entry = [&](int s) {                                     // the gradient of the state behind clip s
+#pragma unroll
+        for (int m = 0; m < 4; ++m) g[m] = 0.f;
+        if (a.dfinal && s >= 0 && s < n) scan_load4(a.dfinal + ((size_t)s * a.channels + L.d) * N, L.j, N, g);
     };
-    // rows go down: s = the clip of the current row, [first, next) its rows
+    auto leave = [&](int s) {                                     // g is the gradient of the state in front of clip s
+        if (a.dstate && s >= 0 && s < n && L.in) scan_store4(a.dstate + ((size_t)s * a.channels + L.d) * N, L.j, N, g);
+    };
+    // s = the clip of row end-1, first = its first row
     int s = __builtin_amdgcn_readfirstlane(seq_find(a.clips, c1 - 1));
     int first = s >= 0 ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, s)) : 0;
-    if (a.dstate && L.in)                                         // empty clips between this chunk's last row and the next row
-        for (int e = s + 1; e < n && seq_start(a.clips, e + 1) <= c1; ++e) empty(e);
-    if (s >= 0 && s < n) {
-        if (seq_start(a.clips, s + 1) <= c1) { if (a.dfinal) scan_load4(a.dfinal + ((size_t)s * a.channels + L.d) * N, L.j, N, g); }
-        else if (a.chunks > 1) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
-    }
+    if (a.dstate)                                                 // empty clips between this chunk's last row and the next row
+        for (int e = s + 1; e < n && seq_start(a.clips, e + 1) <= c1; ++e) { entry(e); leave(e); }
+    if (s >= 0 && s < n && seq_start(a.clips, s + 1) > c1) {
+        if (a.chunks > 1) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
+    } else entry(s);
+    const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));            // rows that belong to a clip
+    const unsigned at_u = (unsigned)(L.q * (int)a.ldu + L.d) * sizeof(T), at_d = (unsigned)(L.q * (int)a.ldd + L.d) * sizeof(T);
+    const unsigned at_z = (unsigned)(L.q * (int)a.ldz + L.d) * sizeof(T), at_y = (unsigned)(L.q * (int)a.lddy + L.d) * sizeof(T);
+    const unsigned at_du = (unsigned)(L.q * (int)a.lddu + L.d) * sizeof(T), at_dd = (unsigned)(L.q * (int)a.lddd + L.d) * sizeof(T), at_dz = (unsigned)(L.q * (int)a.lddz + L.d) * sizeof(T);
+    float* my_red = red[wave] + (lane >> 5) * N4 + 4 * L.j + 2 * ((lane >> 4) & 1);               // (its last row takes what no row wants)
     T ru[4], rd[4], rz[4], ry[4];
+    seq_f4 kept[2];
+    ScanStage<T, LPC> stB, stC;
     auto fetch = [&](int t0) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t r = max(0, min(t0 + 4 * k + L.q, a.rows - 1));
-            ru[k] = ((const T*)a.u)[r * a.ldu + L.d];
-            rd[k] = ((const T*)a.delta)[r * a.ldd + L.d];
-            ry[k] = ((const T*)a.dy)[r * a.lddy + L.d];
-            if (a.z) rz[k] = ((const T*)a.z)[r * a.ldz + L.d];
-        }
+        scan_fetch<T>(a.u, a.ldu, at_u, t0, L.q, a.rows, ru);
+        scan_fetch<T>(a.delta, a.ldd, at_d, t0, L.q, a.rows, rd);
+        scan_fetch<T>(a.dy, a.lddy, at_y, t0, L.q, a.rows, ry);
+        if (a.z) scan_fetch<T>(a.z, a.ldz, at_z, t0, L.q, a.rows, rz);
+        stB.load(a.B, a.ldb, t0, a.rows, N);
+        stC.load(a.C, a.ldc, t0, a.rows, N);
+        const float* p = a.ckpt + ((size_t)(t0 / SCAN_KEEP) * a.channels + scan_again(L.d)) * N4 + 4 * L.j;
+        kept[0] = *(const seq_f4*)p;
+        kept[1] = t0 + SCAN_KEEP < a.rows ? *(const seq_f4*)(p + (size_t)a.channels * N4) : seq_f4{0.f, 0.f, 0.f, 0.f};
     };
-    int t0 = (c1 - 1) / SCAN_TILE * SCAN_TILE, buf = 0;
+    int t0 = (c1 - 1) / SCAN_TILE * SCAN_TILE, buf = 0, end = c1;
     if (c1 > c0) {
         fetch(t0);
-        scan_stage<T, LPC>(a, t0, lo, min(hi, c1), sB[0], sC[0]);
+        stB.store(sB[0], t0, lo, hi);
+        stC.store(sC[0], t0, lo, hi);
     }
     __syncthreads();
     for (; c1 > c0 && t0 >= c0; t0 -= SCAN_TILE, buf ^= 1) {
-        float st[4], x[4], u[4], dy[4], ys[4], sb_[4], sa_[4], hp[SCAN_TILE][4];
+        float st[4], u[4], dy[4];
         T raw_d[4], raw_z[4], raw_y[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int r = t0 + 4 * k + L.q;
-            const bool live = r >= lo && r < min(hi, c1);
             raw_d[k] = rd[k]; raw_z[k] = rz[k]; raw_y[k] = ry[k];
-            u[k] = live ? (float)ru[k] : 0.f;
+            u[k] = (float)ru[k];
             const float raw = (float)rd[k] + bias;
-            st[k] = live ? (a.softplus ? scan_softplus(raw) : raw) : 0.f;
-            x[k] = st[k] * u[k];
-            dy[k] = live ? (float)ry[k] : 0.f;
-            if (a.z && live) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
-            ys[k] = 0.f; sb_[k] = 0.f; sa_[k] = 0.f;
+            st[k] = a.softplus ? scan_softplus(raw) : raw;
+            dy[k] = (float)ry[k];
+            if (a.z) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
         }
-        float h[4];
-        {
-            const seq_f4 v = *(const seq_f4*)(a.ckpt + ((size_t)(t0 / SCAN_TILE) * a.channels + L.d) * N4 + 4 * L.j);
+        const bool more = t0 - SCAN_TILE >= c0;
+        T* pu = (T*)a.du + (int64_t)t0 * a.lddu;
+        T* pd = (T*)a.ddelta + (int64_t)t0 * a.lddd;
+        T* pz = (T*)a.dz + (int64_t)t0 * a.lddz;
+        const seq_f4 k0 = kept[0], k1 = kept[1];
+        do {                                                      // the tile's pieces: rows at .. end-1
+            const int at = max(t0, first);
+            const bool whole = at == t0 && end == t0 + SCAN_TILE, live = at >= lo && at < hi;     // (of a clip, or of none)
+            float s4[4], x4[4], d4[4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) h[m] = v[m];
-        }
-        if (t0 - SCAN_TILE >= c0) {
-            fetch(t0 - SCAN_TILE);
-            scan_stage<T, LPC>(a, t0 - SCAN_TILE, lo, min(hi, c1), sB[buf ^ 1], sC[buf ^ 1]);
-        }
-        // forward through the tile again, keeping the state in front of every row
-        {
-            ScanWalk w = {s, 0x7fffffff};
-            if (s >= 0 && first <= t0) { if (s < n) w.next = __builtin_amdgcn_readfirstlane(seq_start(a.clips, s + 1)); }
-            else w = scan_walk(a.clips, t0);
-            if (w.s >= 0 && w.s < n && seq_start(a.clips, w.s) == t0) {
+            for (int k = 0; k < 4; ++k) { s4[k] = st[k]; x4[k] = st[k] * u[k]; d4[k] = dy[k]; }
+            if (!whole || !live || !L.in) {                       // (lanes past the last channel take part in the sums with zeros)
 #pragma unroll
-                for (int m = 0; m < 4; ++m) h[m] = 0.f;
-                if (a.state) scan_load4(a.state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h);
+                for (int k = 0; k < 4; ++k) {
+                    const int r = t0 + 4 * k + L.q;
+                    const bool mine = live && L.in && r >= at && r < end;
+                    s4[k] = mine ? s4[k] : 0.f; x4[k] = mine ? x4[k] : 0.f; d4[k] = mine ? d4[k] : 0.f;
+                }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int half = 1; half >= 0; --half) {
+                const int h0 = t0 + half * SCAN_KEEP;
+                if (at >= h0 + SCAN_KEEP || end <= h0) continue;
+                const float *tB = sB[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4), *tC = sC[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
+                float h[4], ex[SCAN_KEEP][4], ah[SCAN_KEEP][4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int i = 4 * k + q, p = t0 + i;
-                    if (p >= w.next && w.s < n && p < c1) {
-                        ++w.s;
-                        while (w.s < n && seq_start(a.clips, w.s + 1) <= p) ++w.s;
-                        w.next = w.s < n ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, w.s + 1)) : 0x7fffffff;
+                for (int m = 0; m < 4; ++m) h[m] = half ? k1[m] : k0[m];
+                if (at == first && at >= h0) {                    // the clip starts here
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) h[m] = 0.f;
-                        if (a.state && w.s < n) scan_load4(a.state + ((size_t)w.s * a.channels + L.d) * N, L.j, N, h);
-                    }
-                    const float sb = quad_bcast(st[k], q), xb = quad_bcast(x[k], q);
-                    const seq_f4 b4 = *(const seq_f4*)(sB[buf] + i * N4 + 4 * L.j);
+                    for (int m = 0; m < 4; ++m) h[m] = 0.f;
+                    if (a.state && live) scan_load4(a.state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
+                }
+#pragma unroll
+                for (int i = 0; i < SCAN_KEEP; ++i) {
+                    const int k = 2 * half + i / 4;
+                    const float sb = quad_bcast(s4[k], i & 3), xb = quad_bcast(x4[k], i & 3);
+                    const seq_f4 b4 = *(const seq_f4*)(tB + i * N4);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
-                        hp[i][m] = h[m];
-                        h[m] = fmaf(seq_exp2(sb * A2[m]), h[m], xb * b4[m]);
+                        ex[i][m] = seq_exp2(sb * A2[m]);
+                        ah[i][m] = ex[i][m] * h[m];
+                        h[m] = fmaf(xb, b4[m], ah[i][m]);
+                    }
+                }
+                if (half == 0 && more && at == t0) fetch(t0 - SCAN_TILE);
+#pragma unroll
+                for (int kk = 1; kk >= 0; --kk) {
+                    const int k = 2 * half + kk;
+                    float ys[4], gbs[4], gas[4];
+#pragma unroll
+                    for (int q = 3; q >= 0; --q) {
+                        const int i = 4 * kk + q;
+                        const float sb = quad_bcast(s4[k], q), xb = quad_bcast(x4[k], q), db = quad_bcast(d4[k], q);
+                        const seq_f4 b4 = *(const seq_f4*)(tB + i * N4), c4 = *(const seq_f4*)(tC + i * N4);
+                        float vb[4], vc[4];
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const float ht = fmaf(xb, b4[m], ah[i][m]);
+                            ys[q] = m ? fmaf(c4[m], ht, ys[q]) : c4[0] * ht;
+                            g[m] = fmaf(c4[m], db, g[m]);
+                            vb[m] = g[m] * xb;
+                            vc[m] = db * ht;
+                            gbs[q] = m ? fmaf(g[m], b4[m], gbs[q]) : g[0] * b4[0];
+                            const float f = g[m] * ah[i][m];
+                            gas[q] = m ? fmaf(A2[m], f, gas[q]) : A2[0] * f;
+                            dA[m] = fmaf(sb, f, dA[m]);
+                            g[m] *= ex[i][m];
+                        }
+                        wave_fold<LPC>(vb, vc);                   // (the lanes that hold one sum write it to one place)
+                        const int p = h0 + i;
+                        *(float2*)(my_red + (p >= at && p < end ? (p - t0) * W : SCAN_TILE * W)) = make_float2(vb[0], vb[1]);
+                    }
+                    // the lane's row of these four
+                    const float y = quad_rows<LPC>(ys, L.q), gb = quad_rows<LPC>(gbs, L.q), ga = quad_rows<LPC>(gas, L.q);
+                    const int r = t0 + 4 * k + L.q;
+                    const bool mine = L.in && (whole || (r >= at && r < end));
+                    const float uk = live && mine ? u[k] : 0.f;
+                    const float slope = a.softplus ? seq_sigmoid((float)raw_d[k] + bias) : 1.f;
+                    const float dd = live && mine ? fmaf(uk, gb, SEQ_LN2 * ga) * slope : 0.f;
+                    dbias += dd;
+                    dD = fmaf(d4[k], uk, dD);
+                    if (mine && L.j < 4) {
+                        scan_at(pu, scan_again(at_du) + 4 * k * (unsigned)a.lddu * sizeof(T)) = (T)fmaf(Dd, d4[k], s4[k] * gb);
+                        scan_at(pd, scan_again(at_dd) + 4 * k * (unsigned)a.lddd * sizeof(T)) = (T)dd;
+                        if (a.z) {
+                            const float z = (float)raw_z[k], sg = seq_sigmoid(z);
+                            const float dz = (float)raw_y[k] * fmaf(Dd, uk, y) * sg * fmaf(z, 1.f - sg, 1.f);
+                            scan_at(pz, scan_again(at_dz) + 4 * k * (unsigned)a.lddz * sizeof(T)) = (T)(live ? dz : 0.f);
+                        }
                     }
                 }
             }
-        }
-        // and back
-#pragma unroll
-        for (int k = 3; k >= 0; --k) {
-#pragma unroll
-            for (int q = 3; q >= 0; --q) {
-                const int i = 4 * k + q, p = t0 + i;
-                if (p < c1 && p < first) {                        // the row belongs to an earlier clip: its last row
+            end = at;
+            if (at == first && s >= 0) {                          // the clip started with the piece: on to the one in front
+                leave(s);
+                if (at > c0) {
                     const int was = s;
-                    while (s >= 0 && seq_start(a.clips, s) > p) --s;
-                    first = s >= 0 ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, s)) : -1;
-                    if (a.dstate && L.in) for (int e = s + 1; e < was; ++e) empty(e);
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) g[m] = 0.f;
-                    if (a.dfinal && s >= 0) scan_load4(a.dfinal + ((size_t)s * a.channels + L.d) * N, L.j, N, g);
-                }
-                const float sb = quad_bcast(st[k], q), xb = quad_bcast(x[k], q), db = quad_bcast(dy[k], q);
-                const seq_f4 b4 = *(const seq_f4*)(sB[buf] + i * N4 + 4 * L.j);
-                const seq_f4 c4 = *(const seq_f4*)(sC[buf] + i * N4 + 4 * L.j);
-                float y = 0.f, gb = 0.f, ga = 0.f, vb[4], vc[4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const float e = seq_exp2(sb * A2[m]), ah = e * hp[i][m];
-                    const float ht = fmaf(xb, b4[m], ah);
-                    y = fmaf(c4[m], ht, y);
-                    g[m] = fmaf(c4[m], db, g[m]);
-                    vb[m] = g[m] * xb;
-                    vc[m] = db * ht;
-                    gb = fmaf(g[m], b4[m], gb);
-                    const float f = g[m] * ah;
-                    ga = fmaf(A2[m], f, ga);
-                    dA[m] = fmaf(sb, f, dA[m]);
-                    g[m] *= e;
-                }
-                if (a.dstate && p == first && p < c1 && s >= 0 && s < n && L.in)
-                    scan_store4(a.dstate + ((size_t)s * a.channels + L.d) * N, L.j, N, g);
-                y = chan_sum<LPC>(y); gb = chan_sum<LPC>(gb); ga = chan_sum<LPC>(ga);
-                const bool mine = L.q == q;
-                ys[k] = mine ? y : ys[k]; sb_[k] = mine ? gb : sb_[k]; sa_[k] = mine ? ga : sa_[k];
-                if (!L.in) {
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) { vb[m] = 0.f; vc[m] = 0.f; }
-                }
-                wave_fold<LPC>(vb, vc);
-                if ((lane & 15) < LPC) {
-                    float* w2 = red[wave] + i * W + (lane >> 5) * N4 + 4 * L.j + 2 * ((lane >> 4) & 1);
-                    w2[0] = vb[0]; w2[1] = vb[1];
+                    while (s >= 0 && seq_start(a.clips, s) >= at) --s;
+                    first = s >= 0 ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, s)) : 0;
+                    if (a.dstate) for (int e = s + 1; e < was; ++e) { entry(e); leave(e); }
+                    entry(s);
                 }
             }
+        } while (end > t0);
+        if (more) {
+            stB.store(sB[buf ^ 1], t0 - SCAN_TILE, lo, hi);
+            stC.store(sC[buf ^ 1], t0 - SCAN_TILE, lo, hi);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int r = t0 + 4 * k + L.q;
-            const bool live = r >= lo && r < min(hi, c1);
-            const float raw = (float)raw_d[k] + bias;
-            const float slope = a.softplus ? seq_sigmoid(raw) : 1.f;
-            const float du = fmaf(Dd, dy[k], st[k] * sb_[k]);
-            const float dd = live ? fmaf(u[k], sb_[k], SEQ_LN2 * sa_[k]) * slope : 0.f;
-            dbias += dd;
-            dD = fmaf(dy[k], u[k], dD);
-            if (r < c1 && L.in && L.j < 4) {
-                ((T*)a.du)[(int64_t)r * a.lddu + L.d] = (T)du;
-                ((T*)a.ddelta)[(int64_t)r * a.lddd + L.d] = (T)dd;
-                if (a.z) {
-                    const float z = (float)raw_z[k], sg = seq_sigmoid(z);
-                    const float dz = (float)raw_y[k] * fmaf(Dd, u[k], ys[k]) * sg * fmaf(z, 1.f - sg, 1.f);
-                    ((T*)a.dz)[(int64_t)r * a.lddz + L.d] = (T)(live ? dz : 0.f);
-                }
-            }
-        }
-        __syncthreads();                                          // red complete; sB / sC of the next tile staged
+        __syncthreads();                                          // red complete; B and C of the next tile in place
         for (int e = threadIdx.x; e < SCAN_TILE * W; e += 256) {
             const int r = t0 + e / W;
             if (r < c1) a.part_bc[((int64_t)blockIdx.x * a.rows + r) * W + e % W] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
         }
         __syncthreads();                                          // red read
     }
-    if (a.dstate && L.in && chunk == 0) {                         // empty clips in front of the first row
+    if (a.dstate && chunk == 0) {                                 // empty clips in front of the first row
         const int s0 = seq_find(a.clips, 0);
-        for (int e = 0; e < s0 && e < n; ++e) empty(e);
+        for (int e = 0; e < s0 && e < n; ++e) { entry(e); leave(e); }
     }
     dD += seq_dpp<0xB1>(dD); dD += seq_dpp<0x4E>(dD);
     dbias += seq_dpp<0xB1>(dbias); dbias += seq_dpp<0x4E>(dbias);
@@ -680,6 +749,9 @@ static bool scan_shape_ok(int64_t rows, int channels, int n_state, int dtype) {
            dtype >= 0 && dtype <= 2;
 }
 
+// a tile's rows are addressed by 32-bit offsets from its first
+static bool scan_ld_ok(int64_t ld, int width) { return ld >= width && ld <= (1 << 24); }
+
 static int64_t scan_carry_floats(int chunks, int channels, int n_state) {
     if (chunks <= 1) return 4;
     const int n4 = 4 * scan_lpc(n_state);
@@ -740,7 +812,7 @@ extern "C" int eventad_selective_scan_workspace(int64_t rows, int channels, int 
 
 extern "C" int eventad_selective_scan_checkpoint(int64_t rows, int channels, int n_state, int64_t* bytes) {
     if (!bytes || !scan_shape_ok(rows, channels, n_state, 0)) return EVAD_ERR_ARG;
-    *bytes = (rows + SCAN_TILE - 1) / SCAN_TILE * channels * 16 * scan_lpc(n_state);
+    *bytes = (rows + SCAN_KEEP - 1) / SCAN_KEEP * channels * 16 * scan_lpc(n_state);
     return EVAD_OK;
 }
 
@@ -748,7 +820,8 @@ static bool scan_common(ScanArgs& a, const void* u, int64_t ldu, const void* del
                         int64_t ldb, const void* C, int64_t ldc, const float* D, const void* z, int64_t ldz, const float* bias,
                         int64_t rows, int channels, int n_state, int softplus, int dtype) {
     if (!scan_shape_ok(rows, channels, n_state, dtype) || !A || softplus < 0 || softplus > 1) return false;
-    if (rows && (!u || !delta || !B || !C || ldu < channels || ldd < channels || ldb < n_state || ldc < n_state || (z && ldz < channels))) return false;
+    if (rows && (!u || !delta || !B || !C || !scan_ld_ok(ldu, channels) || !scan_ld_ok(ldd, channels) || !scan_ld_ok(ldb, n_state) ||
+                 !scan_ld_ok(ldc, n_state) || (z && !scan_ld_ok(ldz, channels)))) return false;
     a.u = u; a.ldu = ldu; a.delta = delta; a.ldd = ldd; a.A = A; a.B = B; a.ldb = ldb; a.C = C; a.ldc = ldc; a.D = D;
     a.z = z; a.ldz = ldz; a.bias = bias; a.rows = (int)rows; a.channels = channels; a.n_state = n_state; a.softplus = softplus;
     return true;
@@ -763,7 +836,7 @@ extern "C" int eventad_selective_scan_fwd(const void* u, int64_t ldu, const void
     ScanArgs a = {};
     int64_t need = 0;
     if (!scan_common(a, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, delta_bias, rows, channels, n_state, softplus, dtype) ||
-        clips < 1 || (!clip_start && clips != 1) || (rows && (!y || ldy < channels)) || ((uintptr_t)checkpoint & 15) ||
+        clips < 1 || (!clip_start && clips != 1) || (rows && (!y || !scan_ld_ok(ldy, channels))) || ((uintptr_t)checkpoint & 15) ||
         eventad_selective_scan_workspace(rows, channels, n_state, 0, &need) != EVAD_OK || !workspace || workspace_bytes < need ||
         ((uintptr_t)workspace & 15)) return EVAD_ERR_ARG;
     a.clips = SeqClips{clip_start, clips, (int)rows};
@@ -792,8 +865,8 @@ extern "C" int eventad_selective_scan_bwd(const void* u, int64_t ldu, const void
     int64_t need = 0;
     if (!scan_common(a, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, delta_bias, rows, channels, n_state, softplus, dtype) ||
         clips < 1 || (!clip_start && clips != 1) || !dparams || ((uintptr_t)checkpoint & 15) ||
-        (rows && (!dy || !du || !ddelta || !dB || !dC || !checkpoint || lddy < channels || lddu < channels || lddd < channels ||
-                  lddb < n_state || lddc < n_state || (z && (!dz || lddz < channels)))) ||
+        (rows && (!dy || !du || !ddelta || !dB || !dC || !checkpoint || !scan_ld_ok(lddy, channels) || !scan_ld_ok(lddu, channels) ||
+                  !scan_ld_ok(lddd, channels) || lddb < n_state || lddc < n_state || (z && (!dz || !scan_ld_ok(lddz, channels))))) ||
         eventad_selective_scan_workspace(rows, channels, n_state, 1, &need) != EVAD_OK || !workspace || workspace_bytes < need ||
         ((uintptr_t)workspace & 15)) return EVAD_ERR_ARG;
     a.clips = SeqClips{clip_start, clips, (int)rows};

@@ -12,6 +12,7 @@ Every function launches on the current stream of its tensors' device, waits for 
 workspaces come from torch's allocator per call, so captured graphs do not share one.  The functions are differentiable
 (except the single-token and 8-bit forms, which refuse inputs that need a gradient); gradients are not differentiable
 again.  There is no CPU path: tensors must be on a GPU."""
+import contextlib
 import ctypes
 
 import torch
@@ -28,40 +29,48 @@ def _fail(msg, *args):
     raise RuntimeError("eventad_amd.sequence: " + msg % args)
 
 
-def _activation(name, t, shape, like=None):
-    """Checks t [rows, channels]; returns it with adjacent channels."""
+_MAX_LD = 1 << 24               # row strides above this are taken by copying the array
+
+
+def _activation(name, t, rows, width, like=None):
+    """Checks t [rows, width] (None: any); returns it with adjacent channels."""
     if not isinstance(t, torch.Tensor):
         _fail("%s must be a tensor", name)
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        _fail("%s is %s on %s, expected %s on %s", name, t.dtype, t.device, like.dtype, like.device)
-    if t.dtype not in _DTYPE:
+    if like is not None:
+        if t.dtype != like.dtype or t.device != like.device:
+            _fail("%s is %s on %s, expected %s on %s", name, t.dtype, t.device, like.dtype, like.device)
+    elif t.dtype not in _DTYPE:
         _fail("%s must be float32, bfloat16 or float16, not %s", name, t.dtype)
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        _fail("%s has shape %s, expected %s", name, tuple(t.shape), tuple("*" if n is None else n for n in shape))
-    if len(shape) == 2:
-        if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
-            return t
-        return t.contiguous()
-    return t if t.is_contiguous() else t.contiguous()
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (width is not None and shape[1] != width):
+        _fail("%s has shape %s, expected %s", name, tuple(shape), ("*" if rows is None else rows, "*" if width is None else width))
+    ld, step = t.stride()
+    if step == 1 and (shape[1] <= ld <= _MAX_LD or shape[0] <= 1):
+        return t
+    return t.contiguous()
 
 
-def _param(name, t, shape, device):
+def _tensor(name, t, shape, dtype, device):
+    """Checks a parameter or a state; returns it contiguous."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device:
-        _fail("%s must be a float32 tensor on %s", name, device)
-    if tuple(t.shape) != tuple(shape):
-        _fail("%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+        _fail("%s must be a %s tensor on %s", name, dtype, device)
+    if t.shape != shape:
+        _fail("%s has shape %s, expected %s", name, tuple(t.shape), shape)
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _ld(t):
     """Row stride in elements (an array of at most one row may have any)."""
-    return max(t.stride(0), t.shape[1]) if t is not None else 0
+    if t is None:
+        return 0
+    ld, width = t.stride(0), t.shape[1]
+    return ld if width <= ld <= _MAX_LD else width
 
 
 def _p(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
 def _clips(clip_start, rows, device):
@@ -74,13 +83,17 @@ def _clips(clip_start, rows, device):
 
 
 def _gpu(t):
-    if not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _fail("tensors must be on a GPU (there is no CPU path)")
     return t.device
 
 
 def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _bytes(name, *shape):
@@ -93,19 +106,12 @@ def _workspace(nbytes, device):
     return torch.empty(max(16, nbytes), dtype=torch.uint8, device=device)
 
 
-class _on:
-    """Makes the tensors' device current for the launches (a no-op when it is)."""
+_HERE = contextlib.nullcontext()
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on(device):
+    """Makes the tensors' device current for the launches."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 # ---------------------------------------------------------------------------------------------------- causal convolution
@@ -133,7 +139,7 @@ class _ConvFn(torch.autograd.Function):
         rows, D = x.shape
         K = w.shape[1]
         with _on(x.device):
-            dy = torch.zeros_like(x) if dy is None else _activation("the gradient", dy, (rows, D), x)
+            dy = torch.zeros_like(x) if dy is None else _activation("the gradient", dy, rows, D, x)
             dfinal = None if dfinal is None else dfinal.contiguous()
             dx = torch.empty((rows, D), dtype=x.dtype, device=x.device)
             dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[5] else None
@@ -149,14 +155,14 @@ def _conv_args(x, weight, bias, state, activation, clips):
     dev = _gpu(x)
     if activation not in _ACT:
         _fail("activation must be None or 'silu', not %r", activation)
-    x = _activation("x", x, (None, None))
+    x = _activation("x", x, None, None)
     D = x.shape[1]
-    if D < 1 or weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_TAPS:
+    taps = weight.shape[1] if isinstance(weight, torch.Tensor) and weight.dim() == 2 else 0
+    if D < 1 or not 1 <= taps <= MAX_TAPS:
         _fail("weight must be [channels, taps] with 1..%d taps, x [rows, channels] with at least one channel", MAX_TAPS)
-    weight = _param("weight", weight, (D, weight.shape[1]), dev)
-    bias = _param("bias", bias, (D,), dev)
-    if state is not None:
-        state = _activation("state", state, (clips, weight.shape[1] - 1, D), x)
+    weight = _tensor("weight", weight, (D, taps), torch.float32, dev)
+    bias = _tensor("bias", bias, (D,), torch.float32, dev)
+    state = _tensor("state", state, (clips, taps - 1, D), x.dtype, dev)
     return x, weight, bias, state, _ACT[activation]
 
 
@@ -237,7 +243,7 @@ class _ScanFn(torch.autograd.Function):
         rows, ch = u.shape
         N = A.shape[1]
         with _on(u.device):
-            dy = torch.zeros_like(u) if dy is None else _activation("the gradient", dy, (rows, ch), u)
+            dy = torch.zeros_like(u) if dy is None else _activation("the gradient", dy, rows, ch, u)
             dfinal = None if dfinal is None else dfinal.contiguous()
             new = lambda n: torch.empty((rows, n), dtype=u.dtype, device=u.device)
             du, dd, dB, dC, dz = new(ch), new(ch), new(N), new(N), new(ch) if z is not None else None
@@ -254,20 +260,18 @@ class _ScanFn(torch.autograd.Function):
 
 
 def _scan_args(u, delta, A, B, C, D, z, bias, state, clips):
-    dev = _gpu(u)
-    u = _activation("u", u, (None, None))
+    dev, f32 = _gpu(u), torch.float32
+    u = _activation("u", u, None, None)
     rows, ch = u.shape
     if ch < 1 or not isinstance(A, torch.Tensor) or A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
         _fail("A must be [channels, states] with 1..%d states, u [rows, channels] with at least one channel", MAX_STATE)
     N = A.shape[1]
-    delta = _activation("delta", delta, (rows, ch), u)
-    A = _param("A", A, (ch, N), dev)
-    B, C = _activation("B", B, (rows, N), u), _activation("C", C, (rows, N), u)
-    D, bias = _param("D", D, (ch,), dev), _param("delta_bias", bias, (ch,), dev)
-    z = None if z is None else _activation("z", z, (rows, ch), u)
-    if state is not None:
-        checked = _param("state", state, (clips, ch, N), dev)
-        state = checked
+    delta = _activation("delta", delta, rows, ch, u)
+    A = _tensor("A", A, (ch, N), f32, dev)
+    B, C = _activation("B", B, rows, N, u), _activation("C", C, rows, N, u)
+    D, bias = _tensor("D", D, (ch,), f32, dev), _tensor("delta_bias", bias, (ch,), f32, dev)
+    z = None if z is None else _activation("z", z, rows, ch, u)
+    state = _tensor("state", state, (clips, ch, N), f32, dev)
     return u, delta, A, B, C, D, z, bias, state
 
 
@@ -312,15 +316,15 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
 # ------------------------------------------------------------------------------------------------------------- RMS norm
 def _norm_args(x, weight, residual, eps):
     dev = _gpu(x)
-    x = _activation("x", x, (None, None))
+    x = _activation("x", x, None, None)
     if x.shape[1] < 1:
         _fail("x must have at least one channel")
     if not float(eps) >= 0.0:
         _fail("eps must not be negative")
     if weight is None:
         _fail("weight must be a float32 tensor")
-    weight = _param("weight", weight, (x.shape[1],), dev)
-    residual = None if residual is None else _activation("residual", residual, tuple(x.shape), x)
+    weight = _tensor("weight", weight, (x.shape[1],), torch.float32, dev)
+    residual = None if residual is None else _activation("residual", residual, x.shape[0], x.shape[1], x)
     return x, weight, residual, float(eps)
 
 
@@ -348,8 +352,8 @@ class _NormFn(torch.autograd.Function):
         h, weight = ctx.saved_tensors
         rows, D = h.shape
         with _on(h.device):
-            dy = torch.zeros_like(h) if dy is None else _activation("the gradient", dy, (rows, D), h)
-            dtotal = None if dtotal is None else _activation("the gradient", dtotal, (rows, D), h)
+            dy = torch.zeros_like(h) if dy is None else _activation("the gradient", dy, rows, D, h)
+            dtotal = None if dtotal is None else _activation("the gradient", dtotal, rows, D, h)
             dh = torch.empty((rows, D), dtype=h.dtype, device=h.device)
             dw = torch.empty(D, device=h.device)
             ws = _workspace(_bytes("eventad_rms_norm_workspace", rows, D), h.device)

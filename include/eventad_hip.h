@@ -508,8 +508,8 @@ int eventad_incr_pool0(const float* y2, const float* map_nhwc, int map_h, int ma
 /* A causal convolution, a selective state-space scan and a root-mean-square norm: what a state-space block over a clip's
  * events or nodes needs beside its matrix products, each with its gradient and its form for one token per clip (the dense
  * pass and the event-by-event update of groups (B)-(K), for a recurrence over the rows themselves).
- * Arrays of activations are [rows, channels] with a row stride in elements (ld* >= channels; adjacent channels are adjacent
- * in memory), of type dtype = 0 float32, 1 bfloat16, 2 float16, all of one call alike; parameters and scan states are
+ * Arrays of activations are [rows, channels] with a row stride in elements (channels <= ld* <= 2^24; adjacent channels are
+ * adjacent in memory), of type dtype = 0 float32, 1 bfloat16, 2 float16, all of one call alike; parameters and scan states are
  * float32, sums are formed in float32.  Rows are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1, clip_start
  * i32[clips+1] on the device, not decreasing, within 0..rows (NULL with clips = 1: all rows are one clip).  Rows of no
  * clip are neither read into a result nor counted in a gradient; their outputs and gradients are written as zeros.
