@@ -698,48 +698,71 @@ __global__ __launch_bounds__(256) void k_scan_bc(const float* __restrict__ part,
     if (c) dC[r * lddc + i] = (T)(s0 + s1); else dB[r * lddb + i] = (T)(s0 + s1);
 }
 
-// One token per clip.  A lane owns four states of a channel: it reads 16 bytes of state and writes 16.  VEC: N is a multiple
-// of 4 and both states are 16-byte aligned.  state_out may be the state itself.
+// One token per clip, bound by the bytes of the states: 4 N in and 4 N out per channel.  A lane owns four states of a channel
+// (16 bytes each way) and goes over four clips at a time, so that four states are requested before the first is used and the
+// lanes of a quad form the step and the gate of one clip each.  VEC: rows of A, B, C and the states are whole and aligned groups
+// of four; otherwise they are read entry by entry.  state_out may be the state itself: a lane reads its entries before it
+// writes them and nobody else needs them.
+template <typename T> struct SeqQuad;
+template <> struct SeqQuad<float> { typedef seq_f4 type; };
+template <> struct SeqQuad<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
+template <> struct SeqQuad<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
+
+template <typename T, bool VEC> __device__ __forceinline__ void step_load4(const T* __restrict__ row, int j, int N, float (&v)[4]) {
+    if constexpr (VEC) {
+        typename SeqQuad<T>::type w = {};
+        if (4 * j < N) w = *(const typename SeqQuad<T>::type*)(row + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = 4 * j + i < N ? (float)row[4 * j + i] : 0.f;
+    }
+}
+
 template <typename T, int LPC, bool VEC>
 __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPC;
-    const int j = threadIdx.x % LPC, N = a.n_state;
-    const int64_t total = (int64_t)a.rows * a.channels;
-    const bool in = at < total;
-    const int64_t cell = in ? at : total - 1;
-    const int s = (int)(cell / a.channels), d = (int)(cell - (int64_t)s * a.channels);
-    float h[4], A[4], b[4], c[4];
-    const float* src = a.state + cell * N;
-    const bool mine = 4 * j < N;
-    if constexpr (VEC) {
-        seq_f4 v = {0.f, 0.f, 0.f, 0.f}, w = {0.f, 0.f, 0.f, 0.f};
-        if (mine) { v = *(const seq_f4*)(src + 4 * j); w = *(const seq_f4*)(a.A + (size_t)d * N + 4 * j); }
+    const ScanLane<LPC> L(a);
+    const int N = a.n_state;
+    float A2[4];
+    step_load4<float, VEC>(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { h[i] = v[i]; A[i] = w[i]; }
-    } else { scan_load4(src, j, N, h); scan_load4(a.A + (size_t)d * N, j, N, A); }
+    for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
+    const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
+    for (int s0 = blockIdx.y * 4; s0 < a.rows; s0 += gridDim.y * 4) {
+        const int64_t mine = min(s0 + L.q, a.rows - 1);           // the clip whose step and output this lane forms
+        float h[4][4], b[4][4], c[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        b[i] = 4 * j + i < N ? (float)((const T*)a.B)[(int64_t)s * a.ldb + 4 * j + i] : 0.f;
-        c[i] = 4 * j + i < N ? (float)((const T*)a.C)[(int64_t)s * a.ldc + 4 * j + i] : 0.f;
-    }
-    const float u = (float)((const T*)a.u)[(int64_t)s * a.ldu + d];
-    const float raw = (float)((const T*)a.delta)[(int64_t)s * a.ldd + d] + (a.bias ? a.bias[d] : 0.f);
-    const float st = a.softplus ? scan_softplus(raw) : raw, x = st * u;
-    float acc = 0.f;
+        for (int q = 0; q < 4; ++q) {
+            const int64_t s = min(s0 + q, a.rows - 1);
+            step_load4<float, VEC>(a.state + (s * a.channels + L.d) * N, L.j, N, h[q]);
+            step_load4<T, VEC>((const T*)a.B + s * a.ldb, L.j, N, b[q]);
+            step_load4<T, VEC>((const T*)a.C + s * a.ldc, L.j, N, c[q]);
+        }
+        const float u = (float)((const T*)a.u)[mine * a.ldu + L.d];
+        const float raw = (float)((const T*)a.delta)[mine * a.ldd + L.d] + bias;
+        const float z = a.z ? (float)((const T*)a.z)[mine * a.ldz + L.d] : 0.f;
+        const float st = a.softplus ? scan_softplus(raw) : raw, x = st * u;
+        float acc[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h[i] = fmaf(seq_exp2(st * (A[i] * SEQ_LOG2E)), h[i], x * b[i]);
-        acc = fmaf(c[i], h[i], acc);
-    }
-    acc = chan_sum<LPC>(acc);
-    if (!in) return;
-    float* dst = a.final_state + cell * N;
-    if constexpr (VEC) { if (mine) *(seq_f4*)(dst + 4 * j) = seq_f4{h[0], h[1], h[2], h[3]}; }
-    else scan_store4(dst, j, N, h);
-    if (j == 0) {
-        float y = fmaf(a.D ? a.D[d] : 0.f, u, acc);
-        if (a.z) { const float z = (float)((const T*)a.z)[(int64_t)s * a.ldz + d]; y *= z * seq_sigmoid(z); }
-        ((T*)a.y)[(int64_t)s * a.ldy + d] = (T)y;
+        for (int q = 0; q < 4; ++q) {
+            const float sb = quad_bcast(st, q), xb = quad_bcast(x, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[q][i] = fmaf(seq_exp2(sb * A2[i]), h[q][i], xb * b[q][i]);
+                acc[q] = i ? fmaf(c[q][i], h[q][i], acc[q]) : c[q][0] * h[q][0];
+            }
+        }
+        const float y = fmaf(Dd, u, quad_rows<LPC>(acc, L.q)) * (a.z ? z * seq_sigmoid(z) : 1.f);
+        if (!L.in) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (s0 + q >= a.rows) break;
+            float* dst = a.final_state + ((int64_t)(s0 + q) * a.channels + L.d) * N;
+            if constexpr (VEC) { if (4 * L.j < N) *(seq_f4*)(dst + 4 * L.j) = seq_f4{h[q][0], h[q][1], h[q][2], h[q][3]}; }
+            else scan_store4(dst, L.j, N, h[q]);
+        }
+        if (L.j < 4 && s0 + L.q < a.rows) ((T*)a.y)[mine * a.ldy + L.d] = (T)y;
     }
 }
 
@@ -787,8 +810,13 @@ template <int WHAT, typename T, int LPC> static int scan_launch2(const ScanArgs&
     if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_adj<T, LPC>), grid, block, 0, st, a);
     if constexpr (WHAT == 3) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bwd<T, LPC>), grid, block, 0, st, a);
     if constexpr (WHAT == 4) {
-        const bool vec = a.n_state % 4 == 0 && seq_aligned(a.state, 0) && seq_aligned(a.final_state, 0) && seq_aligned(a.A, 0);
-        const dim3 g(evad_blocks((long long)a.rows * a.channels * LPC, 256));
+        const int bytes = 4 * sizeof(T);
+        auto quads = [&](const void* p, int64_t ld) { return ((uintptr_t)p | (uintptr_t)(ld * (int64_t)sizeof(T))) % bytes == 0; };
+        const bool vec = a.n_state % 4 == 0 && seq_aligned(a.state, 0) && seq_aligned(a.final_state, 0) && seq_aligned(a.A, 0) &&
+                         quads(a.B, a.ldb) && quads(a.C, a.ldc);
+        // enough workgroups to fill the chip (8 per CU); beyond that a workgroup goes over more clips with the same A
+        const int64_t most = (2048 + grid.x - 1) / grid.x, fours = ((int64_t)a.rows + 3) / 4;
+        const dim3 g(grid.x, (unsigned)(fours < most ? fours : most));
         if (vec) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<T, LPC, true>), g, block, 0, st, a);
         else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<T, LPC, false>), g, block, 0, st, a);
     }
