@@ -297,7 +297,7 @@ template <int WHAT, typename T, int V> static void norm_launch2(const NormArgs& 
     else norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
 }
 template <int WHAT, typename T> static void norm_launch1(const NormArgs& a, bool vec, int groups, hipStream_t st) {
-    constexpr int N = SeqVec<T>::n;
+    constexpr int N = 16 / sizeof(T);
     if (vec && a.channels % N == 0) norm_launch2<WHAT, T, N>(a, groups, st); else norm_launch2<WHAT, T, 1>(a, groups, st);
 }
 template <int WHAT> static int norm_launch(const NormArgs& a, int dtype, bool vec, int groups, hipStream_t st) {

@@ -14,21 +14,15 @@
 #define SEQ_F16 2
 
 typedef float seq_f4 __attribute__((ext_vector_type(4)));
-typedef _Float16 seq_h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 seq_b8 __attribute__((ext_vector_type(8)));
 
-// what one 16-byte access of a type holds
-template <typename T> struct SeqVec;
-template <> struct SeqVec<float> { typedef seq_f4 type; static constexpr int n = 4; };
-template <> struct SeqVec<_Float16> { typedef seq_h8 type; static constexpr int n = 8; };
-template <> struct SeqVec<__bf16> { typedef seq_b8 type; static constexpr int n = 8; };
+// V elements of a type as one access
+template <typename T, int V> struct SeqVec { typedef T type __attribute__((ext_vector_type(V))); };
 
-// V elements at p as floats / back, rounded to nearest even: one 16-byte access, or (V = 1) one element
+// V elements at p as floats / back, rounded to nearest even
 template <typename T, int V> __device__ __forceinline__ void seq_load(const T* __restrict__ p, float (&out)[V]) {
     if constexpr (V == 1) out[0] = (float)*p;
     else {
-        static_assert(V == SeqVec<T>::n, "one 16-byte access");
-        const typename SeqVec<T>::type v = *(const typename SeqVec<T>::type*)p;
+        const typename SeqVec<T, V>::type v = *(const typename SeqVec<T, V>::type*)p;
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = (float)v[i];
     }
@@ -36,10 +30,24 @@ template <typename T, int V> __device__ __forceinline__ void seq_load(const T* _
 template <typename T, int V> __device__ __forceinline__ void seq_store(T* __restrict__ p, const float (&in)[V]) {
     if constexpr (V == 1) *p = (T)in[0];
     else {
-        typename SeqVec<T>::type v;
+        typename SeqVec<T, V>::type v;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = (T)in[i];
-        *(typename SeqVec<T>::type*)p = v;
+        *(typename SeqVec<T, V>::type*)p = v;
+    }
+}
+
+// the same in two steps: request now, convert when it is there
+template <typename T, int V> struct SeqRaw { typedef typename SeqVec<T, V>::type type; };
+template <typename T> struct SeqRaw<T, 1> { typedef T type; };
+template <typename T, int V> __device__ __forceinline__ typename SeqRaw<T, V>::type seq_raw(const T* __restrict__ p) {
+    return *(const typename SeqRaw<T, V>::type*)p;
+}
+template <typename T, int V> __device__ __forceinline__ void seq_unpack(const typename SeqRaw<T, V>::type& v, float (&out)[V]) {
+    if constexpr (V == 1) out[0] = (float)v;
+    else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = (float)v[i];
     }
 }
 

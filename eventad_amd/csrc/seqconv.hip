@@ -7,73 +7,116 @@
 // d_t = dy_t act'(pre_t):  dx_t = sum_k w[:,k] d_{t+(K-1)-k} inside the clip,  dw[:,k] = sum_t d_t x_{t-(K-1)+k},
 // dbias = sum_t d_t.
 //
-// All of it is bound by bytes (2K + 4 operations per element that is read and written once).  A thread owns one 16-byte
-// column of a chunk of rows and slides down it with the K-1 inputs before the current row in registers, so a row is read
-// once plus (K-1) / chunk for the chunk's start.
+// All of it is bound by bytes (2K + 4 operations per element that is read and written once).  A thread owns four adjacent
+// channels (one, where rows are not aligned to four) of a chunk of rows and slides down it with the K-1 inputs before the current
+// row in registers, so a row is read once plus (K-1) / chunk for the chunk's start.  Rows go by in groups of four, requested
+// a group ahead; a group that meets a clip's or the chunk's border goes row by row instead, reading again what it needs.
+// Four channels and not the eight that 16 bytes of a 16-bit type hold: weights and windows of eight are 128 registers, and the
+// waves that fit beside them do not cover the memory's latency.
+// WAVE: with 64 columns or more a wave has one chunk, and the walk over the clips is scalar; narrower arrays put several chunks
+// into a wave.
 #include "seq.h"
 
 #define CONV_MAX_TAPS 8
-#define CONV_AHEAD 4                 // rows requested before the first of them is used
+#define CONV_GROUP 4
+#define CONV_PAIR 2                  // the gradient's group: two arrays in, and collectors beside the window
 
 struct ConvArgs {
     SeqClips clips;
     const void* x; int64_t ldx;
     const float* w; const float* bias;
-    const void* state; void* final_state;            // [clips][K-1][channels]
+    const void* state; void* final_state;            // [clips][taps-1][channels]
     void* y; int64_t ldy;
-    int rows, channels, cols, chunk_rows, chunks, act;
+    int rows, channels, cols, chunk_rows, chunks, act, taps;
     // gradient
     const void* dy; int64_t lddy;
     const void* dfinal; void* dstate;
     void* dx; int64_t lddx;
-    float* part;                                     // [chunks][channels*K + channels]
+    float* part;                                     // [chunks][channels*taps + channels]
 };
 
-// A thread's place: its columns, its rows, and the clip of its current row.
-template <typename T, int V, int K> struct ConvLane {
-    int c, r0, r1, s, next;                          // first channel; rows r0..r1-1; clip of the current row; where it ends
+// The kernels are built for K = 2, 3, 4 and 8 taps; K = 8 serves every other number: its first K - taps window entries are zero
+// and stay out of the sums.
+template <int K> __device__ __forceinline__ int conv_skip(const ConvArgs& a) { return K == 8 ? K - a.taps : 0; }
+
+template <bool WAVE> __device__ __forceinline__ int conv_same(int v) { return WAVE ? __builtin_amdgcn_readfirstlane(v) : v; }
+
+// A thread's place: its columns, its rows, its parameters.
+template <typename T, int V, int K, bool WAVE> struct ConvLane {
+    int c, r0, r1, chunk;                            // first channel; rows r0..r1-1
     float w[K][V], b[V];
-};
-
-template <typename T, int V, int K>
-__device__ __forceinline__ bool conv_lane(const ConvArgs& a, ConvLane<T, V, K>& L) {
-    const long long g = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int chunk = (int)(g / a.cols);
-    if (chunk >= a.chunks) return false;
-    L.c = (int)(g - (long long)chunk * a.cols) * V;
-    L.r0 = chunk * a.chunk_rows;
-    L.r1 = min(a.rows, L.r0 + a.chunk_rows);
+    __device__ __forceinline__ bool place(const ConvArgs& a) {
+        if constexpr (WAVE) {
+            const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), per = (a.cols + 63) / 64;
+            chunk = wave / per;
+            const int col = (int)(wave - chunk * per) * 64 + (threadIdx.x & 63);
+            c = col * V;
+            if (chunk >= a.chunks || col >= a.cols) return false;
+        } else {
+            const unsigned g = blockIdx.x * 256 + threadIdx.x;
+            chunk = g / a.cols;
+            c = (int)(g - chunk * a.cols) * V;
+            if (chunk >= a.chunks) return false;
+        }
+        r0 = chunk * a.chunk_rows;
+        r1 = min(a.rows, r0 + a.chunk_rows);
+        const int skip = conv_skip<K>(a);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        L.b[i] = a.bias ? a.bias[L.c + i] : 0.f;
+        for (int i = 0; i < V; ++i) {
+            b[i] = a.bias ? a.bias[c + i] : 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) L.w[k][i] = a.w[(size_t)(L.c + i) * K + k];
+            for (int k = 0; k < K; ++k) w[k][i] = k >= skip ? a.w[(size_t)(c + i) * a.taps + k - skip] : 0.f;
+        }
+        return true;
     }
-    L.s = seq_find(a.clips, L.r0);
-    L.next = L.s < a.clips.n ? seq_start(a.clips, L.s + 1) : 0x7fffffff;
-    return true;
-}
+    __device__ __forceinline__ void pre(const ConvArgs& a, const float (*win)[V], float (&out)[V]) const {   // win[0..K-1]
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = b[i];
+        const int skip = conv_skip<K>(a);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k >= skip)
+#pragma unroll
+                for (int i = 0; i < V; ++i) out[i] = fmaf(w[k][i], win[k][i], out[i]);
+    }
+};
 
 // the K-1 inputs in front of row p of clip s, which starts at `first`
 template <typename T, int V, int K>
-__device__ __forceinline__ void conv_window(const ConvArgs& a, int c, int s, int first, int p, float (&win)[K][V]) {
+__device__ __forceinline__ void conv_window(const ConvArgs& a, int c, int s, int first, int p, float (*win)[V]) {
+    const int skip = conv_skip<K>(a);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         const int q = p - (K - 1) + k;
 #pragma unroll
         for (int i = 0; i < V; ++i) win[k][i] = 0.f;
-        if (s < 0 || s >= a.clips.n) continue;
-        if (q >= first) seq_load<T, V>((const T*)a.x + (int64_t)q * a.ldx + c, win[k]);
-        else if (a.state) seq_load<T, V>((const T*)a.state + ((int64_t)s * (K - 1) + (K - 1 + q - first)) * a.channels + c, win[k]);
+        if (s < 0 || s >= a.clips.n || k < skip) continue;
+        float v[V];
+        if (q >= first) seq_load<T, V>((const T*)a.x + (int64_t)q * a.ldx + c, v);
+        else if (a.state) seq_load<T, V>((const T*)a.state + ((int64_t)s * (a.taps - 1) + (K - 1 - skip + q - first)) * a.channels + c, v);
+        else continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[k][i] = v[i];
     }
 }
 
-// out rows (K-1) of clip s = in rows of the same clip, or zeros
+// rows of a state of clip s: `rows` of K - 1 window entries, or the same clip's rows of `in`, or zeros
 template <typename T, int V, int K>
-__device__ __forceinline__ void conv_copy_state(const ConvArgs& a, int c, int s, const void* in, void* out) {
+__device__ __forceinline__ void conv_store_state(const ConvArgs& a, int c, int s, const float (*win)[V], void* out) {
+    const int skip = conv_skip<K>(a);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-        const int64_t at = ((int64_t)s * (K - 1) + k) * a.channels + c;
+        if (k < skip) continue;
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = win[k][i];
+        seq_store<T, V>((T*)out + ((int64_t)s * (a.taps - 1) + k - skip) * a.channels + c, v);
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void conv_copy_state(const ConvArgs& a, int c, int s, const void* in, void* out) {
+    for (int k = 0; k < a.taps - 1; ++k) {
+        const int64_t at = ((int64_t)s * (a.taps - 1) + k) * a.channels + c;
         float v[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = 0.f;
@@ -82,203 +125,272 @@ __device__ __forceinline__ void conv_copy_state(const ConvArgs& a, int c, int s,
     }
 }
 
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool WAVE>
 __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a) {
-    ConvLane<T, V, K> L;
-    if (!conv_lane<T, V, K>(a, L)) return;
+    ConvLane<T, V, K, WAVE> L;
+    if (!L.place(a)) return;
     const int n = a.clips.n, c = L.c;
-    int s = L.s, next = L.next;
-    float win[K][V];
+    int s = conv_same<WAVE>(seq_find(a.clips, L.r0));
+    int next = s < n ? conv_same<WAVE>(seq_start(a.clips, s + 1)) : 0x7fffffff;       // where the clip ends
+    float win[K - 1 + CONV_GROUP][V];
+    const T* x = (const T*)a.x + (int64_t)L.r0 * a.ldx + c;
+    typename SeqRaw<T, V>::type raw[CONV_GROUP];
+    auto request = [&](int p0) {
+#pragma unroll
+        for (int j = 0; j < CONV_GROUP; ++j) raw[j] = seq_raw<T, V>(x + (int64_t)(min(p0 + j, L.r1 - 1) - L.r0) * a.ldx);
+    };
+    if (L.r1 > L.r0) request(L.r0);
     if (a.final_state)                                          // empty clips at the chunk's first row keep their state
-        for (int e = s - 1; e >= 0 && seq_start(a.clips, e) == L.r0; --e) conv_copy_state<T, V, K>(a, c, e, a.state, a.final_state);
+        for (int e = s - 1; e >= 0 && seq_start(a.clips, e) == L.r0; --e) conv_copy_state<T, V>(a, c, e, a.state, a.final_state);
     conv_window<T, V, K>(a, c, s, s >= 0 ? seq_start(a.clips, s) : 0, L.r0, win);
-    for (int p0 = L.r0; p0 < L.r1; p0 += CONV_AHEAD) {
-        float x[CONV_AHEAD][V];
+    auto row = [&](int p, const float (*w)[V], bool live) {
+        float y[V];
+        L.pre(a, w, y);
 #pragma unroll
-        for (int j = 0; j < CONV_AHEAD; ++j) seq_load<T, V>((const T*)a.x + (int64_t)min(p0 + j, L.r1 - 1) * a.ldx + c, x[j]);
+        for (int i = 0; i < V; ++i) {
+            if (a.act) y[i] *= seq_sigmoid(y[i]);
+            if (!live) y[i] = 0.f;
+        }
+        seq_store<T, V>((T*)a.y + (int64_t)p * a.ldy + c, y);
+    };
+    for (int p0 = L.r0; p0 < L.r1; p0 += CONV_GROUP) {
+        float now[CONV_GROUP][V];
 #pragma unroll
-        for (int j = 0; j < CONV_AHEAD; ++j) {
-            const int p = p0 + j;
-            if (p >= L.r1) break;
-            if (p >= next && s < n) {                           // the clip ended in front of this row
-                if (a.final_state && s >= 0 && p > L.r0) {
+        for (int j = 0; j < CONV_GROUP; ++j) seq_unpack<T, V>(raw[j], now[j]);
+        request(p0 + CONV_GROUP);
+        if (s >= 0 && s < n && next >= p0 + CONV_GROUP && L.r1 >= p0 + CONV_GROUP) {
 #pragma unroll
-                    for (int k = 0; k < K - 1; ++k) seq_store<T, V>((T*)a.final_state + ((int64_t)s * (K - 1) + k) * a.channels + c, win[k]);
-                }
-                ++s;
-                while (s < n && seq_start(a.clips, s + 1) <= p) {
-                    if (a.final_state) conv_copy_state<T, V, K>(a, c, s, a.state, a.final_state);
-                    ++s;
-                }
-                next = s < n ? seq_start(a.clips, s + 1) : 0x7fffffff;
-                conv_window<T, V, K>(a, c, s, p, p, win);
-            }
+            for (int j = 0; j < CONV_GROUP; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) win[K - 1][i] = x[j][i];
-            float y[V];
-            const bool live = s >= 0 && s < n;
+                for (int i = 0; i < V; ++i) win[K - 1 + j][i] = now[j][i];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float acc = L.b[i];
-#pragma unroll
-                for (int k = 0; k < K; ++k) acc = fmaf(L.w[k][i], win[k][i], acc);
-                y[i] = live ? (a.act ? acc * seq_sigmoid(acc) : acc) : 0.f;
-            }
-            seq_store<T, V>((T*)a.y + (int64_t)p * a.ldy + c, y);
+            for (int j = 0; j < CONV_GROUP; ++j) row(p0 + j, win + j, true);
 #pragma unroll
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+                for (int i = 0; i < V; ++i) win[k][i] = win[k + CONV_GROUP][i];
+        } else {
+#pragma unroll 1
+            for (int p = p0; p < min(p0 + CONV_GROUP, L.r1); ++p) {
+                if (p >= next && s < n) {                       // the clip ended in front of this row
+                    if (a.final_state && s >= 0) conv_store_state<T, V, K>(a, c, s, win, a.final_state);
+                    ++s;
+                    while (s < n && seq_start(a.clips, s + 1) <= p) {
+                        if (a.final_state) conv_copy_state<T, V>(a, c, s, a.state, a.final_state);
+                        ++s;
+                    }
+                    next = s < n ? conv_same<WAVE>(seq_start(a.clips, s + 1)) : 0x7fffffff;
+                    conv_window<T, V, K>(a, c, s, p, p, win);
+                }
+                float v[V];
+                seq_load<T, V>((const T*)a.x + (int64_t)p * a.ldx + c, v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) win[K - 1][i] = v[i];
+                row(p, win, s >= 0 && s < n);
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+            }
         }
     }
     if (a.final_state && L.r1 > L.r0 && next <= L.r1 && s < n) { // a clip ends with the chunk
-        if (s >= 0) {
-#pragma unroll
-            for (int k = 0; k < K - 1; ++k) seq_store<T, V>((T*)a.final_state + ((int64_t)s * (K - 1) + k) * a.channels + c, win[k]);
-        }
+        if (s >= 0) conv_store_state<T, V, K>(a, c, s, win, a.final_state);
         if (L.r1 == a.rows)                                     // empty clips behind the last row
-            for (++s; s < n; ++s) conv_copy_state<T, V, K>(a, c, s, a.state, a.final_state);
+            for (++s; s < n; ++s) conv_copy_state<T, V>(a, c, s, a.state, a.final_state);
     }
 }
 
-// One pass down the chunk: d_p is formed once per row (the chunk's K-1 rows behind its end included), and a row's dx is
-// complete K-1 rows later.  acc[k] = what row p-(K-1)+k has collected.
-template <typename T, int V, int K>
-__global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a) {
-    ConvLane<T, V, K> L;
-    if (!conv_lane<T, V, K>(a, L)) return;
-    const int n = a.clips.n, c = L.c;
-    int s = L.s, next = L.next, first = s >= 0 ? seq_start(a.clips, s) : 0;
-    float win[K][V], acc[K][V], dw[K][V], db[V];
+// One pass down the chunk and the K-1 rows behind it: d_p is formed once per row, and a row's dx is complete K-1 rows later.
+// acc[k] = what position p-(K-1)+k of the clip has collected when row p is reached.
+template <typename T, int V, int K, bool WAVE>
+__global__ __launch_bounds__(256, K == 8 ? 1 : 3) void k_conv_bwd(ConvArgs a) {
+    ConvLane<T, V, K, WAVE> L;
+    if (!L.place(a)) return;
+    const int n = a.clips.n, c = L.c, skip = conv_skip<K>(a);
+    int s = conv_same<WAVE>(seq_find(a.clips, L.r0));
+    int next = s < n ? conv_same<WAVE>(seq_start(a.clips, s + 1)) : 0x7fffffff;
+    int first = s >= 0 ? conv_same<WAVE>(seq_start(a.clips, s)) : 0;
+    float win[K - 1 + CONV_PAIR][V], acc[K - 1 + CONV_PAIR][V], dw[K][V], db[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         db[i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) { dw[k][i] = 0.f; acc[k][i] = 0.f; }
+        for (int k = 0; k < K; ++k) dw[k][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K - 1 + CONV_PAIR; ++k) acc[k][i] = 0.f;
     }
+    const int end = min(a.rows, L.r1 + K - 1);                  // (a position is given out K-1 rows behind it, fewer taps or not)
+    const T* x = (const T*)a.x + (int64_t)L.r0 * a.ldx + c;
+    const T* dy = (const T*)a.dy + (int64_t)L.r0 * a.lddy + c;
+    typename SeqRaw<T, V>::type rawx[CONV_PAIR], rawg[CONV_PAIR];
+    auto request = [&](int p0) {
+#pragma unroll
+        for (int j = 0; j < CONV_PAIR; ++j) {
+            const int64_t r = min(p0 + j, end - 1) - L.r0;
+            rawx[j] = seq_raw<T, V>(x + r * a.ldx);
+            rawg[j] = seq_raw<T, V>(dy + r * a.lddy);
+        }
+    };
+    if (end > L.r0) request(L.r0);
+    if (a.dstate)
+        for (int e = s - 1; e >= 0 && seq_start(a.clips, e) == L.r0; --e) conv_copy_state<T, V>(a, c, e, a.dfinal, a.dstate);
+    conv_window<T, V, K>(a, c, s, first, L.r0, win);
+    // row p with its window w and collectors to[0..K-1]
+    auto row = [&](const float (*w)[V], float (*to)[V], const float (&g)[V], bool count) {
+        float d[V], pre[V];
+        if (a.act) {
+            L.pre(a, w, pre);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { const float sg = seq_sigmoid(pre[i]); d[i] = g[i] * (sg * fmaf(pre[i], 1.f - sg, 1.f)); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) d[i] = g[i];
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k >= skip)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (count) dw[k][i] = fmaf(d[i], w[k][i], dw[k][i]);
+                    to[k][i] = fmaf(L.w[k][i], d[i], to[k][i]);
+                }
+        if (count)
+#pragma unroll
+            for (int i = 0; i < V; ++i) db[i] += d[i];
+    };
+    auto put = [&](int q, const float (*v)[V]) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = v[0][i];
+        seq_store<T, V>((T*)a.dx + (int64_t)q * a.lddx + c, o);
+    };
     // the gradient of position q of the current clip: a row of the chunk, or a row of the state of a clip that starts in it
-    auto emit = [&](int q, const float (&v)[V]) {
-        if (q >= first) { if (q >= L.r0 && q < L.r1) seq_store<T, V>((T*)a.dx + (int64_t)q * a.lddx + c, v); }
-        else if (a.dstate && first >= L.r0 && first < L.r1)
-            seq_store<T, V>((T*)a.dstate + ((int64_t)s * (K - 1) + (K - 1 + q - first)) * a.channels + c, v);
+    auto emit = [&](int q, const float (*v)[V]) {
+        if (q >= first) { if (q >= L.r0 && q < L.r1) put(q, v); }
+        else if (a.dstate && first >= L.r0 && first < L.r1 && q >= first - (a.taps - 1)) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = v[0][i];
+            seq_store<T, V>((T*)a.dstate + ((int64_t)s * (a.taps - 1) + (a.taps - 1 + q - first)) * a.channels + c, o);
+        }
     };
     // the clip ended in front of row p: what its last K-1 positions have collected, with the gradient of its final state
     auto flush = [&](int p) {
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) {
-            if (a.dfinal) {
+            if (a.dfinal && k >= skip) {
                 float f[V];
-                seq_load<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + k) * a.channels + c, f);
+                seq_load<T, V>((const T*)a.dfinal + ((int64_t)s * (a.taps - 1) + k - skip) * a.channels + c, f);
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[k][i] += f[i];
             }
-            emit(p - (K - 1) + k, acc[k]);
+            emit(p - (K - 1) + k, acc + k);
         }
     };
-    if (a.dstate)
-        for (int e = s - 1; e >= 0 && seq_start(a.clips, e) == L.r0; --e) conv_copy_state<T, V, K>(a, c, e, a.dfinal, a.dstate);
-    conv_window<T, V, K>(a, c, s, first, L.r0, win);
-    const int end = min(a.rows, L.r1 + K - 1);
     bool done = false;
-    for (int p0 = L.r0; p0 < end && !done; p0 += CONV_AHEAD) {
-        float x[CONV_AHEAD][V], g[CONV_AHEAD][V];
+    for (int p0 = L.r0; p0 < end && !done; p0 += CONV_PAIR) {
+        float g[CONV_PAIR][V], now[CONV_PAIR][V];
 #pragma unroll
-        for (int j = 0; j < CONV_AHEAD; ++j) {
-            const int64_t p = min(p0 + j, end - 1);
-            seq_load<T, V>((const T*)a.x + p * a.ldx + c, x[j]);
-            seq_load<T, V>((const T*)a.dy + p * a.lddy + c, g[j]);
-        }
+        for (int j = 0; j < CONV_PAIR; ++j) { seq_unpack<T, V>(rawx[j], now[j]); seq_unpack<T, V>(rawg[j], g[j]); }
+        request(p0 + CONV_PAIR);
+        if (s >= 0 && s < n && next >= p0 + CONV_PAIR && L.r1 >= p0 + CONV_PAIR && p0 - (K - 1) >= max(first, L.r0)) {
 #pragma unroll
-        for (int j = 0; j < CONV_AHEAD; ++j) {
-            const int p = p0 + j;
-            if (p >= end || done) break;
-            if (p >= next && s < n) {
-                if (s >= 0 && p > L.r0) flush(p);
-                if (p >= L.r1) { done = true; break; }          // the rows behind the chunk belong to another clip
-                ++s;
-                while (s < n && seq_start(a.clips, s + 1) <= p) {
-                    if (a.dstate) conv_copy_state<T, V, K>(a, c, s, a.dfinal, a.dstate);
-                    ++s;
-                }
-                next = s < n ? seq_start(a.clips, s + 1) : 0x7fffffff;
-                first = p;
-                conv_window<T, V, K>(a, c, s, p, p, win);
+            for (int j = 0; j < CONV_PAIR; ++j) {
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) acc[k][i] = 0.f;
-            }
-            if (s < 0 || s >= n) {                              // a row of no clip
-                if (p >= L.r1) { done = true; break; }
-                float zero[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) zero[i] = 0.f;
-                seq_store<T, V>((T*)a.dx + (int64_t)p * a.lddx + c, zero);
-                continue;
+                for (int i = 0; i < V; ++i) win[K - 1 + j][i] = now[j][i];
+                row(win + j, acc + j, g[j], true);
+                put(p0 + j - (K - 1), acc + j);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                win[K - 1][i] = x[j][i];
-                float d = g[j][i];
-                if (a.act) {
-                    float pre = L.b[i];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) pre = fmaf(L.w[k][i], win[k][i], pre);
-                    const float sg = seq_sigmoid(pre);
-                    d *= sg * fmaf(pre, 1.f - sg, 1.f);
-                }
-                if (p < L.r1) {
-                    db[i] += d;
+                for (int k = 0; k < K - 1; ++k) { win[k][i] = win[k + CONV_PAIR][i]; acc[k][i] = acc[k + CONV_PAIR][i]; }
 #pragma unroll
-                    for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d, win[k][i], dw[k][i]);
-                }
-#pragma unroll
-                for (int k = 0; k < K; ++k) acc[k][i] = fmaf(L.w[k][i], d, acc[k][i]);
+                for (int k = K - 1; k < K - 1 + CONV_PAIR; ++k) acc[k][i] = 0.f;
             }
-            emit(p - (K - 1), acc[0]);
+        } else {
+#pragma unroll 1
+            for (int p = p0; p < min(p0 + CONV_PAIR, end); ++p) {
+                if (p >= next && s < n) {
+                    if (s >= 0 && p > L.r0) flush(p);
+                    if (p >= L.r1) { done = true; break; }      // the rows behind the chunk belong to another clip
+                    ++s;
+                    while (s < n && seq_start(a.clips, s + 1) <= p) {
+                        if (a.dstate) conv_copy_state<T, V>(a, c, s, a.dfinal, a.dstate);
+                        ++s;
+                    }
+                    next = s < n ? conv_same<WAVE>(seq_start(a.clips, s + 1)) : 0x7fffffff;
+                    first = p;
+                    conv_window<T, V, K>(a, c, s, p, p, win);
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k)
+                    for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) { win[k][i] = win[k + 1][i]; acc[k][i] = acc[k + 1][i]; }
+                        for (int i = 0; i < V; ++i) acc[k][i] = 0.f;
+                }
+                if (s < 0 || s >= n) {                          // a row of no clip
+                    if (p >= L.r1) { done = true; break; }
+                    float zero[1][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[K - 1][i] = 0.f;
+                    for (int i = 0; i < V; ++i) zero[0][i] = 0.f;
+                    put(p, zero);
+                    continue;
+                }
+                float v[V], gr[V];
+                seq_load<T, V>((const T*)a.x + (int64_t)p * a.ldx + c, v);
+                seq_load<T, V>((const T*)a.dy + (int64_t)p * a.lddy + c, gr);
+#pragma unroll
+                for (int i = 0; i < V; ++i) win[K - 1][i] = v[i];
+                row(win, acc, gr, p < L.r1);
+                emit(p - (K - 1), acc);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) { win[k][i] = win[k + 1][i]; acc[k][i] = acc[k + 1][i]; }
+                    acc[K - 1][i] = 0.f;
+                }
+            }
         }
     }
     if (!done && end > L.r0 && s >= 0 && s < n && next <= end) flush(end);
-    if (a.dstate && L.r1 == a.rows && L.r1 > L.r0) {            // empty clips behind the last row
-        for (int e = n - 1; e >= 0 && seq_start(a.clips, e) == a.rows; --e) conv_copy_state<T, V, K>(a, c, e, a.dfinal, a.dstate);
-    }
-    float* part = a.part + (int64_t)(L.r0 / a.chunk_rows) * ((int64_t)a.channels * (K + 1));
+    if (a.dstate && L.r1 == a.rows && L.r1 > L.r0)              // empty clips behind the last row
+        for (int e = n - 1; e >= 0 && seq_start(a.clips, e) == a.rows; --e) conv_copy_state<T, V>(a, c, e, a.dfinal, a.dstate);
+    float* part = a.part + (int64_t)L.chunk * ((int64_t)a.channels * (a.taps + 1));
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) part[(size_t)(c + i) * K + k] = dw[k][i];
-        part[(size_t)a.channels * K + c + i] = db[i];
+        for (int k = 0; k < K; ++k) if (k >= skip) part[(size_t)(c + i) * a.taps + k - skip] = dw[k][i];
+        part[(size_t)a.channels * a.taps + c + i] = db[i];
     }
 }
 
 // one token per clip: reads the K-1 rows of state, writes them shifted (state_out may be the state itself: a thread reads
-// all rows of its column before it writes one)
+// all rows of its columns before it writes one)
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
-    const long long g = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int s = (int)(g / a.cols);
+    const unsigned g = blockIdx.x * 256 + threadIdx.x;
+    const int s = g / a.cols, skip = conv_skip<K>(a);
     if (s >= a.rows) return;
-    const int c = (int)(g - (long long)s * a.cols) * V;
-    float win[K][V], y[V];
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) seq_load<T, V>((const T*)a.state + ((int64_t)s * (K - 1) + k) * a.channels + c, win[k]);
-    seq_load<T, V>((const T*)a.x + (int64_t)s * a.ldx + c, win[K - 1]);
+    ConvLane<T, V, K, false> L;
+    const int c = (int)(g - s * a.cols) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float acc = a.bias ? a.bias[c + i] : 0.f;
+        L.b[i] = a.bias ? a.bias[c + i] : 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) acc = fmaf(a.w[(size_t)(c + i) * K + k], win[k][i], acc);
-        y[i] = a.act ? acc * seq_sigmoid(acc) : acc;
+        for (int k = 0; k < K; ++k) L.w[k][i] = k >= skip ? a.w[(size_t)(c + i) * a.taps + k - skip] : 0.f;
     }
-    seq_store<T, V>((T*)a.y + (int64_t)s * a.ldy + c, y);
+    float win[K][V], y[V];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) seq_store<T, V>((T*)a.final_state + ((int64_t)s * (K - 1) + k) * a.channels + c, win[k + 1]);
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[k][i] = 0.f;
+        if (k >= skip) seq_load<T, V>(k < K - 1 ? (const T*)a.state + ((int64_t)s * (a.taps - 1) + k - skip) * a.channels + c : (const T*)a.x + (int64_t)s * a.ldx + c, win[k]);
+    }
+    L.pre(a, win, y);
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (a.act) y[i] *= seq_sigmoid(y[i]);
+    seq_store<T, V>((T*)a.y + (int64_t)s * a.ldy + c, y);
+    conv_store_state<T, V, K>(a, c, s, win + 1, a.final_state);
 }
 
 // ---- column sums (seq.h) -------------------------------------------------------------------------------------------------
@@ -318,44 +430,52 @@ int seq_colsum(const float* in, int64_t rows, int64_t cols, float* out, float* s
 
 // ---- entry points --------------------------------------------------------------------------------------------------------
 template <int WHAT, typename T, int V, int K> static void conv_launch3(const ConvArgs& a, hipStream_t st) {
-    const long long items = (long long)a.cols * (WHAT == 2 ? a.rows : a.chunks);
-    const dim3 grid(evad_blocks(items, 256)), block(256);
-    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K>), grid, block, 0, st, a);
-    else if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_bwd<T, V, K>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_step<T, V, K>), grid, block, 0, st, a);
+    const dim3 block(256);
+    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_step<T, V, K>), dim3(evad_blocks((long long)a.cols * a.rows, 256)), block, 0, st, a);
+    else if (a.cols >= 64) {
+        const dim3 grid(evad_blocks((long long)((a.cols + 63) / 64) * a.chunks, 4));
+        if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_bwd<T, V, K, true>), grid, block, 0, st, a);
+    } else {
+        const dim3 grid(evad_blocks((long long)a.cols * a.chunks, 256));
+        if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K, false>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_bwd<T, V, K, false>), grid, block, 0, st, a);
+    }
 }
-template <int WHAT, typename T, int V> static void conv_launch2(const ConvArgs& a, int K, hipStream_t st) {
-    switch (K) {
-        case 1: conv_launch3<WHAT, T, V, 1>(a, st); break;
+template <int WHAT, typename T, int V> static void conv_launch2(const ConvArgs& a, hipStream_t st) {
+    switch (a.taps) {
         case 2: conv_launch3<WHAT, T, V, 2>(a, st); break;
         case 3: conv_launch3<WHAT, T, V, 3>(a, st); break;
         case 4: conv_launch3<WHAT, T, V, 4>(a, st); break;
-        case 5: conv_launch3<WHAT, T, V, 5>(a, st); break;
-        case 6: conv_launch3<WHAT, T, V, 6>(a, st); break;
-        case 7: conv_launch3<WHAT, T, V, 7>(a, st); break;
         default: conv_launch3<WHAT, T, V, 8>(a, st); break;
     }
 }
-template <int WHAT, typename T> static void conv_launch1(ConvArgs& a, int K, bool vec, hipStream_t st) {
-    constexpr int N = SeqVec<T>::n;
-    if (vec && a.channels % N == 0) { a.cols = a.channels / N; conv_launch2<WHAT, T, N>(a, K, st); }
-    else { a.cols = a.channels; conv_launch2<WHAT, T, 1>(a, K, st); }
+template <int WHAT, typename T> static void conv_launch1(ConvArgs& a, bool vec, hipStream_t st) {
+    if (vec && a.channels % 4 == 0) { a.cols = a.channels / 4; conv_launch2<WHAT, T, 4>(a, st); }
+    else { a.cols = a.channels; conv_launch2<WHAT, T, 1>(a, st); }
 }
-template <int WHAT> static int conv_launch(ConvArgs& a, int K, int dtype, bool vec, hipStream_t st) {
-    if (dtype == SEQ_F32) conv_launch1<WHAT, float>(a, K, vec, st);
-    else if (dtype == SEQ_BF16) conv_launch1<WHAT, __bf16>(a, K, vec, st);
-    else conv_launch1<WHAT, _Float16>(a, K, vec, st);
+template <int WHAT> static int conv_launch(ConvArgs& a, int dtype, bool vec, hipStream_t st) {
+    if (dtype == SEQ_F32) conv_launch1<WHAT, float>(a, vec, st);
+    else if (dtype == SEQ_BF16) conv_launch1<WHAT, __bf16>(a, vec, st);
+    else conv_launch1<WHAT, _Float16>(a, vec, st);
     return evad_last_error();
+}
+// rows of four elements start on a border of four elements
+static bool conv_vec(const void* p, int64_t ld, int dtype) {
+    const int e = dtype == SEQ_F32 ? 4 : 2;
+    return (((uintptr_t)p | (uintptr_t)(ld * e)) & (4 * e - 1)) == 0;
 }
 
 static int conv_chunk_rows(int64_t rows, int channels, int backward) {
     // long chunks waste fewer reads at their starts, short ones give the chip more threads
-    return backward ? 64 : 32;
+    const int64_t r = (rows * ((channels + 3) / 4)) >> 19;
+    const int most = backward ? 64 : 32;
+    return r < 4 ? 4 : r > most ? most : (int)r / 4 * 4;
 }
 static bool conv_shape_ok(int64_t rows, int channels, int taps, int dtype) {
+    // (places are counted in 32 bits: a chunk has at least 4 rows, a token of the single-token form one)
     return rows >= 0 && rows <= 0x7ffffff0 && channels >= 1 && channels <= (1 << 20) && taps >= 1 && taps <= CONV_MAX_TAPS && dtype >= 0 && dtype <= 2;
 }
-static int conv_elem(int dtype) { return dtype == SEQ_F32 ? 4 : 2; }
 
 extern "C" int eventad_causal_conv_workspace(int64_t rows, int channels, int taps, int64_t* bytes) {
     if (!bytes || !conv_shape_ok(rows, channels, taps, 0)) return EVAD_ERR_ARG;
@@ -372,14 +492,13 @@ extern "C" int eventad_causal_conv_fwd(const void* x, int64_t ldx, const float* 
         (rows && (!x || !y || ldx < channels || ldy < channels))) return EVAD_ERR_ARG;
     ConvArgs a = {};
     a.clips = SeqClips{clip_start, clips, (int)rows};
-    a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.y = y; a.ldy = ldy; a.rows = (int)rows; a.channels = channels; a.act = act;
+    a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.y = y; a.ldy = ldy; a.rows = (int)rows; a.channels = channels; a.act = act; a.taps = taps;
     if (taps > 1) { a.state = state; a.final_state = final_state; }
     a.chunk_rows = conv_chunk_rows(rows, channels, 0);
     a.chunks = rows ? (int)((rows + a.chunk_rows - 1) / a.chunk_rows) : 1;
     if (!rows && !a.final_state) return EVAD_OK;
-    const int e = conv_elem(dtype);
-    const bool vec = seq_aligned(x, ldx * e) && seq_aligned(y, ldy * e) && seq_aligned(state, 0) && seq_aligned(final_state, 0);
-    return conv_launch<0>(a, taps, dtype, vec, (hipStream_t)stream);
+    const bool vec = conv_vec(x, ldx, dtype) && conv_vec(y, ldy, dtype) && conv_vec(state, 0, dtype) && conv_vec(final_state, 0, dtype);
+    return conv_launch<0>(a, dtype, vec, (hipStream_t)stream);
 }
 
 extern "C" int eventad_causal_conv_bwd(const void* x, int64_t ldx, const float* w, const float* bias, const int32_t* clip_start,
@@ -394,15 +513,14 @@ extern "C" int eventad_causal_conv_bwd(const void* x, int64_t ldx, const float* 
     ConvArgs a = {};
     a.clips = SeqClips{clip_start, clips, (int)rows};
     a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.dy = dy; a.lddy = lddy; a.dx = dx; a.lddx = lddx;
-    a.rows = (int)rows; a.channels = channels; a.act = act;
+    a.rows = (int)rows; a.channels = channels; a.act = act; a.taps = taps;
     if (taps > 1) { a.state = state; a.dfinal = dfinal; a.dstate = dstate; }
     a.chunk_rows = conv_chunk_rows(rows, channels, 1);
     a.chunks = rows ? (int)((rows + a.chunk_rows - 1) / a.chunk_rows) : 1;
     a.part = (float*)workspace;
-    const int e = conv_elem(dtype);
-    const bool vec = seq_aligned(x, ldx * e) && seq_aligned(dy, lddy * e) && seq_aligned(dx, lddx * e) && seq_aligned(state, 0) &&
-                     seq_aligned(dfinal, 0) && seq_aligned(dstate, 0);
-    const int rc = conv_launch<1>(a, taps, dtype, vec, (hipStream_t)stream);
+    const bool vec = conv_vec(x, ldx, dtype) && conv_vec(dy, lddy, dtype) && conv_vec(dx, lddx, dtype) && conv_vec(state, 0, dtype) &&
+                     conv_vec(dfinal, 0, dtype) && conv_vec(dstate, 0, dtype);
+    const int rc = conv_launch<1>(a, dtype, vec, (hipStream_t)stream);
     if (rc) return rc;
     const int64_t cols = (int64_t)channels * (taps + 1);
     return seq_colsum(a.part, a.chunks, cols, dparams, a.part + a.chunks * cols, (hipStream_t)stream);
@@ -416,8 +534,7 @@ extern "C" int eventad_causal_conv_step(const void* x, int64_t ldx, const float*
     if (!clips) return EVAD_OK;
     ConvArgs a = {};
     a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.state = state; a.final_state = state_out; a.y = y; a.ldy = ldy;
-    a.rows = clips; a.channels = channels; a.act = act;
-    const int e = conv_elem(dtype);
-    const bool vec = seq_aligned(x, ldx * e) && seq_aligned(y, ldy * e) && seq_aligned(state, 0) && seq_aligned(state_out, 0);
-    return conv_launch<2>(a, taps, dtype, vec, (hipStream_t)stream);
+    a.rows = clips; a.channels = channels; a.act = act; a.taps = taps;
+    const bool vec = conv_vec(x, ldx, dtype) && conv_vec(y, ldy, dtype) && conv_vec(state, 0, dtype) && conv_vec(state_out, 0, dtype);
+    return conv_launch<2>(a, dtype, vec, (hipStream_t)stream);
 }

@@ -703,15 +703,10 @@ __global__ __launch_bounds__(256) void k_scan_bc(const float* __restrict__ part,
 // lanes of a quad form the step and the gate of one clip each.  VEC: rows of A, B, C and the states are whole and aligned groups
 // of four; otherwise they are read entry by entry.  state_out may be the state itself: a lane reads its entries before it
 // writes them and nobody else needs them.
-template <typename T> struct SeqQuad;
-template <> struct SeqQuad<float> { typedef seq_f4 type; };
-template <> struct SeqQuad<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
-template <> struct SeqQuad<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
-
 template <typename T, bool VEC> __device__ __forceinline__ void step_load4(const T* __restrict__ row, int j, int N, float (&v)[4]) {
     if constexpr (VEC) {
-        typename SeqQuad<T>::type w = {};
-        if (4 * j < N) w = *(const typename SeqQuad<T>::type*)(row + 4 * j);
+        typename SeqVec<T, 4>::type w = {};
+        if (4 * j < N) w = *(const typename SeqVec<T, 4>::type*)(row + 4 * j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = (float)w[i];
     } else {
