@@ -24,68 +24,34 @@ struct NormArgs {
     float* part;                                     // [workgroups][channels]
 };
 
-// sum / maximum over the LANES lanes that share a row
-template <int LANES, typename F> __device__ __forceinline__ F row_sum(F v, F* s) {
-#pragma unroll
-    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) v += __shfl_xor(v, d, 64);
+// sum over the LANES lanes that share a row
+template <int LANES> __device__ __forceinline__ float row_sum(float v, float* s) {
+    v = seq_lane_sum<LANES == 16 ? 16 : 64>(v);
     if constexpr (LANES > 64) {
-        constexpr int WAVES = LANES / 64;
         __syncthreads();
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = s[0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) v += s[i];
+        v = (s[0] + s[1]) + (s[2] + s[3]);
     }
     return v;
 }
-// (of non-negative doubles as bit patterns: NaN is the largest of all and stays)
-template <int LANES> __device__ __forceinline__ double row_max(double v, double* s) {
-    auto top = [](double p, double q) { return __double_as_longlong(p) > __double_as_longlong(q) ? p : q; };
+// maximum of the bit patterns of non-negative floats / doubles (NaN is above all numbers and stays)
+template <int LANES, typename B> __device__ __forceinline__ B row_max(B v, B* s) {
 #pragma unroll
-    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) v = top(v, __shfl_xor(v, d, 64));
+    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) v = max(v, (B)__shfl_xor(v, d, 64));
     if constexpr (LANES > 64) {
-        constexpr int WAVES = LANES / 64;
         __syncthreads();
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = s[0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) v = top(v, s[i]);
+        v = max(max(s[0], s[1]), max(s[2], s[3]));
     }
     return v;
-}
-
-// v rounded towards the odd neighbour, so that a second rounding to fewer bits is the one rounding of v: e4m3 keeps 4 of the
-// 24 bits of a float
-__device__ __forceinline__ float norm_to_odd(double v) {
-    const float f = (float)v;
-    const double back = (double)f;
-    if (back == v || !(fabs(v) < 1e30)) return f;
-    unsigned u = __float_as_uint(f);
-    if (fabs(back) > fabs(v)) --u;                               // towards zero
-    return __uint_as_float(u | 1u);
-}
-
-// y / scale = 448 h w / max|h w| needs no r.  It is formed in float64, where h w is exact, so that a value next to a border
-// of the 8-bit grid falls on the side the definition says.
-__device__ __forceinline__ unsigned norm_e4m3(float h, float w, double inv) {
-    const float f = norm_to_odd((double)h * (double)w * inv);
-    return __builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false) & 0xffu;
-}
-struct NormScale { double inv; float scale; };
-__device__ __forceinline__ NormScale norm_scale(double top, float r) {
-    NormScale s;
-    s.scale = (float)(top * (double)r / 448.0);
-    if (!(s.scale >= 1.17549435e-38f) && s.scale == s.scale) { s.scale = 1.f; s.inv = (double)r; }   // a row of zeros (or next to it)
-    else s.inv = 448.0 / top;
-    return s;
 }
 
 // LOOP: the row does not fit ITERS pieces per lane and is read again for every pass over it.
-template <typename T, int V, int LANES, int ITERS, bool LOOP, bool FP8>
+template <typename T, int V, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
-    __shared__ double s_red[4];
+    __shared__ float s_red[4];
     constexpr int PER = 256 / LANES;
     const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES, D = a.channels;
@@ -125,49 +91,14 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) ss = fmaf(h[k][i], h[k][i], ss);
     }
-    ss = row_sum<LANES, float>(ss, (float*)s_red);
+    ss = row_sum<LANES>(ss, s_red);
     const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
-    NormScale sc = {0.0, 0.f};
-    if constexpr (FP8) {
-        double top = 0.0;
-        auto fold = [&](int c, const float (&v)[V]) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double p = fabs((double)v[i] * (double)a.w[c + i]);
-                if (__double_as_longlong(p) > __double_as_longlong(top)) top = p;
-            }
-        };
-        if constexpr (LOOP) { for (int c = lane * V; c < D; c += LANES * V) { float v[V]; piece(c, v, false); fold(c, v); } }
-        else {
-#pragma unroll
-            for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, h[k]); }
-        }
-        top = row_max<LANES>(top, s_red);
-        sc = norm_scale(top, inv);
-        if (in && lane == 0) a.scale[r] = sc.scale;
-    }
     if (!in) return;
     auto finish = [&](int c, const float (&v)[V]) {
-        if constexpr (FP8) {
-            uint8_t* q = a.q + r * a.ldq + c;
-            if constexpr (V == 1) *q = (uint8_t)norm_e4m3(v[0], a.w[c], sc.inv);
-            else {
-                unsigned word[V / 4];
+        float y[V];
 #pragma unroll
-                for (int i = 0; i < V; i += 4) {
-                    word[i / 4] = 0;
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) word[i / 4] |= norm_e4m3(v[i + m], a.w[c + i + m], sc.inv) << (8 * m);
-                }
-#pragma unroll
-                for (int i = 0; i < V / 4; ++i) ((unsigned*)q)[i] = word[i];
-            }
-        } else {
-            float y[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = v[i] * inv * a.w[c + i];
-            seq_store<T, V>((T*)a.y + r * a.ldy + c, y);
-        }
+        for (int i = 0; i < V; ++i) y[i] = v[i] * inv * a.w[c + i];
+        seq_store<T, V>((T*)a.y + r * a.ldy + c, y);
     };
     if constexpr (LOOP) { for (int c = lane * V; c < D; c += LANES * V) { float v[V]; piece(c, v, false); finish(c, v); } }
     else {
@@ -176,11 +107,154 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
     }
 }
 
+// ---- 8 bits ----------------------------------------------------------------------------------------------------------------
+// y / scale = 448 p / max|p| with p = h w needs no r.  A value next to a border of the 8-bit grid has to fall on the side the
+// definition says, so the quotient is formed in float32 (p, its maximum, 448 / maximum and the product: error below 5 units in the
+// last place) and, where it lies within 8 of a border or among the subnormals, again in float64, where p is exact.  One value
+// in 8,000 of ordinary data does.
+
+// v rounded towards the odd neighbour, so that a second rounding to fewer bits is the one rounding of v: e4m3 keeps 4 of the
+// 24 bits of a float
+__device__ __forceinline__ float norm_to_odd(double v) {
+    const float f = (float)v;
+    const double back = (double)f;
+    if (back == v || !(fabs(v) < 1e30)) return f;
+    unsigned u = __float_as_uint(f);
+    if (fabs(back) > fabs(v)) --u;                               // towards zero
+    return __uint_as_float(u | 1u);
+}
+
+template <typename T, int V, int LANES, int ITERS, bool LOOP>
+__global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
+    __shared__ unsigned long long s_red[4];
+    constexpr int PER = 256 / LANES;
+    const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES, D = a.channels;
+    const bool in = row < a.rows;
+    const int64_t r = in ? row : a.rows - 1;
+    const T* x = (const T*)a.x + r * a.ldx;
+    const T* res = a.res ? (const T*)a.res + r * a.ldr : nullptr;
+    float p[ITERS][V];
+    auto piece = [&](int c, float (&v)[V], bool store) {         // h of the piece at column c
+        seq_load<T, V>(x + c, v);
+        if (res) {
+            float e[V];
+            seq_load<T, V>(res + c, e);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = (float)(T)(v[i] + e[i]);
+            if (store) seq_store<T, V>((T*)a.sum + r * a.lds + c, v);
+        }
+    };
+    float ss = 0.f, top = 0.f, poison = 0.f;
+    auto fold = [&](int c, float (&v)[V]) {                      // h -> p
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            ss = fmaf(v[i], v[i], ss);
+            v[i] *= a.w[c + i];
+            top = fmaxf(top, fabsf(v[i]));
+            poison = fmaf(v[i], 0.f, poison);                    // NaN if anything is not finite
+        }
+    };
+    if constexpr (LOOP) { for (int c = lane * V; c < D; c += LANES * V) { float v[V]; piece(c, v, in); fold(c, v); } }
+    else {
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            const int c = (k * LANES + lane) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[k][i] = 0.f;
+            if (c < D) piece(c, p[k], in);
+        }
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, p[k]); }
+    }
+    ss = row_sum<LANES>(ss, (float*)s_red);
+    const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+    const unsigned own = __float_as_uint(poison == 0.f ? top : __builtin_nanf(""));
+    const unsigned most = row_max<LANES, unsigned>(own, (unsigned*)s_red);
+    float scale = __uint_as_float(most) * inv / 448.f;
+    const bool zero = !(scale >= 1.17549435e-38f) && scale == scale;             // a row of zeros (or next to it)
+    if (zero) scale = 1.f;
+    if (in && lane == 0) a.scale[r] = scale;
+    const float by32 = zero ? inv : 448.f / __uint_as_float(most);
+    // p -> q of a piece; true if a value lies too close to a border, or below the smallest normal one and is not 0
+    auto divide = [&](const float (&v)[V], float (&q)[V]) {
+        unsigned near = 0xffffffffu, low = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            q[i] = v[i] * by32;
+            const unsigned u = __float_as_uint(q[i]);
+            near = min(near, (u - 0x7fff8u) & 0xfffffu);         // (borders: the 20 bits that e4m3 has not are 0x80000)
+            low = min(low, (u & 0x7fffffffu) - 1u);
+        }
+        return near <= 16u || low < 0x3c800000u - 1u;            // 2^-6
+    };
+    bool close = LOOP;
+    if constexpr (!LOOP) {
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            float q[V];
+            if (divide(p[k], q)) close = true;
+        }
+    }
+    // any lane of the row (and of the wave's other rows): then the row's maximum in float64 -- of the entries that share the
+    // float32 maximum, as rounding keeps the order
+    double by = 0.0;
+    if (LANES > 64 ? __syncthreads_or(close) : (int)__any(close)) {
+        unsigned long long exact = 0;
+        if (own == most && own <= 0x7f800000u) {
+            for (int c = lane * V; c < D; c += LANES * V) {
+                float v[V];
+                piece(c, v, false);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (__float_as_uint(fabsf(v[i] * a.w[c + i])) == most)
+                        exact = max(exact, (unsigned long long)__double_as_longlong(fabs((double)v[i] * (double)a.w[c + i])));
+            }
+        }
+        exact = row_max<LANES, unsigned long long>(exact, s_red);
+        by = most > 0x7f800000u ? (double)__builtin_nanf("") : zero ? (double)inv : 448.0 / __longlong_as_double(exact);
+    }
+    if (!in) return;
+    auto finish = [&](int c, const float (&v)[V]) {
+        float q[V];
+        if (divide(v, q)) {
+            float h[V];
+            piece(c, h, false);
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[i] = norm_to_odd((double)h[i] * (double)a.w[c + i] * by);
+        }
+        uint8_t* out = a.q + r * a.ldq + c;
+        if constexpr (V == 1) *out = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[0], 0, false);
+        else {
+            typedef unsigned word __attribute__((ext_vector_type(V / 4)));
+            word o;
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+                o[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], w, true);
+            }
+            *(word*)out = o;
+        }
+    };
+    if constexpr (LOOP) {
+        for (int c = lane * V; c < D; c += LANES * V) {
+            float v[V];
+            piece(c, v, false);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] *= a.w[c + i];
+            finish(c, v);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, p[k]); }
+    }
+}
+
 // A workgroup goes over rows blockIdx.x, blockIdx.x + gridDim.x, ... (x PER rows at a time) and keeps its share of dw in
 // registers (LOOP: in its own row of `part`).
 template <typename T, int V, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
-    __shared__ double s_red[4];
+    __shared__ float s_red[4];
     __shared__ float s_dw[LANES < 256 ? 256 * V * ITERS : 1];
     constexpr int PER = 256 / LANES;
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, D = a.channels;
@@ -221,8 +295,8 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
 #pragma unroll
             for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, h[k], g[k]); }
         }
-        ss = row_sum<LANES, float>(ss, (float*)s_red);
-        eh = row_sum<LANES, float>(eh, (float*)s_red);
+        ss = row_sum<LANES>(ss, s_red);
+        eh = row_sum<LANES>(eh, s_red);
         const float inv = 1.f / sqrtf(ss / (float)D + a.eps), m = inv * inv * (eh / (float)D);
         if (!in) continue;
         auto finish = [&](int c, const float (&hv)[V], const float (&gv)[V], float (&acc)[V]) {
@@ -280,8 +354,8 @@ static int norm_groups(int64_t rows) { return (int)(rows < 1 ? 1 : rows < 1024 ?
 template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static void norm_launch3(const NormArgs& a, int groups, hipStream_t st) {
     constexpr int PER = 256 / LANES;
     const dim3 grid((unsigned)((a.rows + PER - 1) / PER)), block(256);
-    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP, false>), grid, block, 0, st, a);
-    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP, true>), grid, block, 0, st, a);
+    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP>), grid, block, 0, st, a);
+    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fp8<T, V, LANES, ITERS, LOOP>), grid, block, 0, st, a);
     if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_bwd<T, V, LANES, ITERS, LOOP>), dim3(groups), block, 0, st, a);
 }
 // The fewest lanes that hold a row in four pieces each: rows of one wave need no LDS, and short rows share a wave.

@@ -58,6 +58,29 @@ __device__ __forceinline__ float seq_exp2(float x) { return __builtin_amdgcn_exp
 __device__ __forceinline__ float seq_rcp(float x) { return __builtin_amdgcn_rcpf(x); }            // v_rcp_f32, 1 ulp
 __device__ __forceinline__ float seq_sigmoid(float x) { return seq_rcp(1.f + seq_exp2(-SEQ_LOG2E * x)); }
 
+template <int CTRL> __device__ __forceinline__ float seq_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// x = the sum over both halves of the wave: of x in lanes 0..31, of y in lanes 32..63
+__device__ __forceinline__ void seq_swap32(float& x, float y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(y), false, false);
+    x = __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+// x = the sum over each pair of rows of 16 lanes: of x in the even row, of y in the odd one
+__device__ __forceinline__ void seq_swap16(float& x, float y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(y), false, false);
+    x = __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+// sum over 16 or 64 lanes, in all of them: xor 1, xor 2 (quad_perm), the mirrored half row and row, then the rows
+template <int LANES> __device__ __forceinline__ float seq_lane_sum(float v) {
+    v += seq_dpp<0xB1>(v);
+    v += seq_dpp<0x4E>(v);
+    v += seq_dpp<0x141>(v);
+    v += seq_dpp<0x140>(v);
+    if constexpr (LANES == 64) { seq_swap16(v, v); seq_swap32(v, v); }
+    return v;
+}
+
 struct SeqClips { const int* start; int n; int rows; };        // start == nullptr: one clip of all rows
 
 __device__ __forceinline__ int seq_start(const SeqClips& c, int s) { return c.start ? c.start[s] : (s ? c.rows : 0); }

@@ -45,9 +45,6 @@ struct ScanArgs {
     float* part_p;                                   // [chunks][channels*N (dA) | channels (dD) | channels (dbias)]
 };
 
-template <int CTRL> __device__ __forceinline__ float seq_dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
 // value of lane Q of the quad, in all four lanes
 template <int Q> __device__ __forceinline__ float quad_bcast(float v) { return seq_dpp<Q * 0x55>(v); }
 // (as a register of its own: a multiplication with a DPP operand issues at 0.6 of the rate of a plain one -- 31 against 50 T
@@ -57,15 +54,6 @@ __device__ __forceinline__ float quad_bcast(float v, int q) {
     asm("" : "+v"(b));
     return b;
 }
-// sum over the LPC lanes of a channel, in all of them: xor 1, xor 2 (quad_perm), then the mirrored half and whole row of 16
-template <int LPC> __device__ __forceinline__ float chan_sum(float v) {
-    v += seq_dpp<0xB1>(v);
-    v += seq_dpp<0x4E>(v);
-    if constexpr (LPC >= 8) v += seq_dpp<0x141>(v);
-    if constexpr (LPC >= 16) v += seq_dpp<0x140>(v);
-    return v;
-}
-
 // Four rows' partial sums v[0..3] in the LPC lanes of a channel -> the sum of row q in every lane with quad position q: the
 // quads are folded first (mirrored half rows and rows: the lane order inside a quad does not matter to the sum), then a quad
 // exchanges halves twice, which takes 9 operations for four rows instead of 12 for a sum in all lanes and a select.
@@ -468,19 +456,11 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
 // halves of each half while they halve the number of values (a swap serves two values), then DPP rotations add up the
 // channels inside a row of 16 lanes.  Returns, for row r of 16 lanes, v[0..1] = values 2 (r & 1) + {0, 1} of the first four
 // (r < 2) or of the last four (r >= 2).
-__device__ __forceinline__ void swap_add32(float& x, const float& y) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(y), false, false);
-    x = __int_as_float(r[0]) + __int_as_float(r[1]);
-}
-__device__ __forceinline__ void swap_add16(float& x, const float& y) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(y), false, false);
-    x = __int_as_float(r[0]) + __int_as_float(r[1]);
-}
 template <int LPC> __device__ __forceinline__ void wave_fold(float (&b)[4], const float (&c)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) swap_add32(b[i], c[i]);           // lanes 0..31: sums of b, lanes 32..63: sums of c
-    swap_add16(b[0], b[2]);                                       // even rows of 16: entry 0, odd rows: entry 2
-    swap_add16(b[1], b[3]);
+    for (int i = 0; i < 4; ++i) seq_swap32(b[i], c[i]);           // lanes 0..31: sums of b, lanes 32..63: sums of c
+    seq_swap16(b[0], b[2]);                                       // even rows of 16: entry 0, odd rows: entry 2
+    seq_swap16(b[1], b[3]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if constexpr (LPC <= 8) b[i] += seq_dpp<0x128>(b[i]);     // row_ror:8
