@@ -26,7 +26,7 @@ struct NormArgs {
 
 // sum over the LANES lanes that share a row
 template <int LANES> __device__ __forceinline__ float row_sum(float v, float* s) {
-    v = seq_lane_sum<LANES == 16 ? 16 : 64>(v);
+    v = seq_lane_sum<LANES < 64 ? LANES : 64>(v);
     if constexpr (LANES > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
@@ -269,29 +269,38 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) part[c + i] = 0.f;
     }
-    for (int64_t r0 = (int64_t)blockIdx.x * PER; r0 < a.rows; r0 += (int64_t)gridDim.x * PER) {
-        const bool in = r0 + sub < a.rows;
-        const int64_t r = in ? r0 + sub : a.rows - 1;
+    const int64_t step = (int64_t)gridDim.x * PER;
+    // (a row's arrays are requested while the row in front is worked on; without that the sums over a row leave memory idle)
+    typename SeqRaw<T, V>::type rh[ITERS], rg[ITERS], rs[ITERS];
+    auto request = [&](int64_t r) {
+        r = min(r, a.rows - 1);
         const T* hr = (const T*)a.sum + r * a.lds;
         const T* gr = (const T*)a.dy + r * a.lddy;
-        const T* sr = a.dsum ? (const T*)a.dsum + r * a.ldds : nullptr;
-        float h[ITERS][V], g[ITERS][V], ss = 0.f, eh = 0.f;
+        const T* sr = a.dsum ? (const T*)a.dsum + r * a.ldds : hr;
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) {
+            const int c = min((k * LANES + lane) * V, D - V);     // (D is a multiple of V)
+            rh[k] = seq_raw<T, V>(hr + c); rg[k] = seq_raw<T, V>(gr + c); rs[k] = seq_raw<T, V>(sr + c);
+        }
+    };
+    if (!LOOP && a.rows) request((int64_t)blockIdx.x * PER + sub);
+    for (int64_t r0 = (int64_t)blockIdx.x * PER; r0 < a.rows; r0 += step) {
+        const bool in = r0 + sub < a.rows;
+        const int64_t r = in ? r0 + sub : a.rows - 1;
+        float h[ITERS][V], g[ITERS][V], ds[ITERS][V], ss = 0.f, eh = 0.f;
         auto fold = [&](int c, const float (&hv)[V], const float (&gv)[V]) {
 #pragma unroll
             for (int i = 0; i < V; ++i) { ss = fmaf(hv[i], hv[i], ss); eh = fmaf(gv[i] * a.w[c + i], hv[i], eh); }
         };
+        const T* hr = (const T*)a.sum + r * a.lds;
+        const T* gr = (const T*)a.dy + r * a.lddy;
+        const T* sr = a.dsum ? (const T*)a.dsum + r * a.ldds : nullptr;
         if constexpr (LOOP) {
             for (int c = lane * V; c < D; c += LANES * V) { float hv[V], gv[V]; seq_load<T, V>(hr + c, hv); seq_load<T, V>(gr + c, gv); fold(c, hv, gv); }
         } else {
 #pragma unroll
-            for (int k = 0; k < ITERS; ++k) {
-                const int c = (k * LANES + lane) * V;
-                if (c < D) { seq_load<T, V>(hr + c, h[k]); seq_load<T, V>(gr + c, g[k]); }
-                else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) { h[k][i] = 0.f; g[k][i] = 0.f; }
-                }
-            }
+            for (int k = 0; k < ITERS; ++k) { seq_unpack<T, V>(rh[k], h[k]); seq_unpack<T, V>(rg[k], g[k]); seq_unpack<T, V>(rs[k], ds[k]); }
+            request(r0 + step + sub);
 #pragma unroll
             for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, h[k], g[k]); }
         }
@@ -299,31 +308,29 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
         eh = row_sum<LANES>(eh, s_red);
         const float inv = 1.f / sqrtf(ss / (float)D + a.eps), m = inv * inv * (eh / (float)D);
         if (!in) continue;
-        auto finish = [&](int c, const float (&hv)[V], const float (&gv)[V], float (&acc)[V]) {
-            float dh[V], ds[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) ds[i] = 0.f;
-            if (sr) seq_load<T, V>(sr + c, ds);
+        auto finish = [&](int c, const float (&hv)[V], const float (&gv)[V], const float (&sv)[V], float (&acc)[V]) {
+            float dh[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                dh[i] = fmaf(inv, fmaf(-hv[i], m, gv[i] * a.w[c + i]), ds[i]);
+                dh[i] = fmaf(inv, fmaf(-hv[i], m, gv[i] * a.w[c + i]), sr ? sv[i] : 0.f);
                 acc[i] = fmaf(gv[i] * inv, hv[i], acc[i]);
             }
             seq_store<T, V>((T*)a.dh + r * a.lddh + c, dh);
         };
         if constexpr (LOOP) {
             for (int c = lane * V; c < D; c += LANES * V) {
-                float hv[V], gv[V], acc[V];
+                float hv[V], gv[V], sv[V], acc[V];
                 seq_load<T, V>(hr + c, hv); seq_load<T, V>(gr + c, gv);
+                if (sr) seq_load<T, V>(sr + c, sv);
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[i] = part[c + i];
-                finish(c, hv, gv, acc);
+                finish(c, hv, gv, sv, acc);
 #pragma unroll
                 for (int i = 0; i < V; ++i) part[c + i] = acc[i];
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, h[k], g[k], dw[k]); }
+            for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, h[k], g[k], ds[k], dw[k]); }
         }
     }
     if constexpr (!LOOP && LANES == 256) {
@@ -362,7 +369,7 @@ template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static v
 template <int WHAT, typename T, int V> static void norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
     const int pieces = (a.channels + V - 1) / V;
     if (pieces <= 16) norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
-    else if (pieces <= 32) norm_launch3<WHAT, T, V, 16, 2, false>(a, groups, st);
+    else if (pieces <= 32) norm_launch3<WHAT, T, V, 32, 1, false>(a, groups, st);
     else if (pieces <= 64) norm_launch3<WHAT, T, V, 64, 1, false>(a, groups, st);
     else if (pieces <= 128) norm_launch3<WHAT, T, V, 64, 2, false>(a, groups, st);
     else if (pieces <= 256) norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st);

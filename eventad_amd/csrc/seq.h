@@ -71,13 +71,14 @@ __device__ __forceinline__ void seq_swap16(float& x, float y) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(y), false, false);
     x = __int_as_float(r[0]) + __int_as_float(r[1]);
 }
-// sum over 16 or 64 lanes, in all of them: xor 1, xor 2 (quad_perm), the mirrored half row and row, then the rows
+// sum over 16, 32 or 64 lanes, in all of them: xor 1, xor 2 (quad_perm), the mirrored half row and row, then the rows
 template <int LANES> __device__ __forceinline__ float seq_lane_sum(float v) {
     v += seq_dpp<0xB1>(v);
     v += seq_dpp<0x4E>(v);
     v += seq_dpp<0x141>(v);
     v += seq_dpp<0x140>(v);
-    if constexpr (LANES == 64) { seq_swap16(v, v); seq_swap32(v, v); }
+    if constexpr (LANES >= 32) seq_swap16(v, v);
+    if constexpr (LANES >= 64) seq_swap32(v, v);
     return v;
 }
 
