@@ -107,23 +107,40 @@ __device__ __forceinline__ void scan_store4(float* __restrict__ row, int j, int 
 // addresses of a tile's rows 60).
 __device__ __forceinline__ int scan_again(int v) { asm volatile("" : "+v"(v)); return v; }
 
-// base is the same for the whole wave, off in bytes: one scalar base and one 32-bit offset per access
-template <typename T> __device__ __forceinline__ T& scan_at(T* base, unsigned off) { return *(T*)((char*)base + off); }
-template <typename T> __device__ __forceinline__ const T& scan_at(const T* base, unsigned off) { return *(const T*)((const char*)base + off); }
+// A lane's element of four rows of a tile: rows 4 k + q, channel d.  p, the tile's first row, and step, four rows, are the same
+// for the whole wave: one scalar base and one 32-bit offset per access, and no 64-bit arithmetic on the way.
+template <typename T> struct ScanRows {
+    char* p; unsigned step, at;
+    __device__ __forceinline__ ScanRows(const void* base, int64_t ld, int t0, int q, int d)
+        : p((char*)base + (int64_t)t0 * ld * (int)sizeof(T)), step(4 * (unsigned)ld * sizeof(T)), at((unsigned)(q * (int)ld + d) * sizeof(T)) {}
+    __device__ __forceinline__ T& row(int k) const { return *(T*)(p + (scan_again(at) + k * step)); }
+    __device__ __forceinline__ void fetch(T (&v)[4], bool full, int left) const {                // left: rows of the lane's
+        if (full) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = row(k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[k] = (T)0.f; if (4 * k < left) v[k] = row(k); }
+        }
+    }
+    __device__ __forceinline__ void move(int tiles) { p += (int64_t)tiles * (int64_t)(4u * step); }
+};
 
-// B (and C) of a tile on their way to LDS as floats: requested a tile ahead, written when the rows in front are done.  A
-// thread takes one state of every (256 / N4)th row; rows of no clip and states >= N become zero.
+// B or C of a tile on their way to LDS as floats: requested a tile ahead, written when the rows in front are done.  A thread
+// takes one state of every (256 / N4)th row; rows of no clip and states >= N become zero.
 template <typename T, int LPC> struct ScanStage {
     static constexpr int N4 = 4 * LPC, PER = SCAN_TILE * N4 / 256, STEP = 256 / N4;
+    char* p; unsigned step, at; bool in;
     T v[PER];
-    __device__ __forceinline__ void load(const void* base, int64_t ld, int t0, int rows, int N) {
-        const int r = scan_again(threadIdx.x) / N4, n = threadIdx.x % N4;
-        const T* p = (const T*)base + (int64_t)t0 * ld;
-        const bool full = t0 + SCAN_TILE <= rows;
+    __device__ __forceinline__ ScanStage(const void* base, int64_t ld, int t0, int N)
+        : p((char*)base + (int64_t)t0 * ld * (int)sizeof(T)), step(STEP * (unsigned)ld * sizeof(T)), in(threadIdx.x % N4 < N) {
+        at = (unsigned)(threadIdx.x / N4 * (int)ld + min((int)threadIdx.x % N4, N - 1)) * sizeof(T);
+    }
+    __device__ __forceinline__ void load(bool full, int left) {                                  // left: rows of the tile
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             v[i] = (T)0.f;
-            if (n < N && (full || t0 + r + i * STEP < rows)) v[i] = scan_at(p, (unsigned)((r + i * STEP) * (int)ld + n) * sizeof(T));
+            if (full || (int)threadIdx.x / N4 + i * STEP < left) v[i] = *(const T*)(p + (scan_again(at) + i * step));
         }
     }
     __device__ __forceinline__ void store(float* __restrict__ s, int t0, int lo, int hi) const {
@@ -131,23 +148,11 @@ template <typename T, int LPC> struct ScanStage {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int r = t0 + threadIdx.x / N4 + i * STEP;
-            s[threadIdx.x + 256 * i] = clean || (r >= lo && r < hi) ? (float)v[i] : 0.f;
+            s[threadIdx.x + 256 * i] = in && (clean || (r >= lo && r < hi)) ? (float)v[i] : 0.f;
         }
     }
+    __device__ __forceinline__ void move(int tiles) { p += (int64_t)tiles * (int64_t)((SCAN_TILE / STEP) * step); }
 };
-// A lane's element of four rows of a tile: rows t0 + 4 k + q, channel d (at = q ld + d, in bytes)
-template <typename T> __device__ __forceinline__ void scan_fetch(const void* base, int64_t ld, unsigned at, int t0, int q, int rows, T (&v)[4]) {
-    const T* p = (const T*)base + (int64_t)t0 * ld;
-    const unsigned step = 4 * (unsigned)ld * sizeof(T);
-    at = scan_again(at);
-    if (t0 + SCAN_TILE <= rows) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = scan_at(p, at + k * step);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { v[k] = (T)0.f; if (t0 + 4 * k + q < rows) v[k] = scan_at(p, at + k * step); }
-    }
-}
 
 // B or C of a pair of rows, read from LDS a pair ahead (and, with a scheduling barrier behind the reads, not more: the
 // registers would cost waves in flight)
@@ -219,19 +224,21 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     }
     if (c1 <= c0) return;
     const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));           // rows that belong to a clip
-    const unsigned at_u = (unsigned)(L.q * (int)a.ldu + L.d) * sizeof(T), at_d = (unsigned)(L.q * (int)a.ldd + L.d) * sizeof(T);
-    const unsigned at_z = (unsigned)(L.q * (int)a.ldz + L.d) * sizeof(T), at_y = (unsigned)(L.q * (int)a.ldy + L.d) * sizeof(T);
+    const bool gated = WHAT == 0 && a.z;
+    int t0 = at / SCAN_TILE * SCAN_TILE, buf = 0;
+    ScanRows<T> fu(a.u, a.ldu, t0, L.q, L.d), fd(a.delta, a.ldd, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d), oy(a.y, a.ldy, t0, L.q, L.d);
     float span = 0.f;
     T ru[4], rd[4], rz[4];
-    ScanStage<T, LPC> stB, stC;
-    auto fetch = [&](int t0) {
-        scan_fetch<T>(a.u, a.ldu, at_u, t0, L.q, a.rows, ru);
-        scan_fetch<T>(a.delta, a.ldd, at_d, t0, L.q, a.rows, rd);
-        if (WHAT == 0 && a.z) scan_fetch<T>(a.z, a.ldz, at_z, t0, L.q, a.rows, rz);
-        stB.load(a.B, a.ldb, t0, a.rows, N);
-        if (WHAT == 0) stC.load(a.C, a.ldc, t0, a.rows, N);
+    ScanStage<T, LPC> stB(a.B, a.ldb, t0, N), stC(a.C, a.ldc, t0, N);
+    auto fetch = [&](int t) {
+        const bool full = t + SCAN_TILE <= a.rows;
+        const int left = a.rows - t;
+        fu.fetch(ru, full, left - L.q);
+        fd.fetch(rd, full, left - L.q);
+        if (gated) fz.fetch(rz, full, left - L.q);
+        stB.load(full, left);
+        if (WHAT == 0) stC.load(full, left);
     };
-    int t0 = at / SCAN_TILE * SCAN_TILE, buf = 0;
     fetch(t0);
     stB.store(sB[0], t0, lo, hi);
     if (WHAT == 0) stC.store(sC[0], t0, lo, hi);
@@ -244,17 +251,20 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
             const float raw = (float)rd[k] + bias;
             st[k] = a.softplus ? scan_softplus(raw) : raw;
             gate[k] = 1.f;
-            if (WHAT == 0 && a.z) { const float z = (float)rz[k]; gate[k] = z * seq_sigmoid(z); }
+            if (gated) { const float z = (float)rz[k]; gate[k] = z * seq_sigmoid(z); }
         }
         // (WHAT 1: the last tile requests itself again; without a branch here and at the store the rows stay one block of code)
         const bool more = t0 + SCAN_TILE < c1;
         const int t2 = more ? t0 + SCAN_TILE : t0;
-        if (WHAT == 1 || more) fetch(t2);
+        if (WHAT == 1 || more) {
+            fu.move(more); fd.move(more); stB.move(more);
+            if (WHAT == 0) { fz.move(1); stC.move(1); }
+            fetch(t2);
+        }
         auto keep = [&](int row) {                               // the state in front of the row, for the backward pass
             if (WHAT == 0 && a.ckpt && L.in) *(seq_f4*)(a.ckpt + ((size_t)(row / SCAN_KEEP) * a.channels + L.d) * N4 + 4 * L.j) = seq_f4{h[0], h[1], h[2], h[3]};
         };
         keep(t0);
-        T* py = (T*)a.y + (int64_t)t0 * a.ldy;
         const int t1 = min(t0 + SCAN_TILE, c1);
         do {                                                     // the tile's pieces: rows at .. end-1
             const int end = min(t1, w.next);
@@ -295,13 +305,12 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
                 if constexpr (WHAT == 0) ys[k] = quad_rows<LPC>(acc, L.q);
             }
             if constexpr (WHAT == 0) {
-                const unsigned oy = scan_again(at_y);
                 if (L.in && L.j < 4) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int r = t0 + 4 * k + L.q;
                         const float y = fmaf(Dd, u[k], ys[k]) * gate[k];
-                        if (whole || (r >= at && r < end)) scan_at(py, oy + 4 * k * (unsigned)a.ldy * sizeof(T)) = (T)(live ? y : 0.f);
+                        if (whole || (r >= at && r < end)) oy.row(k) = (T)(live ? y : 0.f);
                     }
                 }
                 if (end >= w.next && w.s < n) {                  // a clip ended with the piece
@@ -316,6 +325,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
             }
             at = end;
         } while (at < t1);
+        if (WHAT == 0) oy.move(1);
         if (WHAT == 1 || more) {
             stB.store(sB[buf ^ 1], t2, lo, hi);
             if (WHAT == 0) stC.store(sC[buf ^ 1], t2, lo, hi);
@@ -396,18 +406,19 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
     }
     const int to = min(w.next, c1);                                                // rows [c0, to)
     if (ends && a.dfinal) scan_load4(a.dfinal + ((size_t)w.s * a.channels + L.d) * N, L.j, N, g);
-    const unsigned at_d = (unsigned)(L.q * (int)a.ldd + L.d) * sizeof(T), at_y = (unsigned)(L.q * (int)a.lddy + L.d) * sizeof(T), at_z = (unsigned)(L.q * (int)a.ldz + L.d) * sizeof(T);
     float span = 0.f;
-    T rd[4], ry[4], rz[4];
-    ScanStage<T, LPC> stC;
-    auto fetch = [&](int t0) {
-        scan_fetch<T>(a.delta, a.ldd, at_d, t0, L.q, a.rows, rd);
-        scan_fetch<T>(a.dy, a.lddy, at_y, t0, L.q, a.rows, ry);
-        if (a.z) scan_fetch<T>(a.z, a.ldz, at_z, t0, L.q, a.rows, rz);
-        stC.load(a.C, a.ldc, t0, a.rows, N);
-    };
     int t0 = (to - 1) / SCAN_TILE * SCAN_TILE, buf = 0;
-    fetch(t0);
+    ScanRows<T> fd(a.delta, a.ldd, t0, L.q, L.d), fy(a.dy, a.lddy, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d);
+    T rd[4], ry[4], rz[4];
+    ScanStage<T, LPC> stC(a.C, a.ldc, t0, N);
+    auto fetch = [&](bool full) {
+        const int left = a.rows - t0;
+        fd.fetch(rd, full, left - L.q);
+        fy.fetch(ry, full, left - L.q);
+        if (a.z) fz.fetch(rz, full, left - L.q);
+        stC.load(full, left);
+    };
+    fetch(t0 + SCAN_TILE <= a.rows);
     stC.store(sC[0], t0, c0, to);
     __syncthreads();
     for (; t0 >= c0; t0 -= SCAN_TILE, buf ^= 1) {
@@ -423,8 +434,10 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) { const bool live = t0 + 4 * k + L.q < to; st[k] = live ? st[k] : 0.f; dy[k] = live ? dy[k] : 0.f; }
         }
-        const int t2 = max(c0, t0 - SCAN_TILE);
-        fetch(t2);
+        // (the first tile requests itself again -- or, if it is a short last one of the array too, nothing anyone looks at)
+        const int t2 = max(c0, t0 - SCAN_TILE), down = t2 < t0 ? -1 : 0;
+        fd.move(down); fy.move(down); fz.move(down); stC.move(down);
+        fetch(t2 + SCAN_TILE <= a.rows);
         ScanPair<N4> gC(sC[buf] + 4 * L.j, SCAN_TILE / 2 - 1);
 #pragma unroll
         for (int k = 3; k >= 0; --k) {
@@ -499,27 +512,30 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
         if (a.chunks > 1) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
     } else entry(s);
     const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));            // rows that belong to a clip
-    const unsigned at_u = (unsigned)(L.q * (int)a.ldu + L.d) * sizeof(T), at_d = (unsigned)(L.q * (int)a.ldd + L.d) * sizeof(T);
-    const unsigned at_z = (unsigned)(L.q * (int)a.ldz + L.d) * sizeof(T), at_y = (unsigned)(L.q * (int)a.lddy + L.d) * sizeof(T);
-    const unsigned at_du = (unsigned)(L.q * (int)a.lddu + L.d) * sizeof(T), at_dd = (unsigned)(L.q * (int)a.lddd + L.d) * sizeof(T), at_dz = (unsigned)(L.q * (int)a.lddz + L.d) * sizeof(T);
     float* my_red = red[wave] + (lane >> 5) * N4 + 4 * L.j + 2 * ((lane >> 4) & 1);               // (its last row takes what no row wants)
+    const bool gated = a.z;
+    int t0 = (c1 - 1) / SCAN_TILE * SCAN_TILE, buf = 0, end = c1;
+    ScanRows<T> fu(a.u, a.ldu, t0, L.q, L.d), fd(a.delta, a.ldd, t0, L.q, L.d), fy(a.dy, a.lddy, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d);
+    ScanRows<T> ou(a.du, a.lddu, t0, L.q, L.d), od(a.ddelta, a.lddd, t0, L.q, L.d), oz(a.dz, a.lddz, t0, L.q, L.d);
     T ru[4], rd[4], rz[4], ry[4];
     seq_f4 kept[2];
-    ScanStage<T, LPC> stB, stC;
-    auto fetch = [&](int t0) {
-        scan_fetch<T>(a.u, a.ldu, at_u, t0, L.q, a.rows, ru);
-        scan_fetch<T>(a.delta, a.ldd, at_d, t0, L.q, a.rows, rd);
-        scan_fetch<T>(a.dy, a.lddy, at_y, t0, L.q, a.rows, ry);
-        if (a.z) scan_fetch<T>(a.z, a.ldz, at_z, t0, L.q, a.rows, rz);
-        stB.load(a.B, a.ldb, t0, a.rows, N);
-        stC.load(a.C, a.ldc, t0, a.rows, N);
-        const float* p = a.ckpt + ((size_t)(t0 / SCAN_KEEP) * a.channels + scan_again(L.d)) * N4 + 4 * L.j;
-        kept[0] = *(const seq_f4*)p;
-        kept[1] = t0 + SCAN_KEEP < a.rows ? *(const seq_f4*)(p + (size_t)a.channels * N4) : seq_f4{0.f, 0.f, 0.f, 0.f};
+    ScanStage<T, LPC> stB(a.B, a.ldb, t0, N), stC(a.C, a.ldc, t0, N);
+    const char* pk = (const char*)(a.ckpt + (size_t)(t0 / SCAN_KEEP) * a.channels * N4);
+    const unsigned kept_step = (unsigned)a.channels * N4 * 4, kept_at = (unsigned)(L.d * N4 + 4 * L.j) * 4;
+    auto fetch = [&](bool full) {
+        const int left = a.rows - t0;
+        fu.fetch(ru, full, left - L.q);
+        fd.fetch(rd, full, left - L.q);
+        fy.fetch(ry, full, left - L.q);
+        if (gated) fz.fetch(rz, full, left - L.q);
+        stB.load(full, left);
+        stC.load(full, left);
+        kept[0] = *(const seq_f4*)(pk + scan_again(kept_at));
+        kept[1] = seq_f4{0.f, 0.f, 0.f, 0.f};
+        if (full || left > SCAN_KEEP) kept[1] = *(const seq_f4*)(pk + kept_step + scan_again(kept_at));
     };
-    int t0 = (c1 - 1) / SCAN_TILE * SCAN_TILE, buf = 0, end = c1;
     if (c1 > c0) {
-        fetch(t0);
+        fetch(t0 + SCAN_TILE <= a.rows);
         stB.store(sB[0], t0, lo, hi);
         stC.store(sC[0], t0, lo, hi);
     }
@@ -534,12 +550,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
             const float raw = (float)rd[k] + bias;
             st[k] = a.softplus ? scan_softplus(raw) : raw;
             dy[k] = (float)ry[k];
-            if (a.z) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
+            if (gated) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
         }
         const int t2 = max(c0, t0 - SCAN_TILE);
-        T* pu = (T*)a.du + (int64_t)t0 * a.lddu;
-        T* pd = (T*)a.ddelta + (int64_t)t0 * a.lddd;
-        T* pz = (T*)a.dz + (int64_t)t0 * a.lddz;
         const seq_f4 k0 = kept[0], k1 = kept[1];
         do {                                                      // the tile's pieces: rows at .. end-1
             const int at = max(t0, first);
@@ -559,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
             for (int half = 1; half >= 0; --half) {
                 const int h0 = t0 + half * SCAN_KEEP;
                 if (at >= h0 + SCAN_KEEP || end <= h0) continue;
-                const float *tB = sB[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4), *tC = sC[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
+                const float* tB = sB[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
                 float h[4], ex[SCAN_KEEP][4], ah[SCAN_KEEP][4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) h[m] = half ? k1[m] : k0[m];
@@ -580,7 +593,14 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                         h[m] = fmaf(xb, b4[m], ah[i][m]);
                     }
                 }
-                if (half == 0 && at == t0) fetch(t2);
+                if (half == 0 && at == t0) {                      // (the chunk's first tile requests itself again)
+                    const int down = t2 < t0 ? -1 : 0;
+                    fu.move(down); fd.move(down); fy.move(down); fz.move(down); stB.move(down); stC.move(down);
+                    pk += (int64_t)down * 2 * (int64_t)kept_step;
+                    fetch(t2 + SCAN_TILE <= a.rows);
+                }
+                const float* tC = sC[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
+                tB = sB[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);       // (read again rather than kept in 32 registers)
 #pragma unroll
                 for (int kk = 1; kk >= 0; --kk) {
                     const int k = 2 * half + kk;
@@ -618,12 +638,12 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                     dbias += dd;
                     dD = fmaf(d4[k], uk, dD);
                     if (mine && L.j < 4) {
-                        scan_at(pu, scan_again(at_du) + 4 * k * (unsigned)a.lddu * sizeof(T)) = (T)fmaf(Dd, d4[k], s4[k] * gb);
-                        scan_at(pd, scan_again(at_dd) + 4 * k * (unsigned)a.lddd * sizeof(T)) = (T)dd;
-                        if (a.z) {
+                        ou.row(k) = (T)fmaf(Dd, d4[k], s4[k] * gb);
+                        od.row(k) = (T)dd;
+                        if (gated) {
                             const float z = (float)raw_z[k], sg = seq_sigmoid(z);
                             const float dz = (float)raw_y[k] * fmaf(Dd, uk, y) * sg * fmaf(z, 1.f - sg, 1.f);
-                            scan_at(pz, scan_again(at_dz) + 4 * k * (unsigned)a.lddz * sizeof(T)) = (T)(live ? dz : 0.f);
+                            oz.row(k) = (T)(live ? dz : 0.f);
                         }
                     }
                 }
@@ -642,11 +662,13 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
         } while (end > t0);
         stB.store(sB[buf ^ 1], t2, lo, hi);
         stC.store(sC[buf ^ 1], t2, lo, hi);
+        ou.move(-1); od.move(-1); oz.move(-1);
         __syncthreads();                                          // red complete; B and C of the next tile in place
-        for (int e = threadIdx.x; e < SCAN_TILE * W; e += 256) {
-            const int r = t0 + e / W;
-            if (r < c1) a.part_bc[((int64_t)blockIdx.x * a.rows + r) * W + e % W] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
-        }
+        float* part = a.part_bc + ((int64_t)blockIdx.x * a.rows + t0) * W;
+        const int full = min(SCAN_TILE, c1 - t0) * W;
+#pragma unroll
+        for (int e = threadIdx.x; e < SCAN_TILE * W; e += 256)
+            if (e < full) part[e] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
         __syncthreads();                                          // red read
     }
     if (a.dstate && chunk == 0) {                                 // empty clips in front of the first row
