@@ -123,7 +123,7 @@ template <typename T> struct ScanRows {
             for (int k = 0; k < 4; ++k) { v[k] = (T)0.f; if (4 * k < left) v[k] = row(k); }
         }
     }
-    __device__ __forceinline__ void move(int tiles) { p += (int64_t)tiles * (int64_t)(4u * step); }
+    template <int DIR> __device__ __forceinline__ void move(bool go) { const unsigned by = go ? 4u * step : 0u; p = DIR > 0 ? p + by : p - by; }
 };
 
 // B or C of a tile on their way to LDS as floats: requested a tile ahead, written when the rows in front are done.  A thread
@@ -151,7 +151,7 @@ template <typename T, int LPC> struct ScanStage {
             s[threadIdx.x + 256 * i] = in && (clean || (r >= lo && r < hi)) ? (float)v[i] : 0.f;
         }
     }
-    __device__ __forceinline__ void move(int tiles) { p += (int64_t)tiles * (int64_t)((SCAN_TILE / STEP) * step); }
+    template <int DIR> __device__ __forceinline__ void move(bool go) { const unsigned by = go ? (SCAN_TILE / STEP) * step : 0u; p = DIR > 0 ? p + by : p - by; }
 };
 
 // B or C of a pair of rows, read from LDS a pair ahead (and, with a scheduling barrier behind the reads, not more: the
@@ -257,8 +257,8 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
         const bool more = t0 + SCAN_TILE < c1;
         const int t2 = more ? t0 + SCAN_TILE : t0;
         if (WHAT == 1 || more) {
-            fu.move(more); fd.move(more); stB.move(more);
-            if (WHAT == 0) { fz.move(1); stC.move(1); }
+            fu.template move<1>(more); fd.template move<1>(more); stB.template move<1>(more);
+            if (WHAT == 0) { fz.template move<1>(true); stC.template move<1>(true); }
             fetch(t2);
         }
         auto keep = [&](int row) {                               // the state in front of the row, for the backward pass
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
             }
             at = end;
         } while (at < t1);
-        if (WHAT == 0) oy.move(1);
+        if (WHAT == 0) oy.template move<1>(true);
         if (WHAT == 1 || more) {
             stB.store(sB[buf ^ 1], t2, lo, hi);
             if (WHAT == 0) stC.store(sC[buf ^ 1], t2, lo, hi);
@@ -435,8 +435,9 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
             for (int k = 0; k < 4; ++k) { const bool live = t0 + 4 * k + L.q < to; st[k] = live ? st[k] : 0.f; dy[k] = live ? dy[k] : 0.f; }
         }
         // (the first tile requests itself again -- or, if it is a short last one of the array too, nothing anyone looks at)
-        const int t2 = max(c0, t0 - SCAN_TILE), down = t2 < t0 ? -1 : 0;
-        fd.move(down); fy.move(down); fz.move(down); stC.move(down);
+        const int t2 = max(c0, t0 - SCAN_TILE);
+        const bool down = t2 < t0;
+        fd.template move<-1>(down); fy.template move<-1>(down); fz.template move<-1>(down); stC.template move<-1>(down);
         fetch(t2 + SCAN_TILE <= a.rows);
         ScanPair<N4> gC(sC[buf] + 4 * L.j, SCAN_TILE / 2 - 1);
 #pragma unroll
@@ -483,6 +484,17 @@ template <int LPC> __device__ __forceinline__ void wave_fold(float (&b)[4], cons
 
 // The gradient of a chunk, from its last row to its first, in pieces like the forward's.  A piece takes its tile in halves: forward
 // from the checkpoint, with e_t = exp(s_t A) and e_t h_{t-1} of the 8 rows kept in registers, then back with the adjoint.
+//
+// What only the clips' borders need is read from the kernel's arguments where it is used (rare()): with all of them in scalar
+// registers from the start, the loop moves a hundred scalars per tile in and out of vector registers.
+typedef const __attribute__((address_space(4))) ScanArgs* ScanArgsPtr;
+__device__ __forceinline__ ScanArgsPtr scan_rare() {
+    ScanArgsPtr p = (ScanArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();                          // (the only argument)
+    asm volatile("" : "+s"(p));
+    return p;
+}
+__device__ __forceinline__ int seq_start(ScanArgsPtr p, int s) { const SeqClips c = {p->clips.start, p->clips.n, p->clips.rows}; return seq_start(c, s); }
+
 template <typename T, int LPC>
 __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     constexpr int N4 = 4 * LPC, W = 2 * N4;
@@ -498,10 +510,12 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     auto entry = [&](int s) {                                     // the gradient of the state behind clip s
 #pragma unroll
         for (int m = 0; m < 4; ++m) g[m] = 0.f;
-        if (a.dfinal && s >= 0 && s < n) scan_load4(a.dfinal + ((size_t)s * a.channels + L.d) * N, L.j, N, g);
+        const ScanArgsPtr r = scan_rare();
+        if (r->dfinal && s >= 0 && s < r->clips.n) scan_load4(r->dfinal + ((size_t)s * r->channels + L.d) * N, L.j, N, g);
     };
     auto leave = [&](int s) {                                     // g is the gradient of the state in front of clip s
-        if (a.dstate && s >= 0 && s < n && L.in) scan_store4(a.dstate + ((size_t)s * a.channels + L.d) * N, L.j, N, g);
+        const ScanArgsPtr r = scan_rare();
+        if (r->dstate && s >= 0 && s < r->clips.n && L.in) scan_store4(r->dstate + ((size_t)s * r->channels + L.d) * N, L.j, N, g);
     };
     // s = the clip of row end-1, first = its first row
     int s = __builtin_amdgcn_readfirstlane(seq_find(a.clips, c1 - 1));
@@ -579,7 +593,8 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                 if (at == first && at >= h0) {                    // the clip starts here
 #pragma unroll
                     for (int m = 0; m < 4; ++m) h[m] = 0.f;
-                    if (a.state && live) scan_load4(a.state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
+                    const ScanArgsPtr r = scan_rare();
+                    if (r->state && live) scan_load4(r->state + ((size_t)s * r->channels + L.d) * N, L.j, N, h);
                 }
 #pragma unroll
                 for (int i = 0; i < SCAN_KEEP; ++i) {
@@ -594,9 +609,10 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                     }
                 }
                 if (half == 0 && at == t0) {                      // (the chunk's first tile requests itself again)
-                    const int down = t2 < t0 ? -1 : 0;
-                    fu.move(down); fd.move(down); fy.move(down); fz.move(down); stB.move(down); stC.move(down);
-                    pk += (int64_t)down * 2 * (int64_t)kept_step;
+                    const bool down = t2 < t0;
+                    fu.template move<-1>(down); fd.template move<-1>(down); fy.template move<-1>(down); fz.template move<-1>(down);
+                    stB.template move<-1>(down); stC.template move<-1>(down);
+                    pk -= down ? 2u * kept_step : 0u;
                     fetch(t2 + SCAN_TILE <= a.rows);
                 }
                 const float* tC = sC[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
@@ -653,34 +669,38 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                 leave(s);
                 if (at > c0) {
                     const int was = s;
-                    while (s >= 0 && seq_start(a.clips, s) >= at) --s;
-                    first = s >= 0 ? __builtin_amdgcn_readfirstlane(seq_start(a.clips, s)) : 0;
-                    if (a.dstate) for (int e = s + 1; e < was; ++e) { entry(e); leave(e); }
+                    const ScanArgsPtr r = scan_rare();
+                    while (s >= 0 && seq_start(r, s) >= at) --s;
+                    first = s >= 0 ? __builtin_amdgcn_readfirstlane(seq_start(r, s)) : 0;
+                    if (r->dstate) for (int e = s + 1; e < was; ++e) { entry(e); leave(e); }
                     entry(s);
                 }
             }
         } while (end > t0);
         stB.store(sB[buf ^ 1], t2, lo, hi);
         stC.store(sC[buf ^ 1], t2, lo, hi);
-        ou.move(-1); od.move(-1); oz.move(-1);
+        ou.template move<-1>(true); od.template move<-1>(true); oz.template move<-1>(true);
         __syncthreads();                                          // red complete; B and C of the next tile in place
-        float* part = a.part_bc + ((int64_t)blockIdx.x * a.rows + t0) * W;
+        const ScanArgsPtr r = scan_rare();
+        float* part = r->part_bc + ((int64_t)blockIdx.x * r->rows + t0) * W;
         const int full = min(SCAN_TILE, c1 - t0) * W;
 #pragma unroll
         for (int e = threadIdx.x; e < SCAN_TILE * W; e += 256)
             if (e < full) part[e] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
         __syncthreads();                                          // red read
     }
-    if (a.dstate && chunk == 0) {                                 // empty clips in front of the first row
-        const int s0 = seq_find(a.clips, 0);
-        for (int e = 0; e < s0 && e < n; ++e) { entry(e); leave(e); }
+    if (scan_rare()->dstate && chunk == 0) {                                 // empty clips in front of the first row
+        const SeqClips c = {scan_rare()->clips.start, scan_rare()->clips.n, scan_rare()->clips.rows};
+        const int s0 = seq_find(c, 0);
+        for (int e = 0; e < s0 && e < c.n; ++e) { entry(e); leave(e); }
     }
     dD += seq_dpp<0xB1>(dD); dD += seq_dpp<0x4E>(dD);
     dbias += seq_dpp<0xB1>(dbias); dbias += seq_dpp<0x4E>(dbias);
     if (L.in) {
-        float* part = a.part_p + (int64_t)chunk * a.channels * (N + 2);
+        const ScanArgsPtr r = scan_rare();
+        float* part = r->part_p + (int64_t)chunk * r->channels * (N + 2);
         scan_store4(part + (size_t)L.d * N, L.j, N, dA);
-        if (L.j == 0) { part[(size_t)a.channels * N + L.d] = dD; part[(size_t)a.channels * (N + 1) + L.d] = dbias; }
+        if (L.j == 0) { part[(size_t)r->channels * N + L.d] = dD; part[(size_t)r->channels * (N + 1) + L.d] = dbias; }
     }
 }
 
