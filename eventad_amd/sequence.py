@@ -12,80 +12,103 @@ Every function launches on the current stream of its tensors' device, waits for 
 workspaces come from torch's allocator per call, so captured graphs do not share one.  The functions are differentiable
 (except the single-token and 8-bit forms, which refuse inputs that need a gradient); gradients are not differentiable
 again.  There is no CPU path: tensors must be on a GPU."""
-import contextlib
 import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import call, stream_handle
+from ._lib import NativeError, load
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACT = {None: 0, "silu": 1}
+_F32, _I32 = torch.float32, torch.int32
 MAX_TAPS, MAX_STATE = 8, 64
+_MAX_LD = 1 << 24               # row strides above this are taken by copying the array
+
+# A single-token call is bound by this file: the checks below compare identities and device numbers, read each attribute once
+# and pass plain integers to the library.
 
 
 def _fail(msg, *args):
     raise RuntimeError("eventad_amd.sequence: " + msg % args)
 
 
-_MAX_LD = 1 << 24               # row strides above this are taken by copying the array
+_functions = {}
 
 
-def _activation(name, t, rows, width, like=None):
-    """Checks t [rows, width] (None: any); returns it with adjacent channels."""
+def _call(name, *args):
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(load(), name)
+    rc = f(*args)
+    if rc:
+        raise NativeError("%s failed with code %d%s" % (name, rc, " (bad argument)" if rc == -1 else " (hipError_t)"))
+
+
+def _device(t):
+    """The GPU's number."""
     if not isinstance(t, torch.Tensor):
-        _fail("%s must be a tensor", name)
-    if like is not None:
-        if t.dtype != like.dtype or t.device != like.device:
-            _fail("%s is %s on %s, expected %s on %s", name, t.dtype, t.device, like.dtype, like.device)
-    elif t.dtype not in _DTYPE:
-        _fail("%s must be float32, bfloat16 or float16, not %s", name, t.dtype)
-    shape = t.shape
-    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (width is not None and shape[1] != width):
-        _fail("%s has shape %s, expected %s", name, tuple(shape), ("*" if rows is None else rows, "*" if width is None else width))
+        _fail("expected a tensor, got %s", type(t).__name__)
+    index = t.get_device() if t.is_cuda else -1
+    if index < 0:
+        _fail("tensors must be on a GPU (there is no CPU path)")
+    return index
+
+
+def _elsewhere(index):
+    return index != torch._C._cuda_getDevice()
+
+
+def _stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _rows(name, t, rows, width, dtype, index):
+    """Checks an array [rows, width] (None: any) -> it with adjacent channels, and its row stride in elements."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        _fail("%s must be a %s tensor on GPU %d", name, dtype, index)
+    if t.dim() != 2:
+        _fail("%s has %d dimensions, expected [rows, channels]", name, t.dim())
+    n, m = t.shape
+    if (rows is not None and n != rows) or (width is not None and m != width):
+        _fail("%s has shape %s, expected %s", name, (n, m), ("*" if rows is None else rows, "*" if width is None else width))
     ld, step = t.stride()
-    if step == 1 and (shape[1] <= ld <= _MAX_LD or shape[0] <= 1):
-        return t
-    return t.contiguous()
+    if step == 1 and m <= ld <= _MAX_LD:
+        return t, ld
+    if n <= 1 and (step == 1 or m <= 1):                         # (one row: any stride)
+        return t, m
+    return t.contiguous(), m
 
 
-def _tensor(name, t, shape, dtype, device):
-    """Checks a parameter or a state; returns it contiguous."""
+def _tensor(name, t, shape, dtype, index):
+    """Checks a parameter or a state -> it, contiguous (None stays None)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
-        _fail("%s must be a %s tensor on %s", name, dtype, device)
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        _fail("%s must be a %s tensor on GPU %d", name, dtype, index)
     if t.shape != shape:
         _fail("%s has shape %s, expected %s", name, tuple(t.shape), shape)
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _ld(t):
-    """Row stride in elements (an array of at most one row may have any)."""
-    if t is None:
-        return 0
-    ld, width = t.stride(0), t.shape[1]
-    return ld if width <= ld <= _MAX_LD else width
+def _gradient(g, like):
+    """An incoming gradient as an array [rows, channels] of like's type, zeros for None; with its row stride."""
+    if g is None:
+        g = torch.zeros_like(like, memory_format=torch.contiguous_format)
+    return _rows("the gradient", g, like.shape[0], like.shape[1], like.dtype, like.get_device())
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _clips(clip_start, rows, device):
+def _clips(clip_start, index):
     if clip_start is None:
         return None, 1
-    if not isinstance(clip_start, torch.Tensor) or clip_start.dtype != torch.int32 or clip_start.device != device or \
+    if not isinstance(clip_start, torch.Tensor) or clip_start.dtype is not _I32 or clip_start.get_device() != index or \
             clip_start.dim() != 1 or clip_start.numel() < 2:
-        _fail("clip_start must be int32[clips + 1] on %s", device)
+        _fail("clip_start must be int32[clips + 1] on GPU %d", index)
     return clip_start.contiguous(), clip_start.numel() - 1
-
-
-def _gpu(t):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _fail("tensors must be on a GPU (there is no CPU path)")
-    return t.device
 
 
 def _needs_grad(*tensors):
@@ -98,72 +121,76 @@ def _needs_grad(*tensors):
 
 def _bytes(name, *shape):
     n = ctypes.c_int64(0)
-    call(name, *shape, ctypes.byref(n))
+    _call(name, *shape, ctypes.byref(n))
     return n.value
 
 
-def _workspace(nbytes, device):
-    return torch.empty(max(16, nbytes), dtype=torch.uint8, device=device)
+def _workspace(nbytes, like):
+    return like.new_empty(max(16, nbytes), dtype=torch.uint8)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device):
-    """Makes the tensors' device current for the launches."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def _state_out(state, out):
+    if out is None or out is state:
+        return state
+    if not isinstance(out, torch.Tensor) or out.dtype is not state.dtype or out.get_device() != state.get_device() or \
+            out.shape != state.shape or not out.is_contiguous():
+        _fail("state_out must be a contiguous tensor like state")
+    if abs(out.data_ptr() - state.data_ptr()) < state.numel() * state.element_size() and out.data_ptr() != state.data_ptr():
+        _fail("state_out overlaps state")
+    return out
 
 
 # ---------------------------------------------------------------------------------------------------- causal convolution
-def _conv_fwd(x, w, bias, starts, clips, state, act, want_state):
+def _conv_args(x, weight, bias, state, activation, clips, index):
+    if activation not in _ACT:
+        _fail("activation must be None or 'silu', not %r", activation)
+    if x.dtype not in _DTYPE:
+        _fail("x must be float32, bfloat16 or float16, not %s", x.dtype)
+    x, ldx = _rows("x", x, None, None, x.dtype, index)
+    D = x.shape[1]
+    taps = weight.shape[1] if isinstance(weight, torch.Tensor) and weight.dim() == 2 else 0
+    if D < 1 or not 1 <= taps <= MAX_TAPS:
+        _fail("weight must be [channels, taps] with 1..%d taps, x [rows, channels] with at least one channel", MAX_TAPS)
+    weight = _tensor("weight", weight, (D, taps), _F32, index)
+    bias = _tensor("bias", bias, (D,), _F32, index)
+    state = _tensor("state", state, (clips, taps - 1, D), x.dtype, index)
+    return x, ldx, weight, bias, state, taps
+
+
+def _conv_fwd(x, ldx, w, bias, starts, clips, state, act, want_state):
     rows, D = x.shape
-    y = torch.empty((rows, D), dtype=x.dtype, device=x.device)
-    final = torch.empty((clips, w.shape[1] - 1, D), dtype=x.dtype, device=x.device) if want_state else None
-    call("eventad_causal_conv_fwd", _p(x), _ld(x), _p(w), _p(bias), _p(starts), clips, _p(state), _p(final), _p(y), D, rows, D,
-         w.shape[1], act, _DTYPE[x.dtype], stream_handle())
+    taps = w.shape[1]
+    y = x.new_empty((rows, D))
+    final = x.new_empty((clips, taps - 1, D)) if want_state else None
+    _call("eventad_causal_conv_fwd", _p(x), ldx, _p(w), _p(bias), _p(starts), clips, _p(state), _p(final), _p(y), D, rows, D, taps, act,
+          _DTYPE[x.dtype], _stream(x.get_device()))
     return y, final
 
 
 class _ConvFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, starts, clips, state, act, want_state):
+    def forward(ctx, x, w, bias, state, ldx, starts, clips, act, want_state):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, w, bias, starts, state)
-        ctx.clips, ctx.act = clips, act
-        return _conv_fwd(x, w, bias, starts, clips, state, act, want_state)
+        ctx.save_for_backward(x, w, bias, state, starts)
+        ctx.ldx, ctx.clips, ctx.act = ldx, clips, act
+        return _conv_fwd(x, ldx, w, bias, starts, clips, state, act, want_state)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
-        x, w, bias, starts, state = ctx.saved_tensors
+        x, w, bias, state, starts = ctx.saved_tensors
         rows, D = x.shape
         K = w.shape[1]
-        with _on(x.device):
-            dy = torch.zeros_like(x) if dy is None else _activation("the gradient", dy, rows, D, x)
+        with torch.cuda.device(x.device):
+            dy, ldy = _gradient(dy, x)
             dfinal = None if dfinal is None else dfinal.contiguous()
-            dx = torch.empty((rows, D), dtype=x.dtype, device=x.device)
-            dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[5] else None
-            dp = torch.empty(D * (K + 1), device=x.device)
-            n = _bytes("eventad_causal_conv_workspace", rows, D, K)
-            ws = _workspace(n, x.device)
-            call("eventad_causal_conv_bwd", _p(x), _ld(x), _p(w), _p(bias), _p(starts), ctx.clips, _p(state), _p(dy), _ld(dy), _p(dfinal),
-                 _p(dx), D, _p(dstate), _p(dp), _p(ws), ws.numel(), rows, D, K, ctx.act, _DTYPE[x.dtype], stream_handle())
-        return dx, dp[:D * K].view(D, K), dp[D * K:] if bias is not None else None, None, None, dstate, None, None
-
-
-def _conv_args(x, weight, bias, state, activation, clips):
-    dev = _gpu(x)
-    if activation not in _ACT:
-        _fail("activation must be None or 'silu', not %r", activation)
-    x = _activation("x", x, None, None)
-    D = x.shape[1]
-    taps = weight.shape[1] if isinstance(weight, torch.Tensor) and weight.dim() == 2 else 0
-    if D < 1 or not 1 <= taps <= MAX_TAPS:
-        _fail("weight must be [channels, taps] with 1..%d taps, x [rows, channels] with at least one channel", MAX_TAPS)
-    weight = _tensor("weight", weight, (D, taps), torch.float32, dev)
-    bias = _tensor("bias", bias, (D,), torch.float32, dev)
-    state = _tensor("state", state, (clips, taps - 1, D), x.dtype, dev)
-    return x, weight, bias, state, _ACT[activation]
+            dx = x.new_empty((rows, D))
+            dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
+            dp = w.new_empty(D * (K + 1))
+            ws = _workspace(_bytes("eventad_causal_conv_workspace", rows, D, K), x)
+            _call("eventad_causal_conv_bwd", _p(x), ctx.ldx, _p(w), _p(bias), _p(starts), ctx.clips, _p(state), _p(dy), ldy, _p(dfinal),
+                  _p(dx), D, _p(dstate), _p(dp), _p(ws), ws.numel(), rows, D, K, ctx.act, _DTYPE[x.dtype], _stream(x.get_device()))
+        return dx, dp[:D * K].view(D, K), dp[D * K:] if bias is not None else None, dstate, None, None, None, None, None
 
 
 def causal_conv(x, weight, bias=None, clip_start=None, state=None, activation="silu", return_state=False):
@@ -173,13 +200,16 @@ def causal_conv(x, weight, bias=None, clip_start=None, state=None, activation="s
     [channels]; activation None or "silu" (x sigmoid(x)).  state [clips, taps - 1, channels], of x's type, holds the inputs in
     front of each clip's first row, oldest first (None: zeros).
     -> y, or (y, final_state) with return_state: the inputs in front of the row that would follow each clip."""
-    starts, clips = _clips(clip_start, x.shape[0] if isinstance(x, torch.Tensor) else 0, _gpu(x))
-    x, weight, bias, state, act = _conv_args(x, weight, bias, state, activation, clips)
-    with _on(x.device):
-        if _needs_grad(x, weight, bias, state):
-            y, final = _ConvFn.apply(x, weight, bias, starts, clips, state, act, return_state)
-        else:
-            y, final = _conv_fwd(x, weight, bias, starts, clips, state, act, return_state)
+    index = _device(x)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return causal_conv(x, weight, bias, clip_start, state, activation, return_state)
+    starts, clips = _clips(clip_start, index)
+    x, ldx, weight, bias, state, _ = _conv_args(x, weight, bias, state, activation, clips, index)
+    if _needs_grad(x, weight, bias, state):
+        y, final = _ConvFn.apply(x, weight, bias, state, ldx, starts, clips, _ACT[activation], return_state)
+    else:
+        y, final = _conv_fwd(x, ldx, weight, bias, starts, clips, state, _ACT[activation], return_state)
     return (y, final) if return_state else y
 
 
@@ -189,90 +219,86 @@ def causal_conv_step(x, weight, state, bias=None, activation="silu", state_out=N
     channels]."""
     if _needs_grad(x, weight, state, bias):
         _fail("the single-token form has no gradient: use causal_conv, or torch.no_grad()")
-    x, weight, bias, checked, act = _conv_args(x, weight, bias, state, activation, x.shape[0])
+    index = _device(x)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return causal_conv_step(x, weight, state, bias, activation, state_out)
+    x, ldx, weight, bias, checked, taps = _conv_args(x, weight, bias, state, activation, x.shape[0] if x.dim() else 0, index)
     if checked is not state or checked is None:
         _fail("state must be contiguous, of x's type, [clips, taps - 1, channels]")
     out = _state_out(state, state_out)
-    with _on(x.device):
-        y = torch.empty((x.shape[0], x.shape[1]), dtype=x.dtype, device=x.device)
-        call("eventad_causal_conv_step", _p(x), _ld(x), _p(weight), _p(bias), _p(state), _p(out), _p(y), x.shape[1], x.shape[0],
-             x.shape[1], weight.shape[1], act, _DTYPE[x.dtype], stream_handle())
-        torch.autograd.graph.increment_version(out)              # written behind autograd's back
+    clips, D = x.shape
+    y = x.new_empty((clips, D))
+    _call("eventad_causal_conv_step", x.data_ptr(), ldx, weight.data_ptr(), _p(bias), state.data_ptr(), out.data_ptr(), y.data_ptr(), D, clips,
+          D, taps, _ACT[activation], _DTYPE[x.dtype], _stream(index))
+    torch.autograd.graph.increment_version(out)                  # (written behind autograd's back)
     return y
 
 
-def _state_out(state, out):
-    if out is None or out is state:
-        return state
-    if not isinstance(out, torch.Tensor) or out.dtype != state.dtype or out.device != state.device or out.shape != state.shape or \
-            not out.is_contiguous():
-        _fail("state_out must be a contiguous tensor like state")
-    size = state.numel() * state.element_size()
-    if abs(out.data_ptr() - state.data_ptr()) < size and out.data_ptr() != state.data_ptr():
-        _fail("state_out overlaps state")
-    return out
-
-
 # -------------------------------------------------------------------------------------------------------- selective scan
-def _scan_fwd(u, delta, A, B, C, D, z, bias, starts, clips, state, softplus, want_state, want_checkpoint):
+def _scan_args(u, delta, A, B, C, D, z, bias, state, clips, index):
+    """-> the checked tensors, and the row strides of u, delta, B, C, z"""
+    dt = u.dtype
+    if dt not in _DTYPE:
+        _fail("u must be float32, bfloat16 or float16, not %s", dt)
+    u, ldu = _rows("u", u, None, None, dt, index)
+    rows, ch = u.shape
+    N = A.shape[1] if isinstance(A, torch.Tensor) and A.dim() == 2 else 0
+    if ch < 1 or not 1 <= N <= MAX_STATE:
+        _fail("A must be [channels, states] with 1..%d states, u [rows, channels] with at least one channel", MAX_STATE)
+    delta, ldd = _rows("delta", delta, rows, ch, dt, index)
+    A = _tensor("A", A, (ch, N), _F32, index)
+    B, ldb = _rows("B", B, rows, N, dt, index)
+    C, ldc = _rows("C", C, rows, N, dt, index)
+    D = _tensor("D", D, (ch,), _F32, index)
+    z, ldz = (None, 0) if z is None else _rows("z", z, rows, ch, dt, index)
+    bias = _tensor("delta_bias", bias, (ch,), _F32, index)
+    state = _tensor("state", state, (clips, ch, N), _F32, index)
+    return (u, delta, A, B, C, D, z, bias, state), (ldu, ldd, ldb, ldc, ldz)
+
+
+def _scan_fwd(u, delta, A, B, C, D, z, bias, state, lds, starts, clips, softplus, want_state, want_checkpoint):
     rows, ch = u.shape
     N = A.shape[1]
-    y = torch.empty((rows, ch), dtype=u.dtype, device=u.device)
-    final = torch.empty((clips, ch, N), device=u.device) if want_state else None
-    ckpt = _workspace(_bytes("eventad_selective_scan_checkpoint", rows, ch, N), u.device) if want_checkpoint else None
-    ws = _workspace(_bytes("eventad_selective_scan_workspace", rows, ch, N, 0), u.device)
-    call("eventad_selective_scan_fwd", _p(u), _ld(u), _p(delta), _ld(delta), _p(A), _p(B), _ld(B), _p(C), _ld(C), _p(D), _p(z), _ld(z),
-         _p(bias), _p(starts), clips, _p(state), _p(final), _p(y), ch, _p(ckpt), _p(ws), ws.numel(), rows, ch, N, softplus,
-         _DTYPE[u.dtype], stream_handle())
+    ldu, ldd, ldb, ldc, ldz = lds
+    y = u.new_empty((rows, ch))
+    final = A.new_empty((clips, ch, N)) if want_state else None
+    ckpt = _workspace(_bytes("eventad_selective_scan_checkpoint", rows, ch, N), u) if want_checkpoint else None
+    ws = _workspace(_bytes("eventad_selective_scan_workspace", rows, ch, N, 0), u)
+    _call("eventad_selective_scan_fwd", _p(u), ldu, _p(delta), ldd, _p(A), _p(B), ldb, _p(C), ldc, _p(D), _p(z), ldz, _p(bias), _p(starts), clips,
+          _p(state), _p(final), _p(y), ch, _p(ckpt), _p(ws), ws.numel(), rows, ch, N, softplus, _DTYPE[u.dtype], _stream(u.get_device()))
     return y, final, ckpt
 
 
 class _ScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, bias, starts, clips, state, softplus, want_state):
+    def forward(ctx, u, delta, A, B, C, D, z, bias, state, lds, starts, clips, softplus, want_state):
         ctx.set_materialize_grads(False)
-        y, final, ckpt = _scan_fwd(u, delta, A, B, C, D, z, bias, starts, clips, state, softplus, want_state, True)
-        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, starts, state, ckpt)
-        ctx.clips, ctx.softplus = clips, softplus
+        y, final, ckpt = _scan_fwd(u, delta, A, B, C, D, z, bias, state, lds, starts, clips, softplus, want_state, True)
+        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, state, starts, ckpt)
+        ctx.lds, ctx.clips, ctx.softplus = lds, clips, softplus
         return y, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
-        u, delta, A, B, C, D, z, bias, starts, state, ckpt = ctx.saved_tensors
+        u, delta, A, B, C, D, z, bias, state, starts, ckpt = ctx.saved_tensors
         rows, ch = u.shape
         N = A.shape[1]
-        with _on(u.device):
-            dy = torch.zeros_like(u) if dy is None else _activation("the gradient", dy, rows, ch, u)
+        ldu, ldd, ldb, ldc, ldz = ctx.lds
+        with torch.cuda.device(u.device):
+            dy, ldy = _gradient(dy, u)
             dfinal = None if dfinal is None else dfinal.contiguous()
-            new = lambda n: torch.empty((rows, n), dtype=u.dtype, device=u.device)
+            new = lambda n: u.new_empty((rows, n))
             du, dd, dB, dC, dz = new(ch), new(ch), new(N), new(N), new(ch) if z is not None else None
-            dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[10] else None
-            dp = torch.empty(ch * (N + 2), device=u.device)
-            ws = _workspace(_bytes("eventad_selective_scan_workspace", rows, ch, N, 1), u.device)
-            call("eventad_selective_scan_bwd", _p(u), _ld(u), _p(delta), _ld(delta), _p(A), _p(B), _ld(B), _p(C), _ld(C), _p(D), _p(z),
-                 _ld(z), _p(bias), _p(starts), ctx.clips, _p(state), _p(ckpt), _p(dy), _ld(dy), _p(dfinal), _p(du), ch, _p(dd), ch,
-                 _p(dB), N, _p(dC), N, _p(dz), ch, _p(dstate), _p(dp), _p(ws), ws.numel(), rows, ch, N, ctx.softplus,
-                 _DTYPE[u.dtype], stream_handle())
-        dA = dp[:ch * N].view(ch, N)
-        return (du, dd, dA, dB, dC, dp[ch * N:ch * (N + 1)] if D is not None else None, dz,
-                dp[ch * (N + 1):] if bias is not None else None, None, None, dstate, None, None)
-
-
-def _scan_args(u, delta, A, B, C, D, z, bias, state, clips):
-    dev, f32 = _gpu(u), torch.float32
-    u = _activation("u", u, None, None)
-    rows, ch = u.shape
-    if ch < 1 or not isinstance(A, torch.Tensor) or A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
-        _fail("A must be [channels, states] with 1..%d states, u [rows, channels] with at least one channel", MAX_STATE)
-    N = A.shape[1]
-    delta = _activation("delta", delta, rows, ch, u)
-    A = _tensor("A", A, (ch, N), f32, dev)
-    B, C = _activation("B", B, rows, N, u), _activation("C", C, rows, N, u)
-    D, bias = _tensor("D", D, (ch,), f32, dev), _tensor("delta_bias", bias, (ch,), f32, dev)
-    z = None if z is None else _activation("z", z, rows, ch, u)
-    state = _tensor("state", state, (clips, ch, N), f32, dev)
-    return u, delta, A, B, C, D, z, bias, state
+            dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[8] else None
+            dp = A.new_empty(ch * (N + 2))
+            ws = _workspace(_bytes("eventad_selective_scan_workspace", rows, ch, N, 1), u)
+            _call("eventad_selective_scan_bwd", _p(u), ldu, _p(delta), ldd, _p(A), _p(B), ldb, _p(C), ldc, _p(D), _p(z), ldz, _p(bias), _p(starts),
+                  ctx.clips, _p(state), _p(ckpt), _p(dy), ldy, _p(dfinal), _p(du), ch, _p(dd), ch, _p(dB), N, _p(dC), N, _p(dz), ch,
+                  _p(dstate), _p(dp), _p(ws), ws.numel(), rows, ch, N, ctx.softplus, _DTYPE[u.dtype], _stream(u.get_device()))
+        return (du, dd, dp[:ch * N].view(ch, N), dB, dC, dp[ch * N:ch * (N + 1)] if D is not None else None, dz,
+                dp[ch * (N + 1):] if bias is not None else None, dstate, None, None, None, None, None)
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=True, clip_start=None, state=None,
@@ -282,14 +308,22 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     u, delta, z [rows, channels]; B, C [rows, states], shared by the channels; A float32 [channels, states], states 1..64;
     D, delta_bias float32 [channels].  D, z and delta_bias may be None; delta_softplus=False takes delta + delta_bias as the step
     itself.  state float32 [clips, channels, states] = h in front of each clip's first row (None: zeros).
-    -> y, or (y, final_state) with return_state: h behind each clip's last row (an empty clip keeps its state)."""
-    starts, clips = _clips(clip_start, u.shape[0] if isinstance(u, torch.Tensor) else 0, _gpu(u))
-    u, delta, A, B, C, D, z, delta_bias, state = _scan_args(u, delta, A, B, C, D, z, delta_bias, state, clips)
-    with _on(u.device):
-        if _needs_grad(u, delta, A, B, C, D, z, delta_bias, state):
-            y, final = _ScanFn.apply(u, delta, A, B, C, D, z, delta_bias, starts, clips, state, int(bool(delta_softplus)), return_state)
-        else:
-            y, final, _ = _scan_fwd(u, delta, A, B, C, D, z, delta_bias, starts, clips, state, int(bool(delta_softplus)), return_state, False)
+    -> y, or (y, final_state) with return_state: h behind each clip's last row (an empty clip keeps its state).
+
+    Every clip's end inside a group of 16 rows costs that group another turn: a batch whose clips are all a row or two long is
+    better served by selective_scan_step.  With a gradient pending, the call keeps 2 x channels x (states, rounded up to 16, 32
+    or 64) bytes per 4 rows."""
+    index = _device(u)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return selective_scan(u, delta, A, B, C, D, z, delta_bias, delta_softplus, clip_start, state, return_state)
+    starts, clips = _clips(clip_start, index)
+    t, lds = _scan_args(u, delta, A, B, C, D, z, delta_bias, state, clips, index)
+    softplus = int(bool(delta_softplus))
+    if _needs_grad(*t):
+        y, final = _ScanFn.apply(*t, lds, starts, clips, softplus, return_state)
+    else:
+        y, final, _ = _scan_fwd(*t, lds, starts, clips, softplus, return_state, False)
     return (y, final) if return_state else y
 
 
@@ -299,51 +333,55 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     and left as it was.  -> y [clips, channels]."""
     if _needs_grad(u, delta, A, B, C, state, D, z, delta_bias):
         _fail("the single-token form has no gradient: use selective_scan, or torch.no_grad()")
-    u, delta, A, B, C, D, z, delta_bias, checked = _scan_args(u, delta, A, B, C, D, z, delta_bias, state, u.shape[0])
+    index = _device(u)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return selective_scan_step(u, delta, A, B, C, state, D, z, delta_bias, delta_softplus, state_out)
+    (u, delta, A, B, C, D, z, delta_bias, checked), (ldu, ldd, ldb, ldc, ldz) = \
+        _scan_args(u, delta, A, B, C, D, z, delta_bias, state, u.shape[0] if u.dim() else 0, index)
     if checked is not state or checked is None:
         _fail("state must be contiguous float32 [clips, channels, states]")
     out = _state_out(state, state_out)
     clips, ch = u.shape
-    with _on(u.device):
-        y = torch.empty((clips, ch), dtype=u.dtype, device=u.device)
-        call("eventad_selective_scan_step", _p(u), _ld(u), _p(delta), _ld(delta), _p(A), _p(B), _ld(B), _p(C), _ld(C), _p(D), _p(z), _ld(z),
-             _p(delta_bias), _p(state), _p(out), _p(y), ch, clips, ch, A.shape[1], int(bool(delta_softplus)), _DTYPE[u.dtype],
-             stream_handle())
-        torch.autograd.graph.increment_version(out)
+    y = u.new_empty((clips, ch))
+    _call("eventad_selective_scan_step", u.data_ptr(), ldu, delta.data_ptr(), ldd, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc, _p(D),
+          _p(z), ldz, _p(delta_bias), state.data_ptr(), out.data_ptr(), y.data_ptr(), ch, clips, ch, A.shape[1], 1 if delta_softplus else 0,
+          _DTYPE[u.dtype], _stream(index))
+    torch.autograd.graph.increment_version(out)
     return y
 
 
 # ------------------------------------------------------------------------------------------------------------- RMS norm
-def _norm_args(x, weight, residual, eps):
-    dev = _gpu(x)
-    x = _activation("x", x, None, None)
-    if x.shape[1] < 1:
-        _fail("x must have at least one channel")
+def _norm_args(x, weight, residual, eps, index):
+    if x.dtype not in _DTYPE:
+        _fail("x must be float32, bfloat16 or float16, not %s", x.dtype)
+    x, ldx = _rows("x", x, None, None, x.dtype, index)
+    rows, D = x.shape
+    if D < 1 or weight is None:
+        _fail("x must have at least one channel, and weight must be a float32 tensor")
     if not float(eps) >= 0.0:
         _fail("eps must not be negative")
-    if weight is None:
-        _fail("weight must be a float32 tensor")
-    weight = _tensor("weight", weight, (x.shape[1],), torch.float32, dev)
-    residual = None if residual is None else _activation("residual", residual, x.shape[0], x.shape[1], x)
-    return x, weight, residual, float(eps)
+    weight = _tensor("weight", weight, (D,), _F32, index)
+    residual, ldr = (None, 0) if residual is None else _rows("residual", residual, rows, D, x.dtype, index)
+    return x, ldx, weight, residual, ldr
 
 
-def _norm_fwd(x, weight, residual, eps):
+def _norm_fwd(x, ldx, weight, residual, ldr, eps):
     rows, D = x.shape
-    y = torch.empty((rows, D), dtype=x.dtype, device=x.device)
-    total = torch.empty_like(y) if residual is not None else None
-    call("eventad_rms_norm_fwd", _p(x), _ld(x), _p(residual), _ld(residual), _p(weight), _p(total), D, _p(y), D, rows, D, eps,
-         _DTYPE[x.dtype], stream_handle())
+    y = x.new_empty((rows, D))
+    total = x.new_empty((rows, D)) if residual is not None else None
+    _call("eventad_rms_norm_fwd", x.data_ptr(), ldx, _p(residual), ldr, weight.data_ptr(), _p(total), D, y.data_ptr(), D, rows, D, eps,
+          _DTYPE[x.dtype], _stream(x.get_device()))
     return y, total
 
 
 class _NormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps):
+    def forward(ctx, x, weight, residual, ldx, ldr, eps):
         ctx.set_materialize_grads(False)
-        y, total = _norm_fwd(x, weight, residual, eps)
+        y, total = _norm_fwd(x, ldx, weight, residual, ldr, eps)
         ctx.save_for_backward(x if total is None else total, weight)
-        ctx.eps = eps
+        ctx.ldh, ctx.eps = ldx if total is None else x.shape[1], eps
         return y, total
 
     @staticmethod
@@ -351,24 +389,30 @@ class _NormFn(torch.autograd.Function):
     def backward(ctx, dy, dtotal):
         h, weight = ctx.saved_tensors
         rows, D = h.shape
-        with _on(h.device):
-            dy = torch.zeros_like(h) if dy is None else _activation("the gradient", dy, rows, D, h)
-            dtotal = None if dtotal is None else _activation("the gradient", dtotal, rows, D, h)
-            dh = torch.empty((rows, D), dtype=h.dtype, device=h.device)
-            dw = torch.empty(D, device=h.device)
-            ws = _workspace(_bytes("eventad_rms_norm_workspace", rows, D), h.device)
-            call("eventad_rms_norm_bwd", _p(h), _ld(h), _p(weight), _p(dy), _ld(dy), _p(dtotal), _ld(dtotal), _p(dh), D, _p(dw), _p(ws),
-                 ws.numel(), rows, D, ctx.eps, _DTYPE[h.dtype], stream_handle())
-        return dh, dw, dh if ctx.needs_input_grad[2] else None, None
+        with torch.cuda.device(h.device):
+            dy, ldy = _gradient(dy, h)
+            dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h)
+            dh = h.new_empty((rows, D))
+            dw = weight.new_empty(D)
+            ws = _workspace(_bytes("eventad_rms_norm_workspace", rows, D), h)
+            _call("eventad_rms_norm_bwd", _p(h), ctx.ldh, _p(weight), _p(dy), ldy, _p(dtotal), ldt, _p(dh), D, _p(dw), _p(ws), ws.numel(), rows,
+                  D, ctx.eps, _DTYPE[h.dtype], _stream(h.get_device()))
+        return dh, dw, dh if ctx.needs_input_grad[2] else None, None, None, None
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """y = h / sqrt(mean(h^2) + eps) * weight over the channels of a row, weight float32 [channels].  With a residual (like x)
     h = x + residual rounded to their type -- the norm and its gradient are those of the stored sum -- and the result is (y, h);
     without one h = x and the result is y."""
-    x, weight, residual, eps = _norm_args(x, weight, residual, eps)
-    with _on(x.device):
-        y, total = _NormFn.apply(x, weight, residual, eps) if _needs_grad(x, weight, residual) else _norm_fwd(x, weight, residual, eps)
+    index = _device(x)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return rms_norm(x, weight, residual, eps)
+    x, ldx, weight, residual, ldr = _norm_args(x, weight, residual, eps, index)
+    if _needs_grad(x, weight, residual):
+        y, total = _NormFn.apply(x, weight, residual, ldx, ldr, float(eps))
+    else:
+        y, total = _norm_fwd(x, ldx, weight, residual, ldr, eps)
     return y if residual is None else (y, total)
 
 
@@ -377,12 +421,15 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     q torch.float8_e4m3fn [rows, channels] = y / scale rounded to nearest even.  -> (q, scale), or (q, scale, h) with a residual."""
     if _needs_grad(x, weight, residual):
         _fail("the 8-bit form has no gradient: use rms_norm, or torch.no_grad()")
-    x, weight, residual, eps = _norm_args(x, weight, residual, eps)
+    index = _device(x)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return rms_norm_fp8(x, weight, residual, eps)
+    x, ldx, weight, residual, ldr = _norm_args(x, weight, residual, eps, index)
     rows, D = x.shape
-    with _on(x.device):
-        q = torch.empty((rows, D), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(rows, device=x.device)
-        total = torch.empty((rows, D), dtype=x.dtype, device=x.device) if residual is not None else None
-        call("eventad_rms_norm_fp8", _p(x), _ld(x), _p(residual), _ld(residual), _p(weight), _p(total), D, _p(q), D, _p(scale), rows, D, eps,
-             _DTYPE[x.dtype], stream_handle())
+    q = x.new_empty((rows, D), dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(rows, dtype=_F32)
+    total = x.new_empty((rows, D)) if residual is not None else None
+    _call("eventad_rms_norm_fp8", x.data_ptr(), ldx, _p(residual), ldr, weight.data_ptr(), _p(total), D, q.data_ptr(), D, scale.data_ptr(), rows,
+          D, eps, _DTYPE[x.dtype], _stream(index))
     return (q, scale) if residual is None else (q, scale, total)
