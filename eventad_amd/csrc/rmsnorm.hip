@@ -358,34 +358,36 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
 
 static int norm_groups(int64_t rows) { return (int)(rows < 1 ? 1 : rows < 1024 ? rows : 1024); }
 
-template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static void norm_launch3(const NormArgs& a, int groups, hipStream_t st) {
+template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static int norm_launch3(const NormArgs& a, int groups, hipStream_t st) {
     constexpr int PER = 256 / LANES;
-    const dim3 grid((unsigned)((a.rows + PER - 1) / PER)), block(256);
+    const long long blocks = (a.rows + PER - 1) / PER;
+    if (WHAT != 2 && blocks * 256 > SEQ_MOST_THREADS) return EVENTAD_ERR_TOO_LARGE;
+    const dim3 grid((unsigned)blocks), block(256);
     if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP>), grid, block, 0, st, a);
     if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fp8<T, V, LANES, ITERS, LOOP>), grid, block, 0, st, a);
     if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_bwd<T, V, LANES, ITERS, LOOP>), dim3(groups), block, 0, st, a);
+    return evad_last_error();
 }
 // The fewest lanes that hold a row in four pieces each: rows of one wave need no LDS, and short rows share a wave.
-template <int WHAT, typename T, int V> static void norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
+template <int WHAT, typename T, int V> static int norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
     const int pieces = (a.channels + V - 1) / V;
-    if (pieces <= 16) norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
-    else if (pieces <= 32) norm_launch3<WHAT, T, V, 32, 1, false>(a, groups, st);
-    else if (pieces <= 64) norm_launch3<WHAT, T, V, 64, 1, false>(a, groups, st);
-    else if (pieces <= 128) norm_launch3<WHAT, T, V, 64, 2, false>(a, groups, st);
-    else if (pieces <= 256) norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st);
-    else if (pieces <= 512) norm_launch3<WHAT, T, V, 256, 2, false>(a, groups, st);
-    else if (pieces <= 1024) norm_launch3<WHAT, T, V, 256, 4, false>(a, groups, st);
-    else norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
+    if (pieces <= 16) return norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
+    if (pieces <= 32) return norm_launch3<WHAT, T, V, 32, 1, false>(a, groups, st);
+    if (pieces <= 64) return norm_launch3<WHAT, T, V, 64, 1, false>(a, groups, st);
+    if (pieces <= 128) return norm_launch3<WHAT, T, V, 64, 2, false>(a, groups, st);
+    if (pieces <= 256) return norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st);
+    if (pieces <= 512) return norm_launch3<WHAT, T, V, 256, 2, false>(a, groups, st);
+    if (pieces <= 1024) return norm_launch3<WHAT, T, V, 256, 4, false>(a, groups, st);
+    return norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
 }
-template <int WHAT, typename T> static void norm_launch1(const NormArgs& a, bool vec, int groups, hipStream_t st) {
+template <int WHAT, typename T> static int norm_launch1(const NormArgs& a, bool vec, int groups, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
-    if (vec && a.channels % N == 0) norm_launch2<WHAT, T, N>(a, groups, st); else norm_launch2<WHAT, T, 1>(a, groups, st);
+    return vec && a.channels % N == 0 ? norm_launch2<WHAT, T, N>(a, groups, st) : norm_launch2<WHAT, T, 1>(a, groups, st);
 }
 template <int WHAT> static int norm_launch(const NormArgs& a, int dtype, bool vec, int groups, hipStream_t st) {
-    if (dtype == SEQ_F32) norm_launch1<WHAT, float>(a, vec, groups, st);
-    else if (dtype == SEQ_BF16) norm_launch1<WHAT, __bf16>(a, vec, groups, st);
-    else norm_launch1<WHAT, _Float16>(a, vec, groups, st);
-    return evad_last_error();
+    if (dtype == SEQ_F32) return norm_launch1<WHAT, float>(a, vec, groups, st);
+    if (dtype == SEQ_BF16) return norm_launch1<WHAT, __bf16>(a, vec, groups, st);
+    return norm_launch1<WHAT, _Float16>(a, vec, groups, st);
 }
 static bool norm_shape_ok(int64_t rows, int channels, int dtype) {
     return rows >= 0 && rows <= 0x7fffff00 && channels >= 1 && channels <= (1 << 24) && dtype >= 0 && dtype <= 2;

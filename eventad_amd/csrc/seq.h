@@ -96,6 +96,8 @@ __device__ __forceinline__ int seq_find(const SeqClips& c, int row) {
     return lo;
 }
 
+#define SEQ_MOST_THREADS 0xffffff00LL          // of one launch (threads are numbered in 32 bits)
+
 static inline bool seq_aligned(const void* p, int64_t row_bytes) { return (((uintptr_t)p | (uintptr_t)row_bytes) & 15) == 0; }
 
 // ---- column sums: out[c] = sum over rows of in[rows][cols], in a fixed order.  `scratch` holds SEQ_SUM_PARTS x cols floats.

@@ -429,36 +429,39 @@ int seq_colsum(const float* in, int64_t rows, int64_t cols, float* out, float* s
 }
 
 // ---- entry points --------------------------------------------------------------------------------------------------------
-template <int WHAT, typename T, int V, int K> static void conv_launch3(const ConvArgs& a, hipStream_t st) {
-    const dim3 block(256);
-    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_step<T, V, K>), dim3(evad_blocks((long long)a.cols * a.rows, 256)), block, 0, st, a);
-    else if (a.cols >= 64) {
-        const dim3 grid(evad_blocks((long long)((a.cols + 63) / 64) * a.chunks, 4));
-        if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_bwd<T, V, K, true>), grid, block, 0, st, a);
-    } else {
-        const dim3 grid(evad_blocks((long long)a.cols * a.chunks, 256));
-        if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K, false>), grid, block, 0, st, a);
+template <int WHAT, typename T, int V, int K> static int conv_launch3(const ConvArgs& a, hipStream_t st) {
+    const bool wave = WHAT != 2 && a.cols >= 64;
+    const long long items = wave ? (long long)((a.cols + 63) / 64) * a.chunks * 64 : (long long)a.cols * (WHAT == 2 ? a.rows : a.chunks);
+    if (items > SEQ_MOST_THREADS) return EVENTAD_ERR_TOO_LARGE;
+    const dim3 grid(evad_blocks(items, 256)), block(256);
+    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_step<T, V, K>), grid, block, 0, st, a);
+    if constexpr (WHAT == 0) {
+        if (wave) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_fwd<T, V, K, false>), grid, block, 0, st, a);
+    }
+    if constexpr (WHAT == 1) {
+        if (wave) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_bwd<T, V, K, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_bwd<T, V, K, false>), grid, block, 0, st, a);
     }
+    return evad_last_error();
 }
-template <int WHAT, typename T, int V> static void conv_launch2(const ConvArgs& a, hipStream_t st) {
+template <int WHAT, typename T, int V> static int conv_launch2(const ConvArgs& a, hipStream_t st) {
     switch (a.taps) {
-        case 2: conv_launch3<WHAT, T, V, 2>(a, st); break;
-        case 3: conv_launch3<WHAT, T, V, 3>(a, st); break;
-        case 4: conv_launch3<WHAT, T, V, 4>(a, st); break;
-        default: conv_launch3<WHAT, T, V, 8>(a, st); break;
+        case 2: return conv_launch3<WHAT, T, V, 2>(a, st);
+        case 3: return conv_launch3<WHAT, T, V, 3>(a, st);
+        case 4: return conv_launch3<WHAT, T, V, 4>(a, st);
+        default: return conv_launch3<WHAT, T, V, 8>(a, st);
     }
 }
-template <int WHAT, typename T> static void conv_launch1(ConvArgs& a, bool vec, hipStream_t st) {
-    if (vec && a.channels % 4 == 0) { a.cols = a.channels / 4; conv_launch2<WHAT, T, 4>(a, st); }
-    else { a.cols = a.channels; conv_launch2<WHAT, T, 1>(a, st); }
+template <int WHAT, typename T> static int conv_launch1(ConvArgs& a, bool vec, hipStream_t st) {
+    const bool four = vec && a.channels % 4 == 0;
+    a.cols = four ? a.channels / 4 : a.channels;
+    return four ? conv_launch2<WHAT, T, 4>(a, st) : conv_launch2<WHAT, T, 1>(a, st);
 }
 template <int WHAT> static int conv_launch(ConvArgs& a, int dtype, bool vec, hipStream_t st) {
-    if (dtype == SEQ_F32) conv_launch1<WHAT, float>(a, vec, st);
-    else if (dtype == SEQ_BF16) conv_launch1<WHAT, __bf16>(a, vec, st);
-    else conv_launch1<WHAT, _Float16>(a, vec, st);
-    return evad_last_error();
+    if (dtype == SEQ_F32) return conv_launch1<WHAT, float>(a, vec, st);
+    if (dtype == SEQ_BF16) return conv_launch1<WHAT, __bf16>(a, vec, st);
+    return conv_launch1<WHAT, _Float16>(a, vec, st);
 }
 // rows of four elements start on a border of four elements
 static bool conv_vec(const void* p, int64_t ld, int dtype) {
@@ -473,7 +476,6 @@ static int conv_chunk_rows(int64_t rows, int channels, int backward) {
     return r < 4 ? 4 : r > most ? most : (int)r / 4 * 4;
 }
 static bool conv_shape_ok(int64_t rows, int channels, int taps, int dtype) {
-    // (places are counted in 32 bits: a chunk has at least 4 rows, a token of the single-token form one)
     return rows >= 0 && rows <= 0x7ffffff0 && channels >= 1 && channels <= (1 << 20) && taps >= 1 && taps <= CONV_MAX_TAPS && dtype >= 0 && dtype <= 2;
 }
 

@@ -708,16 +708,17 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_scan_bc(const float* __restrict__ part, int blocks, int rows, int n4, int N,
                                                  T* __restrict__ dB, int64_t lddb, T* __restrict__ dC, int64_t lddc) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, width = (int64_t)rows * 2 * n4;
-    if (e >= width) return;
-    const int64_t r = e / (2 * n4);
-    const int m = (int)(e - r * 2 * n4), c = m >= n4, i = c ? m - n4 : m;
-    if (i >= N) return;
-    float s0 = 0.f, s1 = 0.f;
-    int b = 0;
-    for (; b + 1 < blocks; b += 2) { s0 += part[b * width + e]; s1 += part[(b + 1) * width + e]; }
-    if (b < blocks) s0 += part[b * width + e];
-    if (c) dC[r * lddc + i] = (T)(s0 + s1); else dB[r * lddb + i] = (T)(s0 + s1);
+    const int64_t width = (int64_t)rows * 2 * n4;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < width; e += (int64_t)gridDim.x * 256) {
+        const int64_t r = e / (2 * n4);
+        const int m = (int)(e - r * 2 * n4), c = m >= n4, i = c ? m - n4 : m;
+        if (i >= N) continue;
+        float s0 = 0.f, s1 = 0.f;
+        int b = 0;
+        for (; b + 1 < blocks; b += 2) { s0 += part[b * width + e]; s1 += part[(b + 1) * width + e]; }
+        if (b < blocks) s0 += part[b * width + e];
+        if (c) dC[r * lddc + i] = (T)(s0 + s1); else dB[r * lddb + i] = (T)(s0 + s1);
+    }
 }
 
 // One token per clip, bound by the bytes of the states: 4 N in and 4 N out per channel.  A lane owns four states of a channel
@@ -950,7 +951,8 @@ extern "C" int eventad_selective_scan_bwd(const void* u, int64_t ldu, const void
     int rc = scan_launch<3>(a, dtype, st);
     if (rc) return rc;
     if (rows) {
-        const dim3 grid(evad_blocks((long long)rows * 2 * n4, 256));
+        const long long blocks = ((long long)rows * 2 * n4 + 255) / 256;
+        const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
         if (dtype == SEQ_F32) hipLaunchKernelGGL(k_scan_bc<float>, grid, dim3(256), 0, st, a.part_bc, groups, (int)rows, n4, n_state, (float*)dB, lddb, (float*)dC, lddc);
         else if (dtype == SEQ_BF16) hipLaunchKernelGGL(k_scan_bc<__bf16>, grid, dim3(256), 0, st, a.part_bc, groups, (int)rows, n4, n_state, (__bf16*)dB, lddb, (__bf16*)dC, lddc);
         else hipLaunchKernelGGL(k_scan_bc<_Float16>, grid, dim3(256), 0, st, a.part_bc, groups, (int)rows, n4, n_state, (_Float16*)dB, lddb, (_Float16*)dC, lddc);

@@ -88,6 +88,56 @@ def test_causal_conv_and_gradient(S, dtype, rows, channels, taps, kind, silu, st
         close("d" + k, g, want[k][0], (sum_units if k in ("weight", "bias") else row_units + taps) * want[k][1])
 
 
+def conv_by_shifts(x, w, bs, b, st, dy, df):
+    """R.conv for arrays of any length: float64 on the GPU, clip by clip, tap by tap."""
+    x, w, bs, st, dy, df = (t.detach().double() for t in (x, w, bs, st, dy, df))
+    K = w.shape[1]
+    out = {k: [torch.zeros_like(t), torch.zeros_like(t)] for k, t in (("y", x), ("x", x), ("weight", w), ("bias", bs), ("state", st))}
+    final = st.clone()
+    for s, (lo, hi) in enumerate(zip(b, b[1:])):
+        n = hi - lo
+        ext = torch.cat([st[s], x[lo:hi]])
+        pre, mag = bs + sum(ext[k:k + n] * w[:, k] for k in range(K)), bs.abs() + sum(ext[k:k + n].abs() * w[:, k].abs() for k in range(K))
+        sg = torch.sigmoid(pre)
+        out["y"][0][lo:hi], out["y"][1][lo:hi] = pre * sg, mag
+        final[s] = ext[n:]
+        d, dm = dy[lo:hi] * sg * (1 + pre * (1 - sg)), dy[lo:hi].abs() * (1 + mag)
+        dext, dextm = torch.zeros_like(ext), torch.zeros_like(ext)
+        dext[n:] += df[s]
+        dextm[n:] += df[s].abs()
+        for k in range(K):
+            dext[k:k + n] += d * w[:, k]
+            dextm[k:k + n] += dm * w[:, k].abs()
+            out["weight"][0][:, k] += (ext[k:k + n] * d).sum(0)
+            out["weight"][1][:, k] += (ext[k:k + n].abs() * dm).sum(0)
+        out["bias"][0] += d.sum(0)
+        out["bias"][1] += dm.sum(0)
+        out["state"][0][s], out["state"][1][s] = dext[:K - 1], dextm[:K - 1]
+        out["x"][0][lo:hi], out["x"][1][lo:hi] = dext[K - 1:], dextm[K - 1:]
+    return {k: tuple(t.cpu() for t in v) for k, v in out.items()}, final.cpu()
+
+
+@pytest.mark.parametrize("dtype,rows,channels,taps", [("f32", 60001, 512, 4), ("bf16", 50003, 300, 4), ("f16", 40001, 513, 3), ("f32", 30011, 131, 2),
+                                                      ("bf16", 40007, 256, 6), ("f32", 300001, 64, 4), ("bf16", 200003, 31, 8)])
+def test_causal_conv_over_long_chunks(S, dtype, rows, channels, taps):
+    """Arrays long enough for chunks of many groups of rows: the unbroken groups, their borders with clips and chunks, waves
+    that are not full, and several chunks per wave."""
+    gen, dt = torch.Generator().manual_seed(rows), DTYPES[dtype]
+    b = [0, 1, 7, 1000, 1000, rows // 2 + 1, rows - 66, rows - 5, rows]
+    clips = len(b) - 1
+    x, w, bs = rnd(gen, rows, channels, dtype=dt), rnd(gen, channels, taps), rnd(gen, channels)
+    st, dy, df = rnd(gen, clips, taps - 1, channels, dtype=dt), rnd(gen, rows, channels, dtype=dt), rnd(gen, clips, taps - 1, channels, dtype=dt)
+    want, final = conv_by_shifts(x, w, bs, b, st, dy, df)
+    L = [leaf(t) for t in (x, w, bs, st)]
+    y, f = S.causal_conv(L[0], L[1], L[2], starts_of(b), L[3], "silu", True)
+    close("y", y, want["y"][0], (taps + 16) * want["y"][1])
+    assert torch.equal(f.double().cpu(), final)
+    # sums over the rows: 4..128 in sequence per chunk, the chunks shared out among 64 workgroups of 4 x 4 sums
+    depth = 2 * taps + 16 + 128 + 2 * rows / 4 / 64 / 16
+    for k, g in zip(("x", "weight", "bias", "state"), torch.autograd.grad([y, f], L, [dy, df])):
+        close("d" + k, g, want[k][0], (depth if k in ("weight", "bias") else 2 * taps + 16) * want[k][1])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("clips,channels,taps", [(1, 1, 1), (1, 8, 4), (6, 256, 4), (5, 13, 3), (33, 40, 8), (3, 16, 2)])
 def test_causal_conv_step(S, dtype, clips, channels, taps):
@@ -115,6 +165,7 @@ SCAN_CASES = [  # rows, channels, states, clips, softplus, which of D z bias sta
     (16, 64, 16, "gaps", True, "Dzb"), (17, 70, 5, "empties", True, "Dzbs"), (64, 20, 16, "one", True, "Dzbs"), (65, 66, 16, "tiles", True, "Dzbs"),
     (200, 33, 16, "tiles", True, "Dzbs"), (200, 65, 16, "all", True, "zb"), (197, 16, 13, "empties", True, "Dzbs"), (150, 9, 24, "three", True, "Dzbs"),
     (130, 40, 32, "tiles", True, "Dzb"), (131, 18, 64, "three", True, "Dzbs"), (66, 5, 33, "gaps", True, "s"), (140, 12, 16, "gaps", True, ""),
+    (400, 6, 16, "tiles", True, "Dzbs"), (390, 5, 20, "one", True, "zbs"), (300, 3, 7, "empties", True, "Dzbs"), (260, 2, 50, "all", True, "Dzs"),
     (90, 8, 8, "all", False, "Dzs"), (260, 4, 1, "one", True, "Dzbs")]
 
 

@@ -100,6 +100,9 @@ def test_sequence_entry_points_refuse_bad_arguments_without_touching_the_gpu():
     for bad in (dict(x=None), dict(w=None), dict(y=None), dict(ldx=7), dict(ldy=7), dict(rows=-1), dict(rows=1 << 31), dict(channels=0),
                 dict(taps=0), dict(taps=9), dict(act=2), dict(dtype=3), dict(clips=0), dict(clips=2)):
         assert conv(**bad) == -1, bad
+    assert conv(rows=(1 << 31) - 16, channels=1 << 16, ldx=1 << 16, ldy=1 << 16) == -3       # too many threads for one launch
+    assert lib.eventad_causal_conv_step(buf, 64, buf, None, buf, buf, buf, 64, 1 << 30, 64, 4, 1, 0, None) == -3
+    assert lib.eventad_rms_norm_fwd(buf, 5000, None, 0, buf, None, 0, buf, 5000, 1 << 30, 5000, 1e-6, 0, None) == -3
     assert conv(rows=0) == 0                                     # nothing to do, nothing launched
     assert lib.eventad_causal_conv_bwd(buf, 8, buf, None, None, 1, None, buf, 8, None, buf, 8, None, buf, buf, 16, 4, 8, 4, 1, 0, None) == -1
     assert lib.eventad_causal_conv_step(buf, 8, buf, None, None, None, buf, 8, 2, 8, 4, 1, 0, None) == -1
@@ -108,7 +111,7 @@ def test_sequence_entry_points_refuse_bad_arguments_without_touching_the_gpu():
         ("z", None), ("ldz", 0), ("bias", None), ("starts", None), ("clips", 1), ("state", None), ("final", None), ("y", buf), ("ldy", 8),
         ("ckpt", None), ("ws", buf), ("wsb", 1 << 16), ("rows", 4), ("channels", 8), ("n", 16), ("softplus", 1), ("dtype", 0), ("stream", None))])
     for bad in (dict(u=None), dict(delta=None), dict(A=None), dict(B=None), dict(C=None), dict(y=None), dict(ws=None), dict(wsb=8),
-                dict(ldu=7), dict(ldb=15), dict(ldc=15), dict(z=buf, ldz=7), dict(clips=2), dict(clips=0), dict(n=0), dict(n=65),
+                dict(ldu=7), dict(ldu=(1 << 24) + 1), dict(ldb=15), dict(ldc=15), dict(z=buf, ldz=7), dict(clips=2), dict(clips=0), dict(n=0), dict(n=65),
                 dict(softplus=2), dict(dtype=-1), dict(rows=-1), dict(ckpt=ctypes.c_void_p(8 + 1))):
         assert scan(**bad) == -1, bad
     assert lib.eventad_selective_scan_bwd(*([None] * 1 + [8] + [None] * 1 + [8] + [None] * 2 + [16, None, 16, None, None, 0, None, None, 1, None,
