@@ -12,7 +12,9 @@ Every function launches on the current stream of its tensors' device, waits for 
 workspaces come from torch's allocator per call, so captured graphs do not share one.  The functions are differentiable
 (except the single-token and 8-bit forms, which refuse inputs that need a gradient); gradients are not differentiable
 again.  There is no CPU path: tensors must be on a GPU."""
+import contextlib
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -57,6 +59,13 @@ def _device(t):
 
 def _elsewhere(index):
     return index != torch._C._cuda_getDevice()
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(index):
+    return torch.cuda.device(index) if _elsewhere(index) else _here
 
 
 def _stream(index):
@@ -119,7 +128,9 @@ def _needs_grad(*tensors):
     return False
 
 
+@functools.lru_cache(maxsize=4096)
 def _bytes(name, *shape):
+    """What the library's size function says for a shape."""
     n = ctypes.c_int64(0)
     _call(name, *shape, ctypes.byref(n))
     return n.value
@@ -181,7 +192,7 @@ class _ConvFn(torch.autograd.Function):
         x, w, bias, state, starts = ctx.saved_tensors
         rows, D = x.shape
         K = w.shape[1]
-        with torch.cuda.device(x.device):
+        with _on(x.get_device()):
             dy, ldy = _gradient(dy, x)
             dfinal = None if dfinal is None else dfinal.contiguous()
             dx = x.new_empty((rows, D))
@@ -286,7 +297,7 @@ class _ScanFn(torch.autograd.Function):
         rows, ch = u.shape
         N = A.shape[1]
         ldu, ldd, ldb, ldc, ldz = ctx.lds
-        with torch.cuda.device(u.device):
+        with _on(u.get_device()):
             dy, ldy = _gradient(dy, u)
             dfinal = None if dfinal is None else dfinal.contiguous()
             new = lambda n: u.new_empty((rows, n))
@@ -389,7 +400,7 @@ class _NormFn(torch.autograd.Function):
     def backward(ctx, dy, dtotal):
         h, weight = ctx.saved_tensors
         rows, D = h.shape
-        with torch.cuda.device(h.device):
+        with _on(h.get_device()):
             dy, ldy = _gradient(dy, h)
             dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h)
             dh = h.new_empty((rows, D))
