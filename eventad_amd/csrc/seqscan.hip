@@ -167,6 +167,16 @@ template <int N4> struct ScanPair {
     __device__ __forceinline__ seq_f4 row(int i) const { return v[(i >> 1) & 1][i & 1]; }
 };
 
+// Rows at .. end-1 of a staged tile, zeros in the place of the others.  A piece that shares its tile with another clip reads this
+// copy: its own input and step of the other rows are zero, but a B or C that is infinite or no number there would get through.
+template <int N4> __device__ __forceinline__ void scan_mask(float* dst, const float* src, int t0, int at, int end) {
+#pragma unroll
+    for (int e = threadIdx.x; e < SCAN_TILE * N4; e += 256) {
+        const int r = t0 + e / N4;
+        dst[e] = r >= at && r < end ? src[e] : 0.f;
+    }
+}
+
 // The walk over the clips' ends while rows go up (all values are the same in the whole workgroup).
 struct ScanWalk { int s, next; };
 __device__ __forceinline__ ScanWalk scan_walk(const SeqClips& c, int row) {
@@ -185,7 +195,7 @@ __device__ __forceinline__ ScanWalk scan_walk(const SeqClips& c, int row) {
 template <typename T, int LPC, int WHAT>
 __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     constexpr int N4 = 4 * LPC;
-    __shared__ __attribute__((aligned(16))) float sB[2][SCAN_TILE * N4], sC[2][SCAN_TILE * N4];
+    __shared__ __attribute__((aligned(16))) float sB[WHAT == 0 ? 3 : 2][SCAN_TILE * N4], sC[WHAT == 0 ? 3 : 1][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y;
     const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
@@ -223,7 +233,8 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
         else entry(w.s);
     }
     if (c1 <= c0) return;
-    const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));           // rows that belong to a clip
+    // rows that belong to a clip (WHAT 1: to the one that matters)
+    const int lo = WHAT == 1 ? at : max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));
     const bool gated = WHAT == 0 && a.z;
     int t0 = at / SCAN_TILE * SCAN_TILE, buf = 0;
     ScanRows<T> fu(a.u, a.ldu, t0, L.q, L.d), fd(a.delta, a.ldd, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d), oy(a.y, a.ldy, t0, L.q, L.d);
@@ -241,7 +252,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     };
     fetch(t0);
     stB.store(sB[0], t0, lo, hi);
-    if (WHAT == 0) stC.store(sC[0], t0, lo, hi);
+    if constexpr (WHAT == 0) stC.store(sC[0], t0, lo, hi);
     __syncthreads();
     for (; t0 < c1; t0 += SCAN_TILE, buf ^= 1) {
         float st[4], u[4], gate[4];
@@ -268,8 +279,16 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
         const int t1 = min(t0 + SCAN_TILE, c1);
         do {                                                     // the tile's pieces: rows at .. end-1
             const int end = min(t1, w.next);
-            const float *tB = sB[buf] + scan_again(4 * L.j), *tC = sC[buf] + scan_again(4 * L.j);
             const bool whole = at == t0 && end == t0 + SCAN_TILE, live = at >= lo && at < hi;    // (of a clip, or of none)
+            int use = buf;
+            if (WHAT == 0 && !whole) {
+                use = 2;
+                __syncthreads();                                 // (the piece in front has read its copy)
+                scan_mask<N4>(sB[use], sB[buf], t0, at, end);
+                if constexpr (WHAT == 0) scan_mask<N4>(sC[use], sC[buf], t0, at, end);
+                __syncthreads();
+            }
+            const float *tB = sB[use] + scan_again(4 * L.j), *tC = WHAT == 0 ? sC[use] + scan_again(4 * L.j) : tB;
             float s4[4], x4[4], ys[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { s4[k] = st[k]; x4[k] = st[k] * u[k]; }
@@ -328,7 +347,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
         if (WHAT == 0) oy.template move<1>(true);
         if (WHAT == 1 || more) {
             stB.store(sB[buf ^ 1], t2, lo, hi);
-            if (WHAT == 0) stC.store(sC[buf ^ 1], t2, lo, hi);
+            if constexpr (WHAT == 0) stC.store(sC[buf ^ 1], t2, lo, hi);
         }
         __syncthreads();
     }
@@ -354,7 +373,7 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
     const int d = (int)(at / n4), i = (int)(at - (int64_t)d * n4);
     const float A2 = i < a.n_state ? a.A[(size_t)d * a.n_state + i] * SEQ_LOG2E : 0.f;
     const int share = (a.chunks + 15) / 16, first = group * share, last = min(a.chunks, first + share);
-    float in = 0.f, pass = 1.f;
+    float in = 0.f, pass = 1.f;                                   // pass < 0: a clip starts in the group, nothing gets through
     for (int turn = 0; turn < 2; ++turn) {                       // 0: compose, 1: hand on
         for (int k0 = first; k0 < last; k0 += 8) {
             float own[8], sp[8]; int fl[8];
@@ -370,15 +389,14 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
                 const float e = fl[j] ? 0.f : seq_exp2(sp[j] * A2);
                 if (turn) a.carry[c * width + at] = in;
                 in = fl[j] ? own[j] : fmaf(e, in, own[j]);
-                pass *= e;
+                pass = fl[j] || pass < 0.f ? -1.f : pass * e;
             }
         }
         if (turn == 0) {
             s_own[group][col] = in; s_pass[group][col] = pass;
             __syncthreads();
             in = 0.f;
-            // (nothing passes a group that holds a fresh start: its factor is 0, and 0 x infinity must not appear)
-            for (int g = 0; g < group; ++g) { const float p = s_pass[g][col]; in = p != 0.f ? fmaf(p, in, s_own[g][col]) : s_own[g][col]; }
+            for (int g = 0; g < group; ++g) { const float p = s_pass[g][col]; in = p < 0.f ? s_own[g][col] : fmaf(p, in, s_own[g][col]); }
         }
     }
 }
@@ -498,7 +516,7 @@ __device__ __forceinline__ int seq_start(ScanArgsPtr p, int s) { const SeqClips 
 template <typename T, int LPC>
 __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     constexpr int N4 = 4 * LPC, W = 2 * N4;
-    __shared__ __attribute__((aligned(16))) float sB[2][SCAN_TILE * N4], sC[2][SCAN_TILE * N4], red[4][(SCAN_TILE + 1) * W];
+    __shared__ __attribute__((aligned(16))) float sB[3][SCAN_TILE * N4], sC[3][SCAN_TILE * N4], red[4][(SCAN_TILE + 1) * W];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
@@ -571,6 +589,14 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
         do {                                                      // the tile's pieces: rows at .. end-1
             const int at = max(t0, first);
             const bool whole = at == t0 && end == t0 + SCAN_TILE, live = at >= lo && at < hi;     // (of a clip, or of none)
+            int use = buf;
+            if (!whole) {
+                use = 2;
+                __syncthreads();                                  // (the piece in front has read its copy)
+                scan_mask<N4>(sB[2], sB[buf], t0, at, end);
+                scan_mask<N4>(sC[2], sC[buf], t0, at, end);
+                __syncthreads();
+            }
             float s4[4], x4[4], d4[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { s4[k] = st[k]; x4[k] = st[k] * u[k]; d4[k] = dy[k]; }
@@ -586,7 +612,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
             for (int half = 1; half >= 0; --half) {
                 const int h0 = t0 + half * SCAN_KEEP;
                 if (at >= h0 + SCAN_KEEP || end <= h0) continue;
-                const float* tB = sB[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
+                const float* tB = sB[use] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
                 float h[4], ex[SCAN_KEEP][4], ah[SCAN_KEEP][4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) h[m] = half ? k1[m] : k0[m];
@@ -615,8 +641,8 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                     pk -= down ? 2u * kept_step : 0u;
                     fetch(t2 + SCAN_TILE <= a.rows);
                 }
-                const float* tC = sC[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
-                tB = sB[buf] + scan_again(4 * L.j + half * SCAN_KEEP * N4);       // (read again rather than kept in 32 registers)
+                const float* tC = sC[use] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
+                tB = sB[use] + scan_again(4 * L.j + half * SCAN_KEEP * N4);       // (read again rather than kept in 32 registers)
 #pragma unroll
                 for (int kk = 1; kk >= 0; --kk) {
                     const int k = 2 * half + kk;
@@ -654,7 +680,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                     dbias += dd;
                     dD = fmaf(d4[k], uk, dD);
                     if (mine && L.j < 4) {
-                        ou.row(k) = (T)fmaf(Dd, d4[k], s4[k] * gb);
+                        ou.row(k) = (T)(live ? fmaf(Dd, d4[k], s4[k] * gb) : 0.f);
                         od.row(k) = (T)dd;
                         if (gated) {
                             const float z = (float)raw_z[k], sg = seq_sigmoid(z);

@@ -257,6 +257,42 @@ def test_rows_of_no_clip_are_not_looked_at(S, value):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("channels,rows,bounds", [
+    (8, 40, [0, 5, 11, 13, 16, 27, 40]),                         # several clips inside a tile
+    (24, 700, [3, 130, 333, 340, 680, 690]),                     # a clip's end inside a tile of another chunk; rows of no clip
+    (64, 6400, [0, 1000, 3011, 3500, 6400])])                    # clips over several groups of chunks
+@pytest.mark.parametrize("bad", [0, 1, 2])
+def test_a_clip_does_not_spoil_its_neighbours(S, value, channels, rows, bounds, bad):
+    """With one clip's arrays full of NaN or infinities the other clips' results keep every bit."""
+    gen, N, K, clips = torch.Generator().manual_seed(rows + bad), 16, 4, len(bounds) - 1
+    starts, row = starts_of(bounds), torch.arange(rows, device="cuda")
+    hit = (row >= bounds[bad]) & (row < bounds[bad + 1])
+    good_clips = [i for i in range(clips) if i != bad]
+    x, delta, z, dy = (rnd(gen, rows, channels) for _ in range(4))
+    B, C = rnd(gen, rows, N), rnd(gen, rows, N)
+    A, D, w = -rnd(gen, channels, N).abs(), rnd(gen, channels), rnd(gen, channels, K)
+    h0, c0, dh, dc = rnd(gen, clips, channels, N), rnd(gen, clips, K - 1, channels), rnd(gen, clips, channels, N), rnd(gen, clips, K - 1, channels)
+    runs = []
+    for spoil in (False, True):
+        t = [v.clone() for v in (x, delta, B, C, z, dy)]
+        s = [v.clone() for v in (h0, c0, dh, dc)]
+        if spoil:
+            for v in t:
+                v[hit] = value
+            for v in s:
+                v[bad] = value
+        L = [v.requires_grad_() for v in t[:5]] + [s[0].requires_grad_(), s[1].requires_grad_()]
+        y, h = S.selective_scan(L[0], L[1], A, L[2], L[3], D, L[4], clip_start=starts, state=L[5], return_state=True)
+        v, c = S.causal_conv(L[0], w, None, starts, L[6], return_state=True)
+        per_row = list(torch.autograd.grad([y, h], L[:6], [t[5], s[2]], retain_graph=True)) + list(torch.autograd.grad([v, c], [L[0], L[6]], [t[5], s[3]]))
+        runs.append(([y, v, *per_row[:5], per_row[6]], [h, c, per_row[5], per_row[7]]))
+    for a, b in zip(runs[0][0], runs[1][0]):
+        assert torch.equal(a[~hit], b[~hit])
+    for a, b in zip(runs[0][1], runs[1][1]):
+        assert torch.equal(a[good_clips], b[good_clips])
+
+
 def test_no_rows_and_only_empty_clips(S):
     st, cs = torch.randn(3, 4, 16, device="cuda"), torch.randn(3, 2, 4, device="cuda")
     e = lambda n: torch.empty(0, n, device="cuda")
