@@ -813,13 +813,24 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
 // ---- host side -----------------------------------------------------------------------------------------------------------
 static int scan_lpc(int n_state) { return n_state <= 16 ? 4 : n_state <= 32 ? 8 : 16; }
 
-// Rows of a chunk: as many chunks as bring the launch to 1024 workgroups (16 waves per CU; with 512 the passes are 13 % slower at
-// 1024 channels, with 2048 the join grows), none shorter than 64 rows, 128 in the gradient (17920 rows of 256 channels: 205 us
-// with 64, 195 with 128).
+// Rows of a chunk.  The chunks run side by side, so a short array is cut as short as the join of the chunks allows, and a long one
+// into as many as the chip holds at once: 4 workgroups per CU in the forward passes, 2 in the gradient -- one more
+// would wait for a whole round (16 states, bf16; 17920 x 256: 560 workgroups 222 us, 500 of them 185).
+//   forward: 1024 workgroups, chunks of 32 rows or more (1000 x 1024: 29 us, with 16 rows 31), of 16 while that makes no more
+//     than 512 (256 x 256: 19 us, with 32 rows 22, with 64 29); no chunks up to 64 rows, where two launches fewer count (17 against 18).
+//   gradient: 512 workgroups, chunks of 16 rows or more (256 x 256, forward and gradient: 44 us, with 32 rows 48, with 64 65);
+//     1024 where that leaves 256 rows to a chunk, whose ends then level out better (16384 x 1024: 530 us against 542).
 static void scan_chunks(int64_t rows, int channels, int n_state, int backward, int* chunk_rows, int* chunks) {
     const int per = 256 / scan_lpc(n_state);
-    const int64_t groups = (channels + per - 1) / per, target = 1024, least = backward ? 128 : 64;
-    int64_t want = (target + groups - 1) / groups, most = (rows + least - 1) / least;
+    const int64_t groups = (channels + per - 1) / per, by16 = (rows + 15) / 16, by32 = (rows + 31) / 32;
+    int64_t want, most;
+    if (backward) {
+        want = (rows * groups >= 1024 * 256 ? 1024 : 512) / groups;
+        most = by16;
+    } else {
+        want = rows <= 64 ? 1 : 1024 / groups;
+        most = by16 * groups <= 512 ? by16 : by32 * groups > 512 ? by32 : 512 / groups;
+    }
     if (want > most) want = most;
     if (want < 1) want = 1;
     int64_t r = ((rows + want - 1) / want + SCAN_TILE - 1) / SCAN_TILE * SCAN_TILE;
