@@ -293,6 +293,25 @@ def test_a_clip_does_not_spoil_its_neighbours(S, value, channels, rows, bounds, 
         assert torch.equal(a[good_clips], b[good_clips])
 
 
+def test_offsets_outside_the_array_reach_no_row_outside_it(S):
+    """Offsets below 0, above the rows or decreasing give wrong numbers, made of the array's own rows and the given states."""
+    gen, rows, ch, N, K = torch.Generator().manual_seed(4), 70, 8, 16, 4
+    wide = lambda n: torch.full((rows + 64, n), float("nan"), device="cuda")
+    held = [wide(n) for n in (ch, ch, N, N, ch)]
+    t = [v[32:32 + rows] for v in held]
+    for v in t:
+        v.copy_(torch.randn(v.shape, generator=gen))
+    A, w, norm_w = -rnd(gen, ch, N).abs(), rnd(gen, ch, K), rnd(gen, ch)
+    for bounds in ([-5, 30, 75], [-3, -1, rows], [20, 10, 40, 5, 90], [60, 0, 70], [80, 90], [-9, -4]):
+        clips, starts = len(bounds) - 1, starts_of(bounds)
+        h0, c0 = rnd(gen, clips, ch, N), rnd(gen, clips, K - 1, ch)
+        L = [v.detach().requires_grad_() for v in t] + [h0.requires_grad_(), c0.requires_grad_()]
+        y = S.selective_scan(L[0], L[1], A, L[2], L[3], None, L[4], clip_start=starts, state=L[5])
+        v = S.causal_conv(L[0], w, None, starts, L[6])
+        rows_of = [y, v, *torch.autograd.grad(y.sum(), L[:5], retain_graph=True), *torch.autograd.grad(v.sum(), L[:1])]
+        assert all(bool(torch.isfinite(r).all()) for r in rows_of), bounds
+
+
 def test_no_rows_and_only_empty_clips(S):
     st, cs = torch.randn(3, 4, 16, device="cuda"), torch.randn(3, 2, 4, device="cuda")
     e = lambda n: torch.empty(0, n, device="cuda")
