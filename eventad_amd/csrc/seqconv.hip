@@ -54,12 +54,12 @@ template <typename T, int V, int K, bool WAVE> struct ConvLane {
             if (chunk >= a.chunks || col >= a.cols) return false;
         } else {
             const unsigned g = blockIdx.x * 256 + threadIdx.x;
-            chunk = g / a.cols;
-            c = (int)(g - chunk * a.cols) * V;
+            chunk = g / (unsigned)a.cols;
+            c = (int)(g - (unsigned)chunk * a.cols) * V;
             if (chunk >= a.chunks) return false;
         }
         r0 = chunk * a.chunk_rows;
-        r1 = min(a.rows, r0 + a.chunk_rows);
+        r1 = r0 + min(a.chunk_rows, a.rows - r0);                // (the last chunk's end may not fit 32 bits)
         const int skip = conv_skip<K>(a);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -369,10 +369,10 @@ __global__ __launch_bounds__(256, K == 8 ? 1 : 3) void k_conv_bwd(ConvArgs a) {
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
     const unsigned g = blockIdx.x * 256 + threadIdx.x;
-    const int s = g / a.cols, skip = conv_skip<K>(a);
+    const int s = g / (unsigned)a.cols, skip = conv_skip<K>(a);
     if (s >= a.rows) return;
     ConvLane<T, V, K, false> L;
-    const int c = (int)(g - s * a.cols) * V;
+    const int c = (int)(g - (unsigned)s * a.cols) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         L.b[i] = a.bias ? a.bias[c + i] : 0.f;

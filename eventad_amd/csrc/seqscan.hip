@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) float sB[WHAT == 0 ? 3 : 2][SCAN_TILE * N4], sC[WHAT == 0 ? 3 : 1][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y;
-    const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
+    const int c0 = chunk * a.chunk_rows, c1 = c0 + min(a.chunk_rows, a.rows - c0);
     float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
     scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) float sC[2][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y;
-    const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
+    const int c0 = chunk * a.chunk_rows, c1 = c0 + min(a.chunk_rows, a.rows - c0);
     float A2[4], g[4] = {0.f, 0.f, 0.f, 0.f};
     scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) float sB[3][SCAN_TILE * N4], sC[3][SCAN_TILE * N4], red[4][(SCAN_TILE + 1) * W];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int c0 = chunk * a.chunk_rows, c1 = min(a.rows, c0 + a.chunk_rows);
+    const int c0 = chunk * a.chunk_rows, c1 = c0 + min(a.chunk_rows, a.rows - c0);
     float A2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
     scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
@@ -773,12 +773,12 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
-    for (int s0 = blockIdx.y * 4; s0 < a.rows; s0 += gridDim.y * 4) {
-        const int64_t mine = min(s0 + L.q, a.rows - 1);           // the clip whose step and output this lane forms
+    for (int64_t s0 = blockIdx.y * 4; s0 < a.rows; s0 += gridDim.y * 4) {
+        const int64_t mine = min(s0 + L.q, (int64_t)a.rows - 1);           // the clip whose step and output this lane forms
         float h[4][4], b[4][4], c[4][4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int64_t s = min(s0 + q, a.rows - 1);
+            const int64_t s = min(s0 + q, (int64_t)a.rows - 1);
             step_load4<float, VEC>(a.state + (s * a.channels + L.d) * N, L.j, N, h[q]);
             step_load4<T, VEC>((const T*)a.B + s * a.ldb, L.j, N, b[q]);
             step_load4<T, VEC>((const T*)a.C + s * a.ldc, L.j, N, c[q]);
@@ -802,7 +802,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (s0 + q >= a.rows) break;
-            float* dst = a.final_state + ((int64_t)(s0 + q) * a.channels + L.d) * N;
+            float* dst = a.final_state + ((s0 + q) * a.channels + L.d) * N;
             if constexpr (VEC) { if (4 * L.j < N) *(seq_f4*)(dst + 4 * L.j) = seq_f4{h[q][0], h[q][1], h[q][2], h[q][3]}; }
             else scan_store4(dst, L.j, N, h[q]);
         }

@@ -44,7 +44,7 @@ def _call(name, *args):
         f = _functions[name] = getattr(load(), name)
     rc = f(*args)
     if rc:
-        raise NativeError("%s failed with code %d%s" % (name, rc, " (bad argument)" if rc == -1 else " (hipError_t)"))
+        raise NativeError("%s failed with code %d%s" % (name, rc, {-1: " (bad argument)", -3: " (too large for one launch)"}.get(rc, " (hipError_t)")))
 
 
 def _device(t):
@@ -123,7 +123,7 @@ def _clips(clip_start, index):
 def _needs_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 return True
     return False
 

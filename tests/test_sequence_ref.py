@@ -132,3 +132,12 @@ def test_sequence_operators_have_no_cpu_path():
               lambda: S.rms_norm(x, torch.ones(8)), lambda: S.rms_norm_fp8(x, torch.ones(8))):
         with pytest.raises(RuntimeError, match="GPU"):
             f()
+
+
+def test_sequence_operators_take_only_tensors():
+    from eventad_amd import sequence as S
+    x = [[0.0] * 8] * 4
+    for f in (lambda: S.causal_conv(x, x), lambda: S.causal_conv_step(x, x, x), lambda: S.selective_scan(x, x, x, x, x),
+              lambda: S.selective_scan_step(x, x, x, x, x, x), lambda: S.rms_norm(x, x), lambda: S.rms_norm_fp8(x, x), lambda: S.rms_norm(None, None)):
+        with pytest.raises(RuntimeError, match="expected a tensor"):
+            f()
