@@ -819,13 +819,14 @@ static int scan_lpc(int n_state) { return n_state <= 16 ? 4 : n_state <= 32 ? 8 
 //   forward: 1024 workgroups, chunks of 32 rows or more (1000 x 1024: 29 us, with 16 rows 31), of 16 while that makes no more
 //     than 512 (256 x 256: 19 us, with 32 rows 22, with 64 29); no chunks up to 64 rows, where two launches fewer count (17 against 18).
 //   gradient: 512 workgroups, chunks of 16 rows or more (256 x 256, forward and gradient: 44 us, with 32 rows 48, with 64 65);
-//     1024 where that leaves 256 rows to a chunk, whose ends then level out better (16384 x 1024: 530 us against 542).
+//     1024 where that leaves 128 rows to a chunk, whose ends then level out better (12000 x 1024: 398 us against 408; with 64
+//     rows left the second round costs more than that, 17920 x 256: 194 against 185).
 static void scan_chunks(int64_t rows, int channels, int n_state, int backward, int* chunk_rows, int* chunks) {
     const int per = 256 / scan_lpc(n_state);
     const int64_t groups = (channels + per - 1) / per, by16 = (rows + 15) / 16, by32 = (rows + 31) / 32;
     int64_t want, most;
     if (backward) {
-        want = (rows * groups >= 1024 * 256 ? 1024 : 512) / groups;
+        want = (rows * groups >= 1024 * 128 ? 1024 : 512) / groups;
         most = by16;
     } else {
         want = rows <= 64 ? 1 : 1024 / groups;
