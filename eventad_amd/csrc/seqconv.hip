@@ -7,7 +7,8 @@
 // d_t = dy_t act'(pre_t):  dx_t = sum_k w[:,k] d_{t+(K-1)-k} inside the clip,  dw[:,k] = sum_t d_t x_{t-(K-1)+k},
 // dbias = sum_t d_t.
 //
-// All of it is bound by bytes (2K + 4 operations per element that is read and written once).  A thread owns four adjacent
+// All of it is bound by bytes (2K + 4 operations per element that is read and written once): K = 4, 400,000 x 256 f32 819 MB in
+// 153 us (5.4 TB/s), its gradient 1229 MB in 280 us (4.4 TB/s; a copy of 4 GiB runs at 4.75), 17,920 x 1024 f16 73 MB in 19 us.  A thread owns four adjacent
 // channels (one, where rows are not aligned to four) of a chunk of rows and slides down it with the K-1 inputs before the current
 // row in registers, so a row is read once plus (K-1) / chunk for the chunk's start.  Rows go by in groups of four, requested
 // a group ahead; a group that meets a clip's or the chunk's border goes row by row instead, reading again what it needs.
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256, K == 8 ? 1 : 3) void k_conv_bwd(ConvArgs a) {
     }
 }
 
-// one token per clip: reads the K-1 rows of state, writes them shifted (state_out may be the state itself: a thread reads
+// one token per clip (6 x 256: 2.1 us, all of it latency): reads the K-1 rows of state, writes them shifted (state_out may be the state itself: a thread reads
 // all rows of its columns before it writes one)
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
@@ -394,7 +395,8 @@ __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
 }
 
 // ---- column sums (seq.h) -------------------------------------------------------------------------------------------------
-// 64 columns x 4 row lanes per workgroup; gridDim.y workgroups share the rows of a column block.
+// 64 columns x 4 row lanes per workgroup; gridDim.y workgroups share the rows of a column block (8334 rows of 1280 columns, 43 MB:
+// 11 us, and 5 for the 64 parts).
 __global__ __launch_bounds__(256) void k_seq_colsum(const float* __restrict__ in, int64_t rows, int64_t cols, float* __restrict__ out) {
     __shared__ float s[4][64];
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
@@ -469,10 +471,16 @@ static bool conv_vec(const void* p, int64_t ld, int dtype) {
     return (((uintptr_t)p | (uintptr_t)(ld * e)) & (4 * e - 1)) == 0;
 }
 
+// Rows of a chunk.  A long chunk wastes less on the K - 1 rows that it reads beside its own, and in the gradient on its part of dw;
+// a short one gives the chip more threads.  Forward: 2^18 threads, 4 .. 32 rows (6000 x 2048 bf16: 17.4 us, with 2^19 20.0).
+// Gradient, measured with the forward: 2^17 threads, 4 .. 48 rows (6000 x 2048: 50 us, with 2^16 55, with 2^19 88; 400,000 x 256 f32
+// alone 280 us, with 64 rows 301, which leave the third round of workgroups almost empty), of at least 16 rows while 2^16 threads
+// are left (100,000 x 64: 45 us, with 12 rows 49; 2240 x 256: 25 us with 4 rows, with 16 28).
 static int conv_chunk_rows(int64_t rows, int channels, int backward) {
-    // long chunks waste fewer reads at their starts, short ones give the chip more threads
-    const int64_t r = (rows * ((channels + 3) / 4)) >> 19;
-    const int most = backward ? 64 : 32;
+    const int64_t all = rows * ((channels + 3) / 4);
+    int64_t r = backward ? all >> 17 : all >> 18;
+    if (backward && r < 16) r = all >> 16 < 16 ? all >> 16 : 16;
+    const int most = backward ? 48 : 32;
     return r < 4 ? 4 : r > most ? most : (int)r / 4 * 4;
 }
 static bool conv_shape_ok(int64_t rows, int channels, int taps, int dtype) {
