@@ -10,6 +10,8 @@
 //
 // Bound by bytes.  LANES lanes hold a row in registers (ITERS 16-byte pieces each), so every array is read and written once;
 // sums over a row go through DPP / shuffles, over more than a wave through LDS.  Rows too long for registers are read twice.
+// bf16 with residual, 400,000 x 256: 819 MB in 130 us (6.3 TB/s), the gradient 819 MB in 173 us (4.7 TB/s; a copy of 4 GiB runs
+// at 4.75); 8 bits, 16,384 x 2048: 235 MB in 50 us (4.7 TB/s).
 #include "seq.h"
 
 struct NormArgs {
@@ -251,7 +253,8 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
 }
 
 // A workgroup goes over rows blockIdx.x, blockIdx.x + gridDim.x, ... (x PER rows at a time) and keeps its share of dw in
-// registers (LOOP: in its own row of `part`).
+// registers (LOOP: in its own row of `part`).  1024 workgroups, 4 per CU: with the next row requested ahead that is enough
+// loads in flight (188 us without the request, 173 with it), and dw's parts stay at 1024 rows.
 template <typename T, int V, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
     __shared__ float s_red[4];
@@ -368,14 +371,17 @@ template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static i
     if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_bwd<T, V, LANES, ITERS, LOOP>), dim3(groups), block, 0, st, a);
     return evad_last_error();
 }
-// The fewest lanes that hold a row in four pieces each: rows of one wave need no LDS, and short rows share a wave.
+// Short rows share a wave (400,000 x 256 bf16: 148 us, with a wave per row 173), and a row stays in one wave, without LDS, up to two
+// pieces per lane (65,536 x 1024: 101 us, gradient 109; with four waves 103 and 175).  Up to four pieces the gradient, which
+// keeps dw and the next row in registers too, still does better with a wave per row (65,536 x 1280: 153 us against 184), the
+// forward forms with four waves (100,000 x 2048: 276 us against 302).  From there on four waves (16,384 x 4096: 103 us, a wave 117).
 template <int WHAT, typename T, int V> static int norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
     const int pieces = (a.channels + V - 1) / V;
     if (pieces <= 16) return norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
     if (pieces <= 32) return norm_launch3<WHAT, T, V, 32, 1, false>(a, groups, st);
     if (pieces <= 64) return norm_launch3<WHAT, T, V, 64, 1, false>(a, groups, st);
     if (pieces <= 128) return norm_launch3<WHAT, T, V, 64, 2, false>(a, groups, st);
-    if (pieces <= 256) return norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st);
+    if (pieces <= 256) return WHAT == 2 ? norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st) : norm_launch3<WHAT, T, V, 256, 1, false>(a, groups, st);
     if (pieces <= 512) return norm_launch3<WHAT, T, V, 256, 2, false>(a, groups, st);
     if (pieces <= 1024) return norm_launch3<WHAT, T, V, 256, 4, false>(a, groups, st);
     return norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
