@@ -10,8 +10,8 @@
 //   du_t = D dy_t + s_t sum_n g_t B_t        ds_t = u_t sum_n g_t B_t + sum_n A g_t exp(s_t A) h_{t-1}
 //   dA = sum_t s_t g_t exp(s_t A) h_{t-1}    dB_t[n] = sum_d g_t s_t u_t     dC_t[n] = sum_d dy_t h_t
 //
-// Layout: LPC lanes share a channel and hold 4 of its states each in registers (LPC = 4 / 8 / 16 for N <= 16 / 32 / 64), so a
-// wave has 64 / LPC channels and a 256-thread workgroup 256 / LPC.  Rows go by in tiles of 16: the four lanes of a quad form the
+// Layout: LPC lanes share a channel and hold ST of its states each in registers (4 x 1 / 2 / 4 for N <= 4 / 8 / 16, 8 x 4 and 16 x 4
+// for N <= 32 / 64), so a wave has 64 / LPC channels and a 256-thread workgroup 256 / LPC.  Rows go by in tiles of 16: the four lanes of a quad form the
 // step sizes of four different rows (softplus, gate and conversions once per row and channel, not once per lane) and hand
 // them round with DPP; B and C of the tile stand in LDS as floats, read as one 16-byte access per lane and row.
 //
@@ -40,14 +40,14 @@ struct ScanArgs {
     const float *A, *D, *bias, *state;
     float* final_state;
     void* y; int64_t ldy;
-    float* ckpt;                                     // [rows / 8][channels][4 LPC]: the state in front of every 8th row
-    float* carry; float* span; int* flag;            // per chunk: [channels][4 LPC] end state, [channels] sum of s, 1 = stands alone
+    float* ckpt;                                     // [rows / 8][channels][ST LPC]: the state in front of every 8th row
+    float* carry; float* span; int* flag;            // per chunk: [channels][ST LPC] end state, [channels] sum of s, 1 = stands alone
     int rows, channels, n_state, chunk_rows, chunks, softplus;
     // gradient
     const void* dy; int64_t lddy;
     const float* dfinal; float* dstate;
     void *du, *ddelta, *dz; int64_t lddu, lddd, lddz;
-    float* part_bc;                                  // [channel blocks][rows][2][4 LPC]
+    float* part_bc;                                  // [channel blocks][rows][2][ST LPC]
     float* part_p;                                   // [chunks][channels*N (dA) | channels (dD) | channels (dbias)]
 };
 
@@ -98,14 +98,22 @@ template <int LPC> struct ScanLane {
         d = min(d, a.channels - 1);
     }
 };
-// a lane's four entries of a row of N floats
-__device__ __forceinline__ void scan_load4(const float* __restrict__ row, int j, int N, float (&v)[4]) {
+// a lane's ST entries of a row of N floats
+template <int ST> __device__ __forceinline__ void scan_load(const float* __restrict__ row, int j, int N, float (&v)[ST]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = 4 * j + i < N ? row[4 * j + i] : 0.f;
+    for (int i = 0; i < ST; ++i) v[i] = ST * j + i < N ? row[ST * j + i] : 0.f;
 }
-__device__ __forceinline__ void scan_store4(float* __restrict__ row, int j, int N, const float (&v)[4]) {
+template <int ST> __device__ __forceinline__ void scan_store(float* __restrict__ row, int j, int N, const float (&v)[ST]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (4 * j + i < N) row[4 * j + i] = v[i];
+    for (int i = 0; i < ST; ++i) if (ST * j + i < N) row[ST * j + i] = v[i];
+}
+// the same as one access
+template <int ST> using ScanVec = typename SeqVec<float, ST>::type;
+template <int ST> __device__ __forceinline__ ScanVec<ST> scan_vec(const float (&v)[ST]) {
+    ScanVec<ST> r;
+#pragma unroll
+    for (int i = 0; i < ST; ++i) r[i] = v[i];
+    return r;
 }
 
 // The same number, which the compiler takes for a new one: what is read or computed from it is neither moved out of
@@ -134,8 +142,8 @@ template <typename T> struct ScanRows {
 
 // B or C of a tile on their way to LDS as floats: requested a tile ahead, written when the rows in front are done.  A thread
 // takes one state of every (256 / N4)th row; rows of no clip and states >= N become zero.
-template <typename T, int LPC> struct ScanStage {
-    static constexpr int N4 = 4 * LPC, PER = SCAN_TILE * N4 / 256, STEP = 256 / N4;
+template <typename T, int N4> struct ScanStage {
+    static constexpr int ALL = SCAN_TILE * N4, PER = (ALL + 255) / 256, STEP = 256 / N4;
     char* p; unsigned step, at; bool in;
     T v[PER];
     __device__ __forceinline__ ScanStage(const void* base, int64_t ld, int t0, int N)
@@ -146,7 +154,7 @@ template <typename T, int LPC> struct ScanStage {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             v[i] = (T)0.f;
-            if (full || (int)threadIdx.x / N4 + i * STEP < left) v[i] = *(const T*)(p + (scan_again(at) + i * step));
+            if ((full || (int)threadIdx.x / N4 + i * STEP < left) && (ALL >= 256 || (int)threadIdx.x < ALL)) v[i] = *(const T*)(p + (scan_again(at) + i * step));
         }
     }
     __device__ __forceinline__ void store(float* __restrict__ s, int t0, int lo, int hi) const {
@@ -154,23 +162,26 @@ template <typename T, int LPC> struct ScanStage {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int r = t0 + threadIdx.x / N4 + i * STEP;
-            s[threadIdx.x + 256 * i] = in && (clean || (r >= lo && r < hi)) ? (float)v[i] : 0.f;
+            if (ALL >= 256 || (int)threadIdx.x < ALL) s[threadIdx.x + 256 * i] = in && (clean || (r >= lo && r < hi)) ? (float)v[i] : 0.f;
         }
     }
-    template <int DIR> __device__ __forceinline__ void move(bool go) { const unsigned by = go ? (SCAN_TILE / STEP) * step : 0u; p = DIR > 0 ? p + by : p - by; }
+    template <int DIR> __device__ __forceinline__ void move(bool go) {
+        const unsigned by = go ? (STEP > SCAN_TILE ? step / (STEP / SCAN_TILE) : SCAN_TILE / STEP * step) : 0u;
+        p = DIR > 0 ? p + by : p - by;
+    }
 };
 
 // B or C of a pair of rows, read from LDS a pair ahead (and, with a scheduling barrier behind the reads, not more: the
 // registers would cost waves in flight)
-template <int N4> struct ScanPair {
-    const float* p; seq_f4 v[2][2];
+template <int N4, int ST> struct ScanPair {
+    const float* p; ScanVec<ST> v[2][2];
     __device__ __forceinline__ ScanPair(const float* at, int k = 0) : p(at) { read(k); }
     __device__ __forceinline__ void read(int k) {
-        v[k & 1][0] = *(const seq_f4*)(p + 2 * k * N4);
-        v[k & 1][1] = *(const seq_f4*)(p + (2 * k + 1) * N4);
+        v[k & 1][0] = *(const ScanVec<ST>*)(p + 2 * k * N4);
+        v[k & 1][1] = *(const ScanVec<ST>*)(p + (2 * k + 1) * N4);
     }
     __device__ __forceinline__ void ahead(int k) { if (k >= 0 && k < SCAN_TILE / 2) read(k); }
-    __device__ __forceinline__ seq_f4 row(int i) const { return v[(i >> 1) & 1][i & 1]; }
+    __device__ __forceinline__ ScanVec<ST> row(int i) const { return v[(i >> 1) & 1][i & 1]; }
 };
 
 // Rows at .. end-1 of a staged tile, zeros in the place of the others.  A piece that shares its tile with another clip reads this
@@ -192,31 +203,35 @@ __device__ __forceinline__ ScanWalk scan_walk(const SeqClips& c, int row) {
     return w;
 }
 
-// WHAT 0: outputs.  WHAT 1: the chunk's end state for the chunks behind it.
+// WHAT 0: outputs.  WHAT 1: the chunk's end state for the chunks behind it.  Four workgroups per CU; with 16 lanes per channel three,
+// as their staging registers would be spilled at four (16384 x 1024 x 64 bf16: 690 us against 710; with 8 lanes three cost more than the
+// spills, x 24: 322 against 311).
 //
 // A chunk is walked in pieces, the rows that a tile and a clip have in common.  A piece runs through all 16 rows of its
 // tile as straight-line code, with step and input 0 for rows outside it, which leave the state as it is: the usual tile is one
 // piece, a clip's end inside a tile costs one more, and there is no branch between two rows that would keep the reads
 // of B and C from being requested ahead.
-template <typename T, int LPC, int WHAT>
-__global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
-    constexpr int N4 = 4 * LPC;
+template <typename T, int LPC, int ST, int WHAT>
+__global__ __launch_bounds__(256, LPC > 8 ? 3 : 4) void k_scan_fwd(ScanArgs a) {
+    constexpr int N4 = ST * LPC;
     __shared__ __attribute__((aligned(16))) float sB[WHAT == 0 ? 3 : 2][SCAN_TILE * N4], sC[WHAT == 0 ? 3 : 1][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y;
     const int c0 = chunk * a.chunk_rows, c1 = c0 + min(a.chunk_rows, a.rows - c0);
-    float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
-    scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
+    float A2[ST], h[ST];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
+    for (int m = 0; m < ST; ++m) h[m] = 0.f;
+    scan_load(a.A + (size_t)L.d * N, L.j, N, A2);
+#pragma unroll
+    for (int i = 0; i < ST; ++i) A2[i] *= SEQ_LOG2E;
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = WHAT == 0 && a.D ? a.D[L.d] : 0.f;
     auto entry = [&](int s) {                                    // the state in front of clip s
 #pragma unroll
-        for (int m = 0; m < 4; ++m) h[m] = 0.f;
-        if (a.state && s >= 0 && s < n) scan_load4(a.state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
+        for (int m = 0; m < ST; ++m) h[m] = 0.f;
+        if (a.state && s >= 0 && s < n) scan_load(a.state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
     };
     auto leave = [&](int s) {                                    // h is the state behind clip s
-        if (a.final_state && s >= 0 && s < n && L.in) scan_store4(a.final_state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
+        if (a.final_state && s >= 0 && s < n && L.in) scan_store(a.final_state + ((size_t)s * a.channels + L.d) * N, L.j, N, h);
     };
 
     ScanWalk w = scan_walk(a.clips, WHAT == 1 ? c1 - 1 : c0);
@@ -227,7 +242,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
         const bool none = w.s < 0 || w.s >= n || w.next <= c1;
         if (blockIdx.x == 0 && threadIdx.x == 0) a.flag[chunk] = none || first >= c0;
         if (none) {
-            if (L.in) scan_store4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
+            if (L.in) scan_store(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
             return;
         }
         if (first >= c0) { at = first; entry(w.s); }
@@ -235,7 +250,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     } else {
         if (a.final_state)                                       // empty clips at the chunk's first row keep their state
             for (int e = w.s - 1; e >= 0 && seq_start(a.clips, e) == c0; --e) { entry(e); leave(e); }
-        if (w.s >= 0 && w.s < n && first < c0 && chunk > 0) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
+        if (w.s >= 0 && w.s < n && first < c0 && chunk > 0) scan_load(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
         else entry(w.s);
     }
     if (c1 <= c0) return;
@@ -246,7 +261,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     ScanRows<T> fu(a.u, a.ldu, t0, L.q, L.d), fd(a.delta, a.ldd, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d), oy(a.y, a.ldy, t0, L.q, L.d);
     float span = 0.f;
     T ru[4], rd[4], rz[4];
-    ScanStage<T, LPC> stB(a.B, a.ldb, t0, N), stC(a.C, a.ldc, t0, N);
+    ScanStage<T, N4> stB(a.B, a.ldb, t0, N), stC(a.C, a.ldc, t0, N);
     auto fetch = [&](int t) {
         const bool full = t + SCAN_TILE <= a.rows;
         const int left = a.rows - t;
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
             fetch(t2);
         }
         auto keep = [&](int row) {                               // the state in front of the row, for the backward pass
-            if (WHAT == 0 && a.ckpt && L.in) *(seq_f4*)(a.ckpt + ((size_t)(row / SCAN_KEEP) * a.channels + L.d) * N4 + 4 * L.j) = seq_f4{h[0], h[1], h[2], h[3]};
+            if (WHAT == 0 && a.ckpt && L.in) *(ScanVec<ST>*)(a.ckpt + ((size_t)(row / SCAN_KEEP) * a.channels + L.d) * N4 + ST * L.j) = scan_vec(h);
         };
         keep(t0);
         const int t1 = min(t0 + SCAN_TILE, c1);
@@ -294,7 +309,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
                 if constexpr (WHAT == 0) scan_mask<N4>(sC[use], sC[buf], t0, at, end);
                 __syncthreads();
             }
-            const float *tB = sB[use] + scan_again(4 * L.j), *tC = WHAT == 0 ? sC[use] + scan_again(4 * L.j) : tB;
+            const float *tB = sB[use] + scan_again(ST * L.j), *tC = WHAT == 0 ? sC[use] + scan_again(ST * L.j) : tB;
             float s4[4], x4[4], ys[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { s4[k] = st[k]; x4[k] = st[k] * u[k]; }
@@ -306,7 +321,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
                     s4[k] = mine ? s4[k] : 0.f; x4[k] = mine ? x4[k] : 0.f;
                 }
             }
-            ScanPair<N4> gB(tB), gC(WHAT == 0 ? tC : tB);
+            ScanPair<N4, ST> gB(tB), gC(WHAT == 0 ? tC : tB);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float acc[4];
@@ -320,9 +335,9 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     const float sb = quad_bcast(s4[k], q), xb = quad_bcast(x4[k], q);
-                    const seq_f4 b4 = gB.row(4 * k + q), c4 = gC.row(4 * k + q);
+                    const ScanVec<ST> b4 = gB.row(4 * k + q), c4 = gC.row(4 * k + q);
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
+                    for (int m = 0; m < ST; ++m) {
                         h[m] = fmaf(seq_exp2(sb * A2[m]), h[m], xb * b4[m]);
                         if constexpr (WHAT == 0) acc[q] = m ? fmaf(c4[m], h[m], acc[q]) : c4[0] * h[0];
                     }
@@ -359,7 +374,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fwd(ScanArgs a) {
     }
     if constexpr (WHAT == 1) {
         if (L.in) {
-            scan_store4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
+            scan_store(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, h);
             span += seq_dpp<0xB1>(span);
             span += seq_dpp<0x4E>(span);
             if (L.j == 0) a.span[(size_t)chunk * a.channels + L.d] = span;
@@ -376,7 +391,7 @@ template <int REV>
 __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
     __shared__ float s_own[16][16], s_pass[16][16];
     const int col = threadIdx.x & 15, group = threadIdx.x >> 4;
-    const int64_t width = (int64_t)a.channels * n4, at = (int64_t)blockIdx.x * 16 + col;         // (n4 is a multiple of 16)
+    const int64_t width = (int64_t)a.channels * n4, place = (int64_t)blockIdx.x * 16 + col, at = place < width ? place : width - 1;
     const int d = (int)(at / n4), i = (int)(at - (int64_t)d * n4);
     const float A2 = i < a.n_state ? a.A[(size_t)d * a.n_state + i] * SEQ_LOG2E : 0.f;
     const int share = (a.chunks + 15) / 16, first = group * share, last = min(a.chunks, first + share);
@@ -394,7 +409,7 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
                 if (k0 + j >= last) break;
                 const int c = REV ? a.chunks - 1 - (k0 + j) : k0 + j;
                 const float e = fl[j] ? 0.f : seq_exp2(sp[j] * A2);
-                if (turn) a.carry[c * width + at] = in;
+                if (turn && place < width) a.carry[c * width + at] = in;
                 in = fl[j] ? own[j] : fmaf(e, in, own[j]);
                 pass = fl[j] || pass < 0.f ? -1.f : pass * e;
             }
@@ -409,34 +424,37 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
 }
 
 // The adjoint of a chunk by itself: what its rows contribute to dL/dh in front of its first row.  The forward's first pass run
-// backwards, without a gate's or u's part in it: 67 us for 16001 x 1024 x 16 bf16.
-template <typename T, int LPC>
-__global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
-    constexpr int N4 = 4 * LPC;
+// backwards, without a gate's or u's part in it: 67 us for 16001 x 1024 x 16 bf16.  (More than four lanes per channel: three workgroups
+// per CU, without spills, take 10 % less than four; the gradient behind it has two anyway.)
+template <typename T, int LPC, int ST>
+__global__ __launch_bounds__(256, LPC > 4 ? 3 : 4) void k_scan_adj(ScanArgs a) {
+    constexpr int N4 = ST * LPC;
     __shared__ __attribute__((aligned(16))) float sC[2][SCAN_TILE * N4];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y;
     const int c0 = chunk * a.chunk_rows, c1 = c0 + min(a.chunk_rows, a.rows - c0);
-    float A2[4], g[4] = {0.f, 0.f, 0.f, 0.f};
-    scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
+    float A2[ST], g[ST];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
+    for (int m = 0; m < ST; ++m) g[m] = 0.f;
+    scan_load(a.A + (size_t)L.d * N, L.j, N, A2);
+#pragma unroll
+    for (int i = 0; i < ST; ++i) A2[i] *= SEQ_LOG2E;
     const float bias = a.bias ? a.bias[L.d] : 0.f;
     const ScanWalk w = scan_walk(a.clips, c0);
     const bool dead = w.s < 0 || w.s >= n || seq_start(a.clips, w.s) >= c0;        // nothing flows out of the chunk
     const bool ends = w.next <= c1;                                                // the clip ends in it: nothing flows through
     if (blockIdx.x == 0 && threadIdx.x == 0) a.flag[chunk] = dead || ends ? 1 : 0;
     if (dead) {
-        if (L.in) scan_store4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
+        if (L.in) scan_store(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
         return;
     }
     const int to = min(w.next, c1);                                                // rows [c0, to)
-    if (ends && a.dfinal) scan_load4(a.dfinal + ((size_t)w.s * a.channels + L.d) * N, L.j, N, g);
+    if (ends && a.dfinal) scan_load(a.dfinal + ((size_t)w.s * a.channels + L.d) * N, L.j, N, g);
     float span = 0.f;
     int t0 = (to - 1) / SCAN_TILE * SCAN_TILE, buf = 0;
     ScanRows<T> fd(a.delta, a.ldd, t0, L.q, L.d), fy(a.dy, a.lddy, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d);
     T rd[4], ry[4], rz[4];
-    ScanStage<T, LPC> stC(a.C, a.ldc, t0, N);
+    ScanStage<T, N4> stC(a.C, a.ldc, t0, N);
     auto fetch = [&](bool full) {
         const int left = a.rows - t0;
         fd.fetch(rd, full, left - L.q);
@@ -465,7 +483,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
         const bool down = t2 < t0;
         fd.template move<-1>(down); fy.template move<-1>(down); fz.template move<-1>(down); stC.template move<-1>(down);
         fetch(t2 + SCAN_TILE <= a.rows);
-        ScanPair<N4> gC(sC[buf] + 4 * L.j, SCAN_TILE / 2 - 1);
+        ScanPair<N4, ST> gC(sC[buf] + ST * L.j, SCAN_TILE / 2 - 1);
 #pragma unroll
         for (int k = 3; k >= 0; --k) {
             span += st[k];
@@ -476,33 +494,33 @@ __global__ __launch_bounds__(256, 4) void k_scan_adj(ScanArgs a) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const float sb = quad_bcast(st[k], q), db = quad_bcast(dy[k], q);
-                const seq_f4 c4 = gC.row(4 * k + q);
+                const ScanVec<ST> c4 = gC.row(4 * k + q);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) g[m] = seq_exp2(sb * A2[m]) * fmaf(c4[m], db, g[m]);
+                for (int m = 0; m < ST; ++m) g[m] = seq_exp2(sb * A2[m]) * fmaf(c4[m], db, g[m]);
             }
         }
         stC.store(sC[buf ^ 1], t2, c0, to);
         __syncthreads();
     }
     if (L.in) {
-        scan_store4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
+        scan_store(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
         span += seq_dpp<0xB1>(span);
         span += seq_dpp<0x4E>(span);
         if (L.j == 0) a.span[(size_t)chunk * a.channels + L.d] = span;
     }
 }
 
-// 8 values of every lane summed over the channels of the wave.  Two swap-and-add steps fold the halves of the wave and the
-// halves of each half while they halve the number of values (a swap serves two values), then DPP rotations add up the
-// channels inside a row of 16 lanes.  Returns, for row r of 16 lanes, v[0..1] = values 2 (r & 1) + {0, 1} of the first four
-// (r < 2) or of the last four (r >= 2).
-template <int LPC> __device__ __forceinline__ void wave_fold(float (&b)[4], const float (&c)[4]) {
+// 2 ST values of every lane summed over the channels of the wave.  Swap-and-add steps fold the halves of the wave and the halves of
+// each half while they halve the number of values (a swap serves two values), then DPP rotations add up the channels inside a
+// row of 16 lanes.  Row r of 16 lanes returns sums of b (r < 2) or c in b[0 .. FOLD-1], of the states FOLD (r & 1) + 0 .. FOLD-1
+// (ST = 1: of the one state, in both).
+template <int LPC, int ST> __device__ __forceinline__ void wave_fold(float (&b)[ST], const float (&c)[ST]) {
+    constexpr int FOLD = (ST + 1) / 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) seq_swap32(b[i], c[i]);           // lanes 0..31: sums of b, lanes 32..63: sums of c
-    seq_swap16(b[0], b[2]);                                       // even rows of 16: entry 0, odd rows: entry 2
-    seq_swap16(b[1], b[3]);
+    for (int i = 0; i < ST; ++i) seq_swap32(b[i], c[i]);          // lanes 0..31: sums of b, lanes 32..63: sums of c
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < FOLD; ++i) {
+        seq_swap16(b[i], b[ST - FOLD + i]);                       // even rows of 16: entry i, odd rows: entry FOLD + i
         if constexpr (LPC <= 8) b[i] += seq_dpp<0x128>(b[i]);     // row_ror:8
         if constexpr (LPC <= 4) b[i] += seq_dpp<0x124>(b[i]);     // row_ror:4
     }
@@ -523,27 +541,29 @@ __device__ __forceinline__ ScanArgsPtr scan_rare() {
 }
 __device__ __forceinline__ int seq_start(ScanArgsPtr p, int s) { const SeqClips c = {p->clips.start, p->clips.n, p->clips.rows}; return seq_start(c, s); }
 
-template <typename T, int LPC>
+template <typename T, int LPC, int ST>
 __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
-    constexpr int N4 = 4 * LPC, W = 2 * N4;
+    constexpr int N4 = ST * LPC, W = 2 * N4, FOLD = (ST + 1) / 2;
     __shared__ __attribute__((aligned(16))) float sB[3][SCAN_TILE * N4], sC[3][SCAN_TILE * N4], red[4][(SCAN_TILE + 1) * W];
     const ScanLane<LPC> L(a);
     const int N = a.n_state, n = a.clips.n, chunk = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int c0 = chunk * a.chunk_rows, c1 = c0 + min(a.chunk_rows, a.rows - c0);
-    float A2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
-    scan_load4(a.A + (size_t)L.d * N, L.j, N, A2);
+    float A2[ST], g[ST], dA[ST], dD = 0.f, dbias = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
+    for (int m = 0; m < ST; ++m) g[m] = dA[m] = 0.f;
+    scan_load(a.A + (size_t)L.d * N, L.j, N, A2);
+#pragma unroll
+    for (int i = 0; i < ST; ++i) A2[i] *= SEQ_LOG2E;
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
     auto entry = [&](int s) {                                     // the gradient of the state behind clip s
 #pragma unroll
-        for (int m = 0; m < 4; ++m) g[m] = 0.f;
+        for (int m = 0; m < ST; ++m) g[m] = 0.f;
         const ScanArgsPtr r = scan_rare();
-        if (r->dfinal && s >= 0 && s < r->clips.n) scan_load4(r->dfinal + ((size_t)s * r->channels + L.d) * N, L.j, N, g);
+        if (r->dfinal && s >= 0 && s < r->clips.n) scan_load(r->dfinal + ((size_t)s * r->channels + L.d) * N, L.j, N, g);
     };
     auto leave = [&](int s) {                                     // g is the gradient of the state in front of clip s
         const ScanArgsPtr r = scan_rare();
-        if (r->dstate && s >= 0 && s < r->clips.n && L.in) scan_store4(r->dstate + ((size_t)s * r->channels + L.d) * N, L.j, N, g);
+        if (r->dstate && s >= 0 && s < r->clips.n && L.in) scan_store(r->dstate + ((size_t)s * r->channels + L.d) * N, L.j, N, g);
     };
     // s = the clip of row end-1, first = its first row
     int s = __builtin_amdgcn_readfirstlane(seq_find(a.clips, c1 - 1));
@@ -551,19 +571,19 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     if (a.dstate)                                                 // empty clips between this chunk's last row and the next row
         for (int e = s + 1; e < n && seq_start(a.clips, e + 1) <= c1; ++e) { entry(e); leave(e); }
     if (s >= 0 && s < n && seq_start(a.clips, s + 1) > c1) {
-        if (a.chunks > 1) scan_load4(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
+        if (a.chunks > 1) scan_load(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
     } else entry(s);
     const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));            // rows that belong to a clip
-    float* my_red = red[wave] + (lane >> 5) * N4 + 4 * L.j + 2 * ((lane >> 4) & 1);               // (its last row takes what no row wants)
+    float* my_red = red[wave] + (lane >> 5) * N4 + ST * L.j + (ST > 1 ? FOLD * ((lane >> 4) & 1) : 0);               // (its last row takes what no row wants)
     const bool gated = a.z;
     int t0 = (c1 - 1) / SCAN_TILE * SCAN_TILE, buf = 0, end = c1;
     ScanRows<T> fu(a.u, a.ldu, t0, L.q, L.d), fd(a.delta, a.ldd, t0, L.q, L.d), fy(a.dy, a.lddy, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d);
     ScanRows<T> ou(a.du, a.lddu, t0, L.q, L.d), od(a.ddelta, a.lddd, t0, L.q, L.d), oz(a.dz, a.lddz, t0, L.q, L.d);
     T ru[4], rd[4], rz[4], ry[4];
-    seq_f4 kept[2];
-    ScanStage<T, LPC> stB(a.B, a.ldb, t0, N), stC(a.C, a.ldc, t0, N);
+    ScanVec<ST> kept[2];
+    ScanStage<T, N4> stB(a.B, a.ldb, t0, N), stC(a.C, a.ldc, t0, N);
     const char* pk = (const char*)(a.ckpt + (size_t)(t0 / SCAN_KEEP) * a.channels * N4);
-    const unsigned kept_step = (unsigned)a.channels * N4 * 4, kept_at = (unsigned)(L.d * N4 + 4 * L.j) * 4;
+    const unsigned kept_step = (unsigned)a.channels * N4 * 4, kept_at = (unsigned)(L.d * N4 + ST * L.j) * 4;
     auto fetch = [&](bool full) {
         const int left = a.rows - t0;
         fu.fetch(ru, full, left - L.q);
@@ -572,9 +592,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
         if (gated) fz.fetch(rz, full, left - L.q);
         stB.load(full, left);
         stC.load(full, left);
-        kept[0] = *(const seq_f4*)(pk + scan_again(kept_at));
-        kept[1] = seq_f4{0.f, 0.f, 0.f, 0.f};
-        if (full || left > SCAN_KEEP) kept[1] = *(const seq_f4*)(pk + kept_step + scan_again(kept_at));
+        kept[0] = *(const ScanVec<ST>*)(pk + scan_again(kept_at));
+        kept[1] = ScanVec<ST>(0.f);
+        if (full || left > SCAN_KEEP) kept[1] = *(const ScanVec<ST>*)(pk + kept_step + scan_again(kept_at));
     };
     if (c1 > c0) {
         fetch(t0 + SCAN_TILE <= a.rows);
@@ -595,7 +615,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
             if (gated) { const float z = (float)rz[k]; dy[k] *= z * seq_sigmoid(z); }
         }
         const int t2 = max(c0, t0 - SCAN_TILE);
-        const seq_f4 k0 = kept[0], k1 = kept[1];
+        const ScanVec<ST> k0 = kept[0], k1 = kept[1];
         do {                                                      // the tile's pieces: rows at .. end-1
             const int at = max(t0, first);
             const bool whole = at == t0 && end == t0 + SCAN_TILE, live = at >= lo && at < hi;     // (of a clip, or of none)
@@ -622,23 +642,23 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
             for (int half = 1; half >= 0; --half) {
                 const int h0 = t0 + half * SCAN_KEEP;
                 if (at >= h0 + SCAN_KEEP || end <= h0) continue;
-                const float* tB = sB[use] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
-                float h[4], ex[SCAN_KEEP][4], ah[SCAN_KEEP][4];
+                const float* tB = sB[use] + scan_again(ST * L.j + half * SCAN_KEEP * N4);
+                float h[ST], ex[SCAN_KEEP][ST], ah[SCAN_KEEP][ST];
 #pragma unroll
-                for (int m = 0; m < 4; ++m) h[m] = half ? k1[m] : k0[m];
+                for (int m = 0; m < ST; ++m) h[m] = half ? k1[m] : k0[m];
                 if (at == first && at >= h0) {                    // the clip starts here
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) h[m] = 0.f;
+                    for (int m = 0; m < ST; ++m) h[m] = 0.f;
                     const ScanArgsPtr r = scan_rare();
-                    if (r->state && live) scan_load4(r->state + ((size_t)s * r->channels + L.d) * N, L.j, N, h);
+                    if (r->state && live) scan_load(r->state + ((size_t)s * r->channels + L.d) * N, L.j, N, h);
                 }
 #pragma unroll
                 for (int i = 0; i < SCAN_KEEP; ++i) {
                     const int k = 2 * half + i / 4;
                     const float sb = quad_bcast(s4[k], i & 3), xb = quad_bcast(x4[k], i & 3);
-                    const seq_f4 b4 = *(const seq_f4*)(tB + i * N4);
+                    const ScanVec<ST> b4 = *(const ScanVec<ST>*)(tB + i * N4);
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
+                    for (int m = 0; m < ST; ++m) {
                         ex[i][m] = seq_exp2(sb * A2[m]);
                         ah[i][m] = ex[i][m] * h[m];
                         h[m] = fmaf(xb, b4[m], ah[i][m]);
@@ -651,8 +671,8 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                     pk -= down ? 2u * kept_step : 0u;
                     fetch(t2 + SCAN_TILE <= a.rows);
                 }
-                const float* tC = sC[use] + scan_again(4 * L.j + half * SCAN_KEEP * N4);
-                tB = sB[use] + scan_again(4 * L.j + half * SCAN_KEEP * N4);       // (read again rather than kept in 32 registers)
+                const float* tC = sC[use] + scan_again(ST * L.j + half * SCAN_KEEP * N4);
+                tB = sB[use] + scan_again(ST * L.j + half * SCAN_KEEP * N4);       // (read again rather than kept in 32 registers)
 #pragma unroll
                 for (int kk = 1; kk >= 0; --kk) {
                     const int k = 2 * half + kk;
@@ -661,10 +681,10 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                     for (int q = 3; q >= 0; --q) {
                         const int i = 4 * kk + q;
                         const float sb = quad_bcast(s4[k], q), xb = quad_bcast(x4[k], q), db = quad_bcast(d4[k], q);
-                        const seq_f4 b4 = *(const seq_f4*)(tB + i * N4), c4 = *(const seq_f4*)(tC + i * N4);
-                        float vb[4], vc[4];
+                        const ScanVec<ST> b4 = *(const ScanVec<ST>*)(tB + i * N4), c4 = *(const ScanVec<ST>*)(tC + i * N4);
+                        float vb[ST], vc[ST];
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) {
+                        for (int m = 0; m < ST; ++m) {
                             const float ht = fmaf(xb, b4[m], ah[i][m]);
                             ys[q] = m ? fmaf(c4[m], ht, ys[q]) : c4[0] * ht;
                             g[m] = fmaf(c4[m], db, g[m]);
@@ -676,9 +696,10 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
                             dA[m] = fmaf(sb, f, dA[m]);
                             g[m] *= ex[i][m];
                         }
-                        wave_fold<LPC>(vb, vc);                   // (the lanes that hold one sum write it to one place)
+                        wave_fold<LPC, ST>(vb, vc);                   // (the lanes that hold one sum write it to one place)
                         const int p = h0 + i;
-                        *(float2*)(my_red + (p >= at && p < end ? (p - t0) * W : SCAN_TILE * W)) = make_float2(vb[0], vb[1]);
+                        float* to = my_red + (p >= at && p < end ? (p - t0) * W : SCAN_TILE * W);
+                        if constexpr (FOLD == 2) *(float2*)to = make_float2(vb[0], vb[1]); else *to = vb[0];
                     }
                     // the lane's row of these four
                     const float y = quad_rows<LPC>(ys, L.q), gb = quad_rows<LPC>(gbs, L.q), ga = quad_rows<LPC>(gas, L.q);
@@ -735,7 +756,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     if (L.in) {
         const ScanArgsPtr r = scan_rare();
         float* part = r->part_p + (int64_t)chunk * r->channels * (N + 2);
-        scan_store4(part + (size_t)L.d * N, L.j, N, dA);
+        scan_store(part + (size_t)L.d * N, L.j, N, dA);
         if (L.j == 0) { part[(size_t)r->channels * N + L.d] = dD; part[(size_t)r->channels * (N + 1) + L.d] = dbias; }
     }
 }
@@ -815,7 +836,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
             if (s0 + q >= a.rows) break;
             float* dst = a.final_state + ((s0 + q) * a.channels + L.d) * N;
             if constexpr (VEC) { if (4 * L.j < N) *(seq_f4*)(dst + 4 * L.j) = seq_f4{h[q][0], h[q][1], h[q][2], h[q][3]}; }
-            else scan_store4(dst, L.j, N, h[q]);
+            else scan_store<4>(dst, L.j, N, h[q]);
         }
         if (L.j < 4 && s0 + L.q < a.rows) ((T*)a.y)[mine * a.ldy + L.d] = (T)y;
     }
@@ -823,10 +844,11 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
 static int scan_lpc(int n_state) { return n_state <= 16 ? 4 : n_state <= 32 ? 8 : 16; }
+static int scan_width(int n_state) { return n_state <= 4 ? 4 : n_state <= 8 ? 8 : 4 * scan_lpc(n_state); }  // floats of a state as kept here
 
 // Rows of a chunk.  The chunks run side by side, so a short array is cut as short as the join of the chunks allows, and a long one
-// into as many as the chip holds at once: 4 workgroups per CU in the forward passes, 2 in the gradient -- one more
-// would wait for a whole round (16 states, bf16; 17920 x 256: 560 workgroups 222 us, 500 of them 185).
+// into as many as the chip holds at once: 4 workgroups per CU in the forward passes (3 beyond 32 states), 2 in the gradient --
+// one more would wait for a whole round (16 states, bf16; 17920 x 256: 560 workgroups 222 us, 500 of them 185).
 //   forward: 1024 workgroups, chunks of 32 rows or more (1000 x 1024: 29 us, with 16 rows 31), of 16 while that makes no more
 //     than 512 (256 x 256: 19 us, with 32 rows 22, with 64 29); no chunks up to 64 rows, where two launches fewer count (17 against 18).
 //   gradient: 512 workgroups, chunks of 16 rows or more (256 x 256, forward and gradient: 44 us, with 32 rows 48, with 64 65);
@@ -840,7 +862,7 @@ static void scan_chunks(int64_t rows, int channels, int n_state, int backward, i
         want = (rows * groups >= 1024 * 128 ? 1024 : 512) / groups;
         most = by16;
     } else {
-        want = rows <= 64 ? 1 : 1024 / groups;
+        want = rows <= 64 ? 1 : (n_state > 32 ? 768 : 1024) / groups;
         most = by16 * groups <= 512 ? by16 : by32 * groups > 512 ? by32 : 512 / groups;
     }
     if (want > most) want = most;
@@ -861,23 +883,23 @@ static bool scan_ld_ok(int64_t ld, int width) { return ld >= width && ld <= (1 <
 
 static int64_t scan_carry_floats(int chunks, int channels, int n_state) {
     if (chunks <= 1) return 4;
-    const int n4 = 4 * scan_lpc(n_state);
+    const int n4 = scan_width(n_state);
     return (int64_t)chunks * channels * n4 + (((int64_t)chunks * channels + 3) & ~3LL) + ((chunks + 3) & ~3);
 }
 static void scan_carry(ScanArgs& a, float* ws) {
-    const int n4 = 4 * scan_lpc(a.n_state);
+    const int n4 = scan_width(a.n_state);
     a.carry = ws;
     a.span = ws + (int64_t)a.chunks * a.channels * n4;
     a.flag = (int*)(a.span + (((int64_t)a.chunks * a.channels + 3) & ~3LL));
 }
 
-template <int WHAT, typename T, int LPC> static int scan_launch2(const ScanArgs& a, hipStream_t st) {
+template <int WHAT, typename T, int LPC, int ST> static int scan_launch2(const ScanArgs& a, hipStream_t st) {
     constexpr int per = 256 / LPC;
     const dim3 grid((a.channels + per - 1) / per, a.chunks), block(256);
-    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_fwd<T, LPC, 0>), grid, block, 0, st, a);
-    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_fwd<T, LPC, 1>), grid, block, 0, st, a);
-    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_adj<T, LPC>), grid, block, 0, st, a);
-    if constexpr (WHAT == 3) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bwd<T, LPC>), grid, block, 0, st, a);
+    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_fwd<T, LPC, ST, 0>), grid, block, 0, st, a);
+    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_fwd<T, LPC, ST, 1>), grid, block, 0, st, a);
+    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_adj<T, LPC, ST>), grid, block, 0, st, a);
+    if constexpr (WHAT == 3) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bwd<T, LPC, ST>), grid, block, 0, st, a);
     if constexpr (WHAT == 4) {
         const int bytes = 4 * sizeof(T);
         auto quads = [&](const void* p, int64_t ld) { return ((uintptr_t)p | (uintptr_t)(ld * (int64_t)sizeof(T))) % bytes == 0; };
@@ -891,11 +913,17 @@ template <int WHAT, typename T, int LPC> static int scan_launch2(const ScanArgs&
     }
     return evad_last_error();
 }
+// Few states: one or two per lane instead of four of which most are none (16384 x 1024 bf16, forward / with gradient: 4 states 94 / 318 us,
+// 8 states 113 / 381, 16 states 153 / 530, which all took before).
 template <int WHAT, typename T> static int scan_launch1(const ScanArgs& a, hipStream_t st) {
+    if (WHAT != 4) {                                             // (a single token is bound by the states' bytes)
+        if (a.n_state <= 4) return scan_launch2<WHAT, T, 4, WHAT == 4 ? 4 : 1>(a, st);
+        if (a.n_state <= 8) return scan_launch2<WHAT, T, 4, WHAT == 4 ? 4 : 2>(a, st);
+    }
     switch (scan_lpc(a.n_state)) {
-        case 4: return scan_launch2<WHAT, T, 4>(a, st);
-        case 8: return scan_launch2<WHAT, T, 8>(a, st);
-        default: return scan_launch2<WHAT, T, 16>(a, st);
+        case 4: return scan_launch2<WHAT, T, 4, 4>(a, st);
+        case 8: return scan_launch2<WHAT, T, 8, 4>(a, st);
+        default: return scan_launch2<WHAT, T, 16, 4>(a, st);
     }
 }
 template <int WHAT> static int scan_launch(const ScanArgs& a, int dtype, hipStream_t st) {
@@ -904,8 +932,8 @@ template <int WHAT> static int scan_launch(const ScanArgs& a, int dtype, hipStre
     return scan_launch1<WHAT, _Float16>(a, st);
 }
 template <int REV> static void scan_join(const ScanArgs& a, hipStream_t st) {
-    const int n4 = 4 * scan_lpc(a.n_state);
-    hipLaunchKernelGGL(k_scan_join<REV>, dim3((unsigned)(a.channels * (n4 / 16))), dim3(256), 0, st, a, n4);
+    const int n4 = scan_width(a.n_state);
+    hipLaunchKernelGGL(k_scan_join<REV>, dim3((unsigned)(((int64_t)a.channels * n4 + 15) / 16)), dim3(256), 0, st, a, n4);
 }
 
 extern "C" int eventad_selective_scan_workspace(int64_t rows, int channels, int n_state, int backward, int64_t* bytes) {
@@ -914,7 +942,7 @@ extern "C" int eventad_selective_scan_workspace(int64_t rows, int channels, int 
     scan_chunks(rows, channels, n_state, backward, &cr, &chunks);
     int64_t f = scan_carry_floats(chunks, channels, n_state);
     if (backward) {
-        const int per = 256 / scan_lpc(n_state), n4 = 4 * scan_lpc(n_state);
+        const int per = 256 / scan_lpc(n_state), n4 = scan_width(n_state);
         const int64_t groups = (channels + per - 1) / per, cols = (int64_t)channels * (n_state + 2);
         f += groups * rows * 2 * n4 + (chunks + SEQ_SUM_PARTS) * cols;
     }
@@ -924,7 +952,7 @@ extern "C" int eventad_selective_scan_workspace(int64_t rows, int channels, int 
 
 extern "C" int eventad_selective_scan_checkpoint(int64_t rows, int channels, int n_state, int64_t* bytes) {
     if (!bytes || !scan_shape_ok(rows, channels, n_state, 0)) return EVAD_ERR_ARG;
-    *bytes = (rows + SCAN_KEEP - 1) / SCAN_KEEP * channels * 16 * scan_lpc(n_state);
+    *bytes = (rows + SCAN_KEEP - 1) / SCAN_KEEP * channels * 4 * scan_width(n_state);
     return EVAD_OK;
 }
 
@@ -987,7 +1015,7 @@ extern "C" int eventad_selective_scan_bwd(const void* u, int64_t ldu, const void
     scan_chunks(rows, channels, n_state, 1, &a.chunk_rows, &a.chunks);
     float* ws = (float*)workspace;
     scan_carry(a, ws);
-    const int per = 256 / scan_lpc(n_state), n4 = 4 * scan_lpc(n_state), groups = (channels + per - 1) / per;
+    const int per = 256 / scan_lpc(n_state), n4 = scan_width(n_state), groups = (channels + per - 1) / per;
     const int64_t cols = (int64_t)channels * (n_state + 2);
     a.part_bc = ws + scan_carry_floats(a.chunks, channels, n_state);
     a.part_p = a.part_bc + (int64_t)groups * rows * 2 * n4;

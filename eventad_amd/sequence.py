@@ -322,8 +322,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     -> y, or (y, final_state) with return_state: h behind each clip's last row (an empty clip keeps its state).
 
     Every clip's end inside a group of 16 rows costs that group another turn: a batch whose clips are all a row or two long is
-    better served by selective_scan_step.  With a gradient pending, the call keeps 2 x channels x (states, rounded up to 16, 32
-    or 64) bytes per 4 rows."""
+    better served by selective_scan_step.  With a gradient pending, the call keeps 2 x channels x (states, rounded up to a power of
+    two from 4 to 64) bytes per 4 rows."""
     index = _device(u)
     if _elsewhere(index):
         with torch.cuda.device(index):

@@ -197,6 +197,13 @@ def test_selective_scan_and_gradient(S, dtype, rows, channels, N, kind, softplus
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,channels,N,kind", [(100, 5, 2, "tiles"), (333, 67, 4, "three"), (260, 1, 3, "gaps"), (70, 130, 4, "empties"),
+                                                  (333, 65, 8, "three"), (260, 3, 6, "gaps"), (90, 130, 5, "tiles"), (40, 3, 8, "singles"), (40, 9, 4, "singles")])
+def test_selective_scan_with_few_states(S, dtype, rows, channels, N, kind):
+    test_selective_scan_and_gradient(S, dtype, rows, channels, N, kind, True, "Dzbs")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("clips,channels,N", [(1, 1, 1), (6, 256, 16), (5, 13, 5), (3, 33, 24), (2, 7, 64), (17, 20, 8)])
 def test_selective_scan_step(S, dtype, clips, channels, N):
     gen, dt = torch.Generator().manual_seed(clips + N), DTYPES[dtype]
