@@ -21,8 +21,8 @@
 // (without C, gate or output), are joined by a short one, and the second pass starts every chunk from its true state.  The
 // adjoint g is split the same way, from the end.
 //
-// Measured, 16 states: 16384 x 1024 bf16 62 us first pass + 8 join + 94 second pass; the operations above would take 37 for one
-// pass.  500,000 x 64 f32 117 + 20 + 183 us (the second pass 575 MB, 3.1 TB/s).  Gradient of 16001 x 1024 bf16 67 us adjoint +
+// Measured, 16 states: 16384 x 1024 bf16 62 us first pass + 7 join + 94 second pass; the operations above would take 37 for one
+// pass.  500,000 x 64 f32 117 + 13 + 183 us (the second pass 575 MB, 3.1 TB/s).  Gradient of 16001 x 1024 bf16 67 us adjoint +
 // 8 + 281 + 13 for the sums; the operations would take 85.  The passes keep the ALU about 75 % issuing; a layout with a channel's 16
 // states in one lane (no broadcasts, sums over channels across the whole wave) takes the same time, more waves per SIMD spill.
 //
@@ -383,44 +383,61 @@ __global__ __launch_bounds__(256, LPC > 8 ? 3 : 4) void k_scan_fwd(ScanArgs a) {
 }
 
 // The chunks' true entry states.  carry[chunk] holds the chunk's own contribution on entry and what flows into the chunk on
-// return (REV: from the last chunk to the first).  A workgroup takes 16 (channel, state) columns; each of its 16 groups of
-// lanes composes a share of the chunks, picks up what the groups in front of it pass on from LDS, and goes over its share
-// again: two short chains of dependent loads where one thread per column has one of `chunks` (1009 chunks of 64 channels: 20 us
-// against 92).
-template <int REV>
-__global__ __launch_bounds__(256) void k_scan_join(ScanArgs a, int n4) {
-    __shared__ float s_own[16][16], s_pass[16][16];
-    const int col = threadIdx.x & 15, group = threadIdx.x >> 4;
+// return (REV: from the last chunk to the first).  A workgroup takes 16 (channel, state) columns; its G groups of 16 lanes read
+// their share of the chunks at once and compose it, G lanes per column compose the shares, and each group goes over its share
+// again, out of registers: one wait for memory.  64 groups beyond 256 chunks, 16 up to there: 1009 chunks of 64 channels x 16 13 us
+// (16 groups that read twice 23, one thread per column 92), 63 chunks of 1024 channels 7.3 (64 groups 11).
+#define JOIN_SHARE 16                // chunks of a group
+// the state behind a stretch that passes on the factor `pass` (< 0: a clip starts in it) and adds `own`; a state of zero stays zero
+// whatever the factor
+__device__ __forceinline__ float join_past(float pass, float in, float own) { return pass < 0.f || in == 0.f ? own : fmaf(pass, in, own); }
+template <int REV, int G>
+__global__ __launch_bounds__(16 * G) void k_scan_join(ScanArgs a, int n4) {
+    __shared__ float s_own[G][17], s_pass[G][17];
+    const int col = threadIdx.x & 15, group = threadIdx.x >> 4, one = threadIdx.x / G, lane = threadIdx.x % G;
     const int64_t width = (int64_t)a.channels * n4, place = (int64_t)blockIdx.x * 16 + col, at = place < width ? place : width - 1;
     const int d = (int)(at / n4), i = (int)(at - (int64_t)d * n4);
     const float A2 = i < a.n_state ? a.A[(size_t)d * a.n_state + i] * SEQ_LOG2E : 0.f;
-    const int share = (a.chunks + 15) / 16, first = group * share, last = min(a.chunks, first + share);
-    float in = 0.f, pass = 1.f;                                   // pass < 0: a clip starts in the group, nothing gets through
-    for (int turn = 0; turn < 2; ++turn) {                       // 0: compose, 1: hand on
-        for (int k0 = first; k0 < last; k0 += 8) {
-            float own[8], sp[8]; int fl[8];
+    const int share = (a.chunks + G - 1) / G, first = group * share, mine = min(share, a.chunks - first);
+    float own[JOIN_SHARE], e[JOIN_SHARE], in = 0.f, pass = 1.f;
+    int alone[JOIN_SHARE];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = min(k0 + j, last - 1), c = REV ? a.chunks - 1 - k : k;
-                own[j] = a.carry[c * width + at]; sp[j] = a.span[(size_t)c * a.channels + d]; fl[j] = a.flag[c];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (k0 + j >= last) break;
-                const int c = REV ? a.chunks - 1 - (k0 + j) : k0 + j;
-                const float e = fl[j] ? 0.f : seq_exp2(sp[j] * A2);
-                if (turn && place < width) a.carry[c * width + at] = in;
-                in = fl[j] ? own[j] : fmaf(e, in, own[j]);
-                pass = fl[j] || pass < 0.f ? -1.f : pass * e;
-            }
+    for (int j = 0; j < JOIN_SHARE; ++j)
+        if (j < share) {
+            const int k = min(first + j, a.chunks - 1), c = REV ? a.chunks - 1 - k : k;
+            own[j] = a.carry[c * width + at];
+            e[j] = a.span[(size_t)c * a.channels + d];
+            alone[j] = a.flag[c];
         }
-        if (turn == 0) {
-            s_own[group][col] = in; s_pass[group][col] = pass;
-            __syncthreads();
-            in = 0.f;
-            for (int g = 0; g < group; ++g) { const float p = s_pass[g][col]; in = p < 0.f ? s_own[g][col] : fmaf(p, in, s_own[g][col]); }
+#pragma unroll
+    for (int j = 0; j < JOIN_SHARE; ++j)
+        if (j < share && j < mine) {
+            e[j] = alone[j] ? -1.f : seq_exp2(e[j] * A2);
+            in = join_past(e[j], in, own[j]);
+            pass = pass < 0.f || e[j] < 0.f ? -1.f : pass * e[j];
+        }
+    s_own[group][col] = in; s_pass[group][col] = pass;
+    __syncthreads();
+    float o = s_own[lane][one], p = s_pass[lane][one];
+#pragma unroll
+    for (int by = 1; by < G; by <<= 1) {
+        const float o1 = __shfl_up(o, by, G), p1 = __shfl_up(p, by, G);
+        if (lane >= by) {
+            o = join_past(p, o1, o);
+            p = p < 0.f || p1 < 0.f ? -1.f : p * p1;
         }
     }
+    o = __shfl_up(o, 1, G);
+    s_own[lane][one] = lane ? o : 0.f;
+    __syncthreads();
+    in = s_own[group][col];
+#pragma unroll
+    for (int j = 0; j < JOIN_SHARE; ++j)
+        if (j < share && j < mine) {
+            const int c = REV ? a.chunks - 1 - (first + j) : first + j;
+            if (place < width) a.carry[c * width + at] = in;
+            in = join_past(e[j], in, own[j]);
+        }
 }
 
 // The adjoint of a chunk by itself: what its rows contribute to dL/dh in front of its first row.  The forward's first pass run
@@ -932,8 +949,10 @@ template <int WHAT> static int scan_launch(const ScanArgs& a, int dtype, hipStre
     return scan_launch1<WHAT, _Float16>(a, st);
 }
 template <int REV> static void scan_join(const ScanArgs& a, hipStream_t st) {
-    const int n4 = scan_width(a.n_state);
-    hipLaunchKernelGGL(k_scan_join<REV>, dim3((unsigned)(((int64_t)a.channels * n4 + 15) / 16)), dim3(256), 0, st, a, n4);
+    const int n4 = scan_width(a.n_state);                        // (scan_chunks makes at most 1024)
+    const dim3 grid((unsigned)(((int64_t)a.channels * n4 + 15) / 16));
+    if (a.chunks > 16 * JOIN_SHARE) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<REV, 64>), grid, dim3(1024), 0, st, a, n4);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<REV, 16>), grid, dim3(256), 0, st, a, n4);
 }
 
 extern "C" int eventad_selective_scan_workspace(int64_t rows, int channels, int n_state, int backward, int64_t* bytes) {
