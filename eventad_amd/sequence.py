@@ -201,7 +201,7 @@ class _ConvFn(torch.autograd.Function):
             ws = _workspace(_bytes("eventad_causal_conv_workspace", rows, D, K), x)
             _call("eventad_causal_conv_bwd", _p(x), ctx.ldx, _p(w), _p(bias), _p(starts), ctx.clips, _p(state), _p(dy), ldy, _p(dfinal),
                   _p(dx), D, _p(dstate), _p(dp), _p(ws), ws.numel(), rows, D, K, ctx.act, _DTYPE[x.dtype], _stream(x.get_device()))
-        return dx, dp[:D * K].view(D, K), dp[D * K:] if bias is not None else None, dstate, None, None, None, None, None
+        return dx, dp.as_strided((D, K), (K, 1)), dp.as_strided((D,), (1,), D * K) if bias is not None else None, dstate, None, None, None, None, None
 
 
 def causal_conv(x, weight, bias=None, clip_start=None, state=None, activation="silu", return_state=False):
@@ -308,8 +308,8 @@ class _ScanFn(torch.autograd.Function):
             _call("eventad_selective_scan_bwd", _p(u), ldu, _p(delta), ldd, _p(A), _p(B), ldb, _p(C), ldc, _p(D), _p(z), ldz, _p(bias), _p(starts),
                   ctx.clips, _p(state), _p(ckpt), _p(dy), ldy, _p(dfinal), _p(du), ch, _p(dd), ch, _p(dB), N, _p(dC), N, _p(dz), ch,
                   _p(dstate), _p(dp), _p(ws), ws.numel(), rows, ch, N, ctx.softplus, _DTYPE[u.dtype], _stream(u.get_device()))
-        return (du, dd, dp[:ch * N].view(ch, N), dB, dC, dp[ch * N:ch * (N + 1)] if D is not None else None, dz,
-                dp[ch * (N + 1):] if bias is not None else None, dstate, None, None, None, None, None)
+        return (du, dd, dp.as_strided((ch, N), (N, 1)), dB, dC, dp.as_strided((ch,), (1,), ch * N) if D is not None else None, dz,
+                dp.as_strided((ch,), (1,), ch * (N + 1)) if bias is not None else None, dstate, None, None, None, None, None)
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=True, clip_start=None, state=None,
@@ -370,11 +370,12 @@ def _norm_args(x, weight, residual, eps, index):
     rows, D = x.shape
     if D < 1 or weight is None:
         _fail("x must have at least one channel, and weight must be a float32 tensor")
-    if not float(eps) >= 0.0:
+    eps = float(eps)
+    if not eps >= 0.0:
         _fail("eps must not be negative")
     weight = _tensor("weight", weight, (D,), _F32, index)
     residual, ldr = (None, 0) if residual is None else _rows("residual", residual, rows, D, x.dtype, index)
-    return x, ldx, weight, residual, ldr
+    return x, ldx, weight, residual, ldr, eps
 
 
 def _norm_fwd(x, ldx, weight, residual, ldr, eps):
@@ -419,9 +420,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     if _elsewhere(index):
         with torch.cuda.device(index):
             return rms_norm(x, weight, residual, eps)
-    x, ldx, weight, residual, ldr = _norm_args(x, weight, residual, eps, index)
+    x, ldx, weight, residual, ldr, eps = _norm_args(x, weight, residual, eps, index)
     if _needs_grad(x, weight, residual):
-        y, total = _NormFn.apply(x, weight, residual, ldx, ldr, float(eps))
+        y, total = _NormFn.apply(x, weight, residual, ldx, ldr, eps)
     else:
         y, total = _norm_fwd(x, ldx, weight, residual, ldr, eps)
     return y if residual is None else (y, total)
@@ -436,7 +437,7 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     if _elsewhere(index):
         with torch.cuda.device(index):
             return rms_norm_fp8(x, weight, residual, eps)
-    x, ldx, weight, residual, ldr = _norm_args(x, weight, residual, eps, index)
+    x, ldx, weight, residual, ldr, eps = _norm_args(x, weight, residual, eps, index)
     rows, D = x.shape
     q = x.new_empty((rows, D), dtype=torch.float8_e4m3fn)
     scale = x.new_empty(rows, dtype=_F32)

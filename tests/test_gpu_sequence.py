@@ -391,6 +391,16 @@ def test_rms_norm_fp8_is_the_nearest_value(S, dtype, rows, channels, residual):
         assert torch.equal(r[2].double().cpu(), want["sum"][0])
 
 
+def test_rms_norm_takes_any_number_as_eps(S):
+    import numpy as np
+    x, w = rnd(torch.Generator().manual_seed(8), 5, 24), torch.ones(24, device="cuda")
+    want = S.rms_norm(x, w, eps=0.5)
+    for eps in (np.float32(0.5), np.float64(0.5), torch.tensor(0.5)):
+        assert torch.equal(S.rms_norm(x, w, eps=eps), want)
+        assert torch.equal(S.rms_norm_fp8(x, w, eps=eps)[1], S.rms_norm_fp8(x, w, eps=0.5)[1])
+    assert torch.equal(S.rms_norm(x, w, eps=1), S.rms_norm(x, w, eps=1.0))
+
+
 def test_rms_norm_fp8_keeps_nan(S):
     x = torch.randn(4, 64, device="cuda")
     x[1, 3] = float("nan")
