@@ -11,7 +11,7 @@
 // Bound by bytes.  LANES lanes hold a row in registers (ITERS 16-byte pieces each), so every array is read and written once;
 // sums over a row go through DPP / shuffles, over more than a wave through LDS.  Rows too long for registers are read twice.
 // bf16 with residual, 400,000 x 256: 819 MB in 130 us (6.3 TB/s), the gradient 819 MB in 173 us (4.7 TB/s; a copy of 4 GiB runs
-// at 4.75); 8 bits, 16,384 x 2048: 235 MB in 50 us (4.7 TB/s).
+// at 4.75); 8 bits, 16,384 x 2048: 235 MB in 48 us (4.9 TB/s), 100,000 x 2048 1434 MB in 272 (5.3).
 #include "seq.h"
 
 struct NormArgs {
@@ -26,34 +26,50 @@ struct NormArgs {
     float* part;                                     // [workgroups][channels]
 };
 
-// sum over the LANES lanes that share a row
+// Sums over the LANES lanes that share a row.  More than a wave exchanges them in s, which a workgroup may use again after one
+// more barrier (two halves in turn, in a loop).
 template <int LANES> __device__ __forceinline__ float row_sum(float v, float* s) {
     v = seq_lane_sum<LANES < 64 ? LANES : 64>(v);
     if constexpr (LANES > 64) {
-        __syncthreads();
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
         __syncthreads();
         v = (s[0] + s[1]) + (s[2] + s[3]);
     }
     return v;
 }
-// maximum of the bit patterns of non-negative floats / doubles (NaN is above all numbers and stays)
-template <int LANES, typename B> __device__ __forceinline__ B row_max(B v, B* s) {
-#pragma unroll
-    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) v = max(v, (B)__shfl_xor(v, d, 64));
+template <int LANES> __device__ __forceinline__ void row_sums(float& v, float& u, float* s) {
+    v = seq_lane_sum<LANES < 64 ? LANES : 64>(v);
+    u = seq_lane_sum<LANES < 64 ? LANES : 64>(u);
     if constexpr (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; s[4 + (threadIdx.x >> 6)] = u; }
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = max(max(s[0], s[1]), max(s[2], s[3]));
+        v = (s[0] + s[1]) + (s[2] + s[3]);
+        u = (s[4] + s[5]) + (s[6] + s[7]);
     }
-    return v;
+}
+// a sum and the maximum of the bit patterns of non-negative floats (NaN is above all numbers and stays)
+__device__ __forceinline__ unsigned most_of(unsigned a, unsigned b) { return a > b ? a : b; }
+template <int LANES> __device__ __forceinline__ void row_sum_max(float& v, unsigned& u, float* s) {
+    v = seq_lane_sum<LANES < 64 ? LANES : 64>(v);
+    u = most_of(u, seq_dpp_bits<0xB1>(u));
+    u = most_of(u, seq_dpp_bits<0x4E>(u));
+    u = most_of(u, seq_dpp_bits<0x141>(u));
+    u = most_of(u, seq_dpp_bits<0x140>(u));
+    if constexpr (LANES >= 32) { const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false); u = most_of(r[0], r[1]); }
+    if constexpr (LANES >= 64) { const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false); u = most_of(r[0], r[1]); }
+    if constexpr (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; s[4 + (threadIdx.x >> 6)] = __uint_as_float(u); }
+        __syncthreads();
+        v = (s[0] + s[1]) + (s[2] + s[3]);
+        const unsigned* m = (const unsigned*)s + 4;
+        u = most_of(most_of(m[0], m[1]), most_of(m[2], m[3]));
+    }
 }
 
 // LOOP: the row does not fit ITERS pieces per lane and is read again for every pass over it.
 template <typename T, int V, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
-    __shared__ float s_red[4];
+    __shared__ __attribute__((aligned(16))) float s_red[4];
     constexpr int PER = 256 / LANES;
     const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES, D = a.channels;
@@ -112,8 +128,8 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
 // ---- 8 bits ----------------------------------------------------------------------------------------------------------------
 // y / scale = 448 p / max|p| with p = h w needs no r.  A value next to a border of the 8-bit grid has to fall on the side the
 // definition says, so the quotient is formed in float32 (p, its maximum, 448 / maximum and the product: error below 5 units in the
-// last place) and, where it lies within 8 of a border or among the subnormals, again in float64, where p is exact.  One value
-// in 8,000 of ordinary data does.
+// last place) and, where it lies within 8 of a border, again in float64, where p is exact.  One value in 60,000 of ordinary data
+// does.
 
 // v rounded towards the odd neighbour, so that a second rounding to fewer bits is the one rounding of v: e4m3 keeps 4 of the
 // 24 bits of a float
@@ -128,7 +144,8 @@ __device__ __forceinline__ float norm_to_odd(double v) {
 
 template <typename T, int V, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
-    __shared__ unsigned long long s_red[4];
+    __shared__ __attribute__((aligned(16))) float s_red[8];
+    __shared__ unsigned long long s_exact[LANES > 64 ? 4 : 1];
     constexpr int PER = 256 / LANES;
     const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES, D = a.channels;
@@ -169,33 +186,39 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
 #pragma unroll
         for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, p[k]); }
     }
-    ss = row_sum<LANES>(ss, (float*)s_red);
-    const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
     const unsigned own = __float_as_uint(poison == 0.f ? top : __builtin_nanf(""));
-    const unsigned most = row_max<LANES, unsigned>(own, (unsigned*)s_red);
+    unsigned most = own;
+    row_sum_max<LANES>(ss, most, s_red);
+    const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
     float scale = __uint_as_float(most) * inv / 448.f;
     const bool zero = !(scale >= 1.17549435e-38f) && scale == scale;             // a row of zeros (or next to it)
     if (zero) scale = 1.f;
     if (in && lane == 0) a.scale[r] = scale;
     const float by32 = zero ? inv : 448.f / __uint_as_float(most);
-    // p -> q of a piece; true if a value lies too close to a border, or below the smallest normal one and is not 0
+    // p -> q of a piece; true if a value lies too close to a border
     auto divide = [&](const float (&v)[V], float (&q)[V]) {
         unsigned near = 0xffffffffu, low = 0xffffffffu;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             q[i] = v[i] * by32;
             const unsigned u = __float_as_uint(q[i]);
-            near = min(near, (u - 0x7fff8u) & 0xfffffu);         // (borders: the 20 bits that e4m3 has not are 0x80000)
-            low = min(low, (u & 0x7fffffffu) - 1u);
+            near = min(near, (u << 12) - 0x7fff8000u);           // (borders: the 20 bits that e4m3 has not are 0x80000)
+            low = min(low, (u << 1) - 2u);
         }
-        return near <= 16u || low < 0x3c800000u - 1u;            // 2^-6
+        bool close = near <= 0x10000u;
+        if (low < 0x79000000u - 2u) {                            // below 2^-6: steps of 2^-9, borders between them
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                close |= fabsf(q[i]) < 0x1p-6f && fabsf(__builtin_amdgcn_fractf(fabsf(q[i]) * 512.f) - 0.5f) <= 0x1p-18f;
+        }
+        return close;
     };
-    bool close = LOOP;
+    bool close = LOOP, close_in[ITERS];
     if constexpr (!LOOP) {
 #pragma unroll
         for (int k = 0; k < ITERS; ++k) {
-            float q[V];
-            if (divide(p[k], q)) close = true;
+            close_in[k] = divide(p[k], p[k]);                    // (p becomes q)
+            close |= close_in[k];
         }
     }
     // any lane of the row (and of the wave's other rows): then the row's maximum in float64 -- of the entries that share the
@@ -213,13 +236,18 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
                         exact = max(exact, (unsigned long long)__double_as_longlong(fabs((double)v[i] * (double)a.w[c + i])));
             }
         }
-        exact = row_max<LANES, unsigned long long>(exact, s_red);
+#pragma unroll
+        for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1) exact = max(exact, (unsigned long long)__shfl_xor(exact, d, 64));
+        if constexpr (LANES > 64) {
+            if ((threadIdx.x & 63) == 0) s_exact[threadIdx.x >> 6] = exact;
+            __syncthreads();
+            exact = max(max(s_exact[0], s_exact[1]), max(s_exact[2], s_exact[3]));
+        }
         by = most > 0x7f800000u ? (double)__builtin_nanf("") : zero ? (double)inv : 448.0 / __longlong_as_double(exact);
     }
     if (!in) return;
-    auto finish = [&](int c, const float (&v)[V]) {
-        float q[V];
-        if (divide(v, q)) {
+    auto finish = [&](int c, float (&q)[V], bool again) {
+        if (again) {
             float h[V];
             piece(c, h, false);
 #pragma unroll
@@ -244,11 +272,12 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
             piece(c, v, false);
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] *= a.w[c + i];
-            finish(c, v);
+            const bool again = divide(v, v);
+            finish(c, v, again);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, p[k]); }
+        for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) finish(c, p[k], close_in[k]); }
     }
 }
 
@@ -257,7 +286,7 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
 // loads in flight (188 us without the request, 173 with it), and dw's parts stay at 1024 rows.
 template <typename T, int V, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
-    __shared__ float s_red[4];
+    __shared__ __attribute__((aligned(16))) float s_red[2][8];
     __shared__ float s_dw[LANES < 256 ? 256 * V * ITERS : 1];
     constexpr int PER = 256 / LANES;
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, D = a.channels;
@@ -287,6 +316,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
         }
     };
     if (!LOOP && a.rows) request((int64_t)blockIdx.x * PER + sub);
+    int turn = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * PER; r0 < a.rows; r0 += step) {
         const bool in = r0 + sub < a.rows;
         const int64_t r = in ? r0 + sub : a.rows - 1;
@@ -307,8 +337,8 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
 #pragma unroll
             for (int k = 0; k < ITERS; ++k) { const int c = (k * LANES + lane) * V; if (c < D) fold(c, h[k], g[k]); }
         }
-        ss = row_sum<LANES>(ss, s_red);
-        eh = row_sum<LANES>(eh, s_red);
+        row_sums<LANES>(ss, eh, s_red[turn]);
+        turn ^= 1;
         const float inv = 1.f / sqrtf(ss / (float)D + a.eps), m = inv * inv * (eh / (float)D);
         if (!in) continue;
         auto finish = [&](int c, const float (&hv)[V], const float (&gv)[V], const float (&sv)[V], float (&acc)[V]) {

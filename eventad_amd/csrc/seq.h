@@ -61,6 +61,9 @@ __device__ __forceinline__ float seq_sigmoid(float x) { return seq_rcp(1.f + seq
 template <int CTRL> __device__ __forceinline__ float seq_dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
+template <int CTRL> __device__ __forceinline__ unsigned seq_dpp_bits(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
 // x = the sum over both halves of the wave: of x in lanes 0..31, of y in lanes 32..63
 __device__ __forceinline__ void seq_swap32(float& x, float y) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(y), false, false);
