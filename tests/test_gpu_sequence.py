@@ -391,6 +391,23 @@ def test_rms_norm_fp8_is_the_nearest_value(S, dtype, rows, channels, residual):
         assert torch.equal(r[2].double().cpu(), want["sum"][0])
 
 
+@pytest.mark.parametrize("channels", [40, 1030, 2048, 4104, 9000])
+def test_rms_norm_fp8_next_to_every_border(S, channels):
+    """Quotients within a few float32 units of the borders between neighbouring 8-bit values, subnormal ones among them."""
+    gen, rows = torch.Generator().manual_seed(channels), 24
+    grid = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    borders = (grid[1:] + grid[:-1]) / 2
+    w = torch.randn(channels, generator=gen)
+    pick = borders[torch.randint(0, len(borders), (rows, channels), generator=gen)] * (1 + torch.randint(-12, 13, (rows, channels), generator=gen) * 2.0 ** -24)
+    sign = torch.randint(0, 2, (rows, channels), generator=gen) * 2.0 - 1
+    x = torch.rand(rows, channels, generator=gen) + 0.5
+    top = (x[:, :1].double() * w[0].double().abs())              # the row's largest |h w|
+    x[:, 1:] = (pick * sign * top / 448 / w.double()).float()[:, 1:]
+    want = R.norm(x, w.cuda(), None, 1e-6)
+    q, _ = S.rms_norm_fp8(x.cuda(), w.cuda())
+    assert torch.equal(q.double().cpu(), want["q"])
+
+
 def test_rms_norm_takes_any_number_as_eps(S):
     import numpy as np
     x, w = rnd(torch.Generator().manual_seed(8), 5, 24), torch.ones(24, device="cuda")
