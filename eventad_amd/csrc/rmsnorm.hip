@@ -404,7 +404,8 @@ template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static i
 // Short rows share a wave (400,000 x 256 bf16: 148 us, with a wave per row 173), and a row stays in one wave, without LDS, up to two
 // pieces per lane (65,536 x 1024: 101 us, gradient 109; with four waves 103 and 175).  Up to four pieces the gradient, which
 // keeps dw and the next row in registers too, still does better with a wave per row (65,536 x 1280: 153 us against 184), the
-// forward forms with four waves (100,000 x 2048: 276 us against 302).  From there on four waves (16,384 x 4096: 103 us, a wave 117).
+// forward forms with four waves (100,000 x 2048: 276 us against 302).  From there on four waves (16,384 x 4096: 103 us, a wave 117), up to
+// eight pieces per lane (12,000 x 8192 f32: 290 us, gradient 338, read again for every pass over the row 369 and 438).
 template <int WHAT, typename T, int V> static int norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
     const int pieces = (a.channels + V - 1) / V;
     if (pieces <= 16) return norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
@@ -414,6 +415,7 @@ template <int WHAT, typename T, int V> static int norm_launch2(const NormArgs& a
     if (pieces <= 256) return WHAT == 2 ? norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st) : norm_launch3<WHAT, T, V, 256, 1, false>(a, groups, st);
     if (pieces <= 512) return norm_launch3<WHAT, T, V, 256, 2, false>(a, groups, st);
     if (pieces <= 1024) return norm_launch3<WHAT, T, V, 256, 4, false>(a, groups, st);
+    if (pieces <= 2048) return norm_launch3<WHAT, T, V, 256, 8, false>(a, groups, st);
     return norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
 }
 template <int WHAT, typename T> static int norm_launch1(const NormArgs& a, bool vec, int groups, hipStream_t st) {
@@ -451,7 +453,7 @@ extern "C" int eventad_rms_norm_fp8(const void* x, int64_t ldx, const void* resi
     a.rows = rows; a.channels = channels; a.eps = eps;
     const int e = dtype == SEQ_F32 ? 4 : 2;
     const bool vec = seq_aligned(x, ldx * e) && (!residual || (seq_aligned(residual, ldr * e) && seq_aligned(sum, lds * e))) &&
-                     ((((uintptr_t)q | (uintptr_t)ldq) & 7) == 0);
+                     ((((uintptr_t)q | (uintptr_t)ldq) & (16 / e - 1)) == 0);
     return norm_launch<1>(a, dtype, vec, 0, (hipStream_t)stream);
 }
 
