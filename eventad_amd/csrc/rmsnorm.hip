@@ -26,6 +26,49 @@ struct NormArgs {
     float* part;                                     // [workgroups][channels]
 };
 
+// A piece of a row: V elements from column c on.  U: rows start anywhere and end inside a piece; whole pieces are still one access
+// each (global memory takes any address), the last one goes element by element.
+template <typename T, int V> struct NormAny { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
+template <typename T, int V, bool U> __device__ __forceinline__ typename SeqRaw<T, V>::type norm_raw(const T* __restrict__ row, int c, int D) {
+    if constexpr (!U) return seq_raw<T, V>(row + min(c, D - V));
+    else {
+        typename SeqRaw<T, V>::type v = {};
+        if (c + V <= D) {
+            const typename NormAny<T, V>::type w = *(const typename NormAny<T, V>::type*)(row + c);
+            v = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) if (c + i < D) v[i] = row[c + i];
+        }
+        return v;
+    }
+}
+template <typename T, int V, bool U> __device__ __forceinline__ void norm_load(const T* __restrict__ row, int c, int D, float (&out)[V]) {
+    if constexpr (!U) seq_load<T, V>(row + c, out);
+    else seq_unpack<T, V>(norm_raw<T, V, U>(row, c, D), out);
+}
+template <typename T, int V, bool U> __device__ __forceinline__ void norm_store(T* __restrict__ row, int c, int D, const float (&in)[V]) {
+    if constexpr (!U) seq_store<T, V>(row + c, in);
+    else if (c + V <= D) {
+        typename NormAny<T, V>::type v;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (T)in[i];
+        *(typename NormAny<T, V>::type*)(row + c) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (c + i < D) row[c + i] = (T)in[i];
+    }
+}
+template <int V, bool U> __device__ __forceinline__ void norm_weights(const float* __restrict__ w, int c, int D, float (&out)[V]) {
+    if (!U || c + V <= D) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = w[c + i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = c + i < D ? w[c + i] : 0.f;
+    }
+}
+
 // Sums over the LANES lanes that share a row.  More than a wave exchanges them in s, which a workgroup may use again after one
 // more barrier (two halves in turn, in a loop).
 template <int LANES> __device__ __forceinline__ float row_sum(float v, float* s) {
@@ -67,7 +110,7 @@ template <int LANES> __device__ __forceinline__ void row_sum_max(float& v, unsig
 }
 
 // LOOP: the row does not fit ITERS pieces per lane and is read again for every pass over it.
-template <typename T, int V, int LANES, int ITERS, bool LOOP>
+template <typename T, int V, bool U, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
     __shared__ __attribute__((aligned(16))) float s_red[4];
     constexpr int PER = 256 / LANES;
@@ -79,13 +122,13 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
     const T* res = a.res ? (const T*)a.res + r * a.ldr : nullptr;
     float h[ITERS][V];
     auto piece = [&](int c, float (&v)[V], bool store) {         // h of the piece at column c
-        seq_load<T, V>(x + c, v);
+        norm_load<T, V, U>(x, c, D, v);
         if (res) {
             float e[V];
-            seq_load<T, V>(res + c, e);
+            norm_load<T, V, U>(res, c, D, e);
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] = (float)(T)(v[i] + e[i]);
-            if (store) seq_store<T, V>((T*)a.sum + r * a.lds + c, v);
+            if (store) norm_store<T, V, U>((T*)a.sum + r * a.lds, c, D, v);
         }
     };
     float ss = 0.f;
@@ -113,10 +156,11 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
     const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
     if (!in) return;
     auto finish = [&](int c, const float (&v)[V]) {
-        float y[V];
+        float y[V], w[V];
+        norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = v[i] * inv * a.w[c + i];
-        seq_store<T, V>((T*)a.y + r * a.ldy + c, y);
+        for (int i = 0; i < V; ++i) y[i] = v[i] * inv * w[i];
+        norm_store<T, V, U>((T*)a.y + r * a.ldy, c, D, y);
     };
     if constexpr (LOOP) { for (int c = lane * V; c < D; c += LANES * V) { float v[V]; piece(c, v, false); finish(c, v); } }
     else {
@@ -142,7 +186,7 @@ __device__ __forceinline__ float norm_to_odd(double v) {
     return __uint_as_float(u | 1u);
 }
 
-template <typename T, int V, int LANES, int ITERS, bool LOOP>
+template <typename T, int V, bool U, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
     __shared__ __attribute__((aligned(16))) float s_red[8];
     __shared__ unsigned long long s_exact[LANES > 64 ? 4 : 1];
@@ -155,21 +199,23 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
     const T* res = a.res ? (const T*)a.res + r * a.ldr : nullptr;
     float p[ITERS][V];
     auto piece = [&](int c, float (&v)[V], bool store) {         // h of the piece at column c
-        seq_load<T, V>(x + c, v);
+        norm_load<T, V, U>(x, c, D, v);
         if (res) {
             float e[V];
-            seq_load<T, V>(res + c, e);
+            norm_load<T, V, U>(res, c, D, e);
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] = (float)(T)(v[i] + e[i]);
-            if (store) seq_store<T, V>((T*)a.sum + r * a.lds + c, v);
+            if (store) norm_store<T, V, U>((T*)a.sum + r * a.lds, c, D, v);
         }
     };
     float ss = 0.f, top = 0.f, poison = 0.f;
     auto fold = [&](int c, float (&v)[V]) {                      // h -> p
+        float w[V];
+        norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             ss = fmaf(v[i], v[i], ss);
-            v[i] *= a.w[c + i];
+            v[i] *= w[i];
             top = fmaxf(top, fabsf(v[i]));
             poison = fmaf(v[i], 0.f, poison);                    // NaN if anything is not finite
         }
@@ -228,12 +274,13 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
         unsigned long long exact = 0;
         if (own == most && own <= 0x7f800000u) {
             for (int c = lane * V; c < D; c += LANES * V) {
-                float v[V];
+                float v[V], w[V];
                 piece(c, v, false);
+                norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (__float_as_uint(fabsf(v[i] * a.w[c + i])) == most)
-                        exact = max(exact, (unsigned long long)__double_as_longlong(fabs((double)v[i] * (double)a.w[c + i])));
+                    if (__float_as_uint(fabsf(v[i] * w[i])) == most)
+                        exact = max(exact, (unsigned long long)__double_as_longlong(fabs((double)v[i] * (double)w[i])));
             }
         }
 #pragma unroll
@@ -248,30 +295,38 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
     if (!in) return;
     auto finish = [&](int c, float (&q)[V], bool again) {
         if (again) {
-            float h[V];
+            float h[V], w[V];
             piece(c, h, false);
+            norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
-            for (int i = 0; i < V; ++i) q[i] = norm_to_odd((double)h[i] * (double)a.w[c + i] * by);
+            for (int i = 0; i < V; ++i) q[i] = norm_to_odd((double)h[i] * (double)w[i] * by);
         }
         uint8_t* out = a.q + r * a.ldq + c;
         if constexpr (V == 1) *out = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[0], 0, false);
         else {
             typedef unsigned word __attribute__((ext_vector_type(V / 4)));
+            typedef unsigned any __attribute__((ext_vector_type(V / 4), aligned(1)));
             word o;
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) {
                 int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
                 o[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], w, true);
             }
-            *(word*)out = o;
+            if constexpr (!U) *(word*)out = o;
+            else if (c + V <= D) *(any*)out = o;
+            else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) if (c + i < D) out[i] = (uint8_t)(o[i / 4] >> (8 * (i & 3)));
+            }
         }
     };
     if constexpr (LOOP) {
         for (int c = lane * V; c < D; c += LANES * V) {
-            float v[V];
+            float v[V], w[V];
             piece(c, v, false);
+            norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] *= a.w[c + i];
+            for (int i = 0; i < V; ++i) v[i] *= w[i];
             const bool again = divide(v, v);
             finish(c, v, again);
         }
@@ -284,7 +339,7 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
 // A workgroup goes over rows blockIdx.x, blockIdx.x + gridDim.x, ... (x PER rows at a time) and keeps its share of dw in
 // registers (LOOP: in its own row of `part`).  1024 workgroups, 4 per CU: with the next row requested ahead that is enough
 // loads in flight (188 us without the request, 173 with it), and dw's parts stay at 1024 rows.
-template <typename T, int V, int LANES, int ITERS, bool LOOP>
+template <typename T, int V, bool U, int LANES, int ITERS, bool LOOP>
 __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
     __shared__ __attribute__((aligned(16))) float s_red[2][8];
     __shared__ float s_dw[LANES < 256 ? 256 * V * ITERS : 1];
@@ -299,7 +354,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
     if constexpr (LOOP) {
         for (int c = lane * V; c < D; c += LANES * V)
 #pragma unroll
-            for (int i = 0; i < V; ++i) part[c + i] = 0.f;
+            for (int i = 0; i < V; ++i) if (!U || c + i < D) part[c + i] = 0.f;
     }
     const int64_t step = (int64_t)gridDim.x * PER;
     // (a row's arrays are requested while the row in front is worked on; without that the sums over a row leave memory idle)
@@ -311,8 +366,8 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
         const T* sr = a.dsum ? (const T*)a.dsum + r * a.ldds : hr;
 #pragma unroll
         for (int k = 0; k < ITERS; ++k) {
-            const int c = min((k * LANES + lane) * V, D - V);     // (D is a multiple of V)
-            rh[k] = seq_raw<T, V>(hr + c); rg[k] = seq_raw<T, V>(gr + c); rs[k] = seq_raw<T, V>(sr + c);
+            const int c = (k * LANES + lane) * V;
+            rh[k] = norm_raw<T, V, U>(hr, c, D); rg[k] = norm_raw<T, V, U>(gr, c, D); rs[k] = norm_raw<T, V, U>(sr, c, D);
         }
     };
     if (!LOOP && a.rows) request((int64_t)blockIdx.x * PER + sub);
@@ -322,14 +377,16 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
         const int64_t r = in ? r0 + sub : a.rows - 1;
         float h[ITERS][V], g[ITERS][V], ds[ITERS][V], ss = 0.f, eh = 0.f;
         auto fold = [&](int c, const float (&hv)[V], const float (&gv)[V]) {
+            float w[V];
+            norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
-            for (int i = 0; i < V; ++i) { ss = fmaf(hv[i], hv[i], ss); eh = fmaf(gv[i] * a.w[c + i], hv[i], eh); }
+            for (int i = 0; i < V; ++i) { ss = fmaf(hv[i], hv[i], ss); eh = fmaf(gv[i] * w[i], hv[i], eh); }
         };
         const T* hr = (const T*)a.sum + r * a.lds;
         const T* gr = (const T*)a.dy + r * a.lddy;
         const T* sr = a.dsum ? (const T*)a.dsum + r * a.ldds : nullptr;
         if constexpr (LOOP) {
-            for (int c = lane * V; c < D; c += LANES * V) { float hv[V], gv[V]; seq_load<T, V>(hr + c, hv); seq_load<T, V>(gr + c, gv); fold(c, hv, gv); }
+            for (int c = lane * V; c < D; c += LANES * V) { float hv[V], gv[V]; norm_load<T, V, U>(hr, c, D, hv); norm_load<T, V, U>(gr, c, D, gv); fold(c, hv, gv); }
         } else {
 #pragma unroll
             for (int k = 0; k < ITERS; ++k) { seq_unpack<T, V>(rh[k], h[k]); seq_unpack<T, V>(rg[k], g[k]); seq_unpack<T, V>(rs[k], ds[k]); }
@@ -342,24 +399,25 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
         const float inv = 1.f / sqrtf(ss / (float)D + a.eps), m = inv * inv * (eh / (float)D);
         if (!in) continue;
         auto finish = [&](int c, const float (&hv)[V], const float (&gv)[V], const float (&sv)[V], float (&acc)[V]) {
-            float dh[V];
+            float dh[V], w[V];
+            norm_weights<V, U>(a.w, c, D, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                dh[i] = fmaf(inv, fmaf(-hv[i], m, gv[i] * a.w[c + i]), sr ? sv[i] : 0.f);
+                dh[i] = fmaf(inv, fmaf(-hv[i], m, gv[i] * w[i]), sr ? sv[i] : 0.f);
                 acc[i] = fmaf(gv[i] * inv, hv[i], acc[i]);
             }
-            seq_store<T, V>((T*)a.dh + r * a.lddh + c, dh);
+            norm_store<T, V, U>((T*)a.dh + r * a.lddh, c, D, dh);
         };
         if constexpr (LOOP) {
             for (int c = lane * V; c < D; c += LANES * V) {
                 float hv[V], gv[V], sv[V], acc[V];
-                seq_load<T, V>(hr + c, hv); seq_load<T, V>(gr + c, gv);
-                if (sr) seq_load<T, V>(sr + c, sv);
+                norm_load<T, V, U>(hr, c, D, hv); norm_load<T, V, U>(gr, c, D, gv);
+                if (sr) norm_load<T, V, U>(sr, c, D, sv);
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = part[c + i];
+                for (int i = 0; i < V; ++i) acc[i] = !U || c + i < D ? part[c + i] : 0.f;
                 finish(c, hv, gv, sv, acc);
 #pragma unroll
-                for (int i = 0; i < V; ++i) part[c + i] = acc[i];
+                for (int i = 0; i < V; ++i) if (!U || c + i < D) part[c + i] = acc[i];
             }
         } else {
 #pragma unroll
@@ -372,7 +430,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
             const int c = (k * LANES + lane) * V;
             if (c < D)
 #pragma unroll
-                for (int i = 0; i < V; ++i) part[c + i] = dw[k][i];
+                for (int i = 0; i < V; ++i) if (!U || c + i < D) part[c + i] = dw[k][i];
         }
     } else if constexpr (!LOOP) {                                  // the workgroup's PER row groups, added in order
 #pragma unroll
@@ -391,14 +449,14 @@ __global__ __launch_bounds__(256) void k_norm_bwd(NormArgs a) {
 
 static int norm_groups(int64_t rows) { return (int)(rows < 1 ? 1 : rows < 1024 ? rows : 1024); }
 
-template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static int norm_launch3(const NormArgs& a, int groups, hipStream_t st) {
+template <int WHAT, typename T, int V, bool U, int LANES, int ITERS, bool LOOP> static int norm_launch3(const NormArgs& a, int groups, hipStream_t st) {
     constexpr int PER = 256 / LANES;
     const long long blocks = (a.rows + PER - 1) / PER;
     if (WHAT != 2 && blocks * 256 > SEQ_MOST_THREADS) return EVENTAD_ERR_TOO_LARGE;
     const dim3 grid((unsigned)blocks), block(256);
-    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, LANES, ITERS, LOOP>), grid, block, 0, st, a);
-    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fp8<T, V, LANES, ITERS, LOOP>), grid, block, 0, st, a);
-    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_bwd<T, V, LANES, ITERS, LOOP>), dim3(groups), block, 0, st, a);
+    if constexpr (WHAT == 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fwd<T, V, U, LANES, ITERS, LOOP>), grid, block, 0, st, a);
+    if constexpr (WHAT == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_fp8<T, V, U, LANES, ITERS, LOOP>), grid, block, 0, st, a);
+    if constexpr (WHAT == 2) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_bwd<T, V, U, LANES, ITERS, LOOP>), dim3(groups), block, 0, st, a);
     return evad_last_error();
 }
 // Short rows share a wave (400,000 x 256 bf16: 148 us, with a wave per row 173), and a row stays in one wave, without LDS, up to two
@@ -406,21 +464,28 @@ template <int WHAT, typename T, int V, int LANES, int ITERS, bool LOOP> static i
 // keeps dw and the next row in registers too, still does better with a wave per row (65,536 x 1280: 153 us against 184), the
 // forward forms with four waves (100,000 x 2048: 276 us against 302).  From there on four waves (16,384 x 4096: 103 us, a wave 117), up to
 // eight pieces per lane (12,000 x 8192 f32: 290 us, gradient 338, read again for every pass over the row 369 and 438).
-template <int WHAT, typename T, int V> static int norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
+template <int WHAT, typename T, int V, bool U> static int norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
     const int pieces = (a.channels + V - 1) / V;
-    if (pieces <= 16) return norm_launch3<WHAT, T, V, 16, 1, false>(a, groups, st);
-    if (pieces <= 32) return norm_launch3<WHAT, T, V, 32, 1, false>(a, groups, st);
-    if (pieces <= 64) return norm_launch3<WHAT, T, V, 64, 1, false>(a, groups, st);
-    if (pieces <= 128) return norm_launch3<WHAT, T, V, 64, 2, false>(a, groups, st);
-    if (pieces <= 256) return WHAT == 2 ? norm_launch3<WHAT, T, V, 64, 4, false>(a, groups, st) : norm_launch3<WHAT, T, V, 256, 1, false>(a, groups, st);
-    if (pieces <= 512) return norm_launch3<WHAT, T, V, 256, 2, false>(a, groups, st);
-    if (pieces <= 1024) return norm_launch3<WHAT, T, V, 256, 4, false>(a, groups, st);
-    if (pieces <= 2048) return norm_launch3<WHAT, T, V, 256, 8, false>(a, groups, st);
-    return norm_launch3<WHAT, T, V, 256, 1, true>(a, groups, st);
+    if (pieces <= 16) return norm_launch3<WHAT, T, V, U, 16, 1, false>(a, groups, st);
+    if (pieces <= 32) return norm_launch3<WHAT, T, V, U, 32, 1, false>(a, groups, st);
+    if (pieces <= 64) return norm_launch3<WHAT, T, V, U, 64, 1, false>(a, groups, st);
+    if (pieces <= 128) return norm_launch3<WHAT, T, V, U, 64, 2, false>(a, groups, st);
+    if (pieces <= 256) return WHAT == 2 ? norm_launch3<WHAT, T, V, U, 64, 4, false>(a, groups, st) : norm_launch3<WHAT, T, V, U, 256, 1, false>(a, groups, st);
+    if (pieces <= 512) return norm_launch3<WHAT, T, V, U, 256, 2, false>(a, groups, st);
+    if (pieces <= 1024) return norm_launch3<WHAT, T, V, U, 256, 4, false>(a, groups, st);
+    if (pieces <= 2048) return norm_launch3<WHAT, T, V, U, 256, 8, false>(a, groups, st);
+    return norm_launch3<WHAT, T, V, U, 256, 1, true>(a, groups, st);
 }
+// Rows that are not whole aligned pieces: pieces all the same (12,000 x 8191 bf16: forward 196 us, with gradient 633, 8 bits 203; element
+// by element 383, 1010 and 536), but few channels one to a lane, as most of the lanes would have none and one a tail
+// (200,000 x 30 bf16: 25 and 59 us against 36 and 112; x 100 38 and 82 against 25 and 65).
 template <int WHAT, typename T> static int norm_launch1(const NormArgs& a, bool vec, int groups, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
-    return vec && a.channels % N == 0 ? norm_launch2<WHAT, T, N>(a, groups, st) : norm_launch2<WHAT, T, 1>(a, groups, st);
+    if (vec && a.channels % N == 0) return norm_launch2<WHAT, T, N, false>(a, groups, st);
+    if (a.channels >= 64) return norm_launch2<WHAT, T, N, true>(a, groups, st);
+    if (a.channels <= 16) return norm_launch3<WHAT, T, 1, false, 16, 1, false>(a, groups, st);
+    if (a.channels <= 32) return norm_launch3<WHAT, T, 1, false, 32, 1, false>(a, groups, st);
+    return norm_launch3<WHAT, T, 1, false, 64, 1, false>(a, groups, st);
 }
 template <int WHAT> static int norm_launch(const NormArgs& a, int dtype, bool vec, int groups, hipStream_t st) {
     if (dtype == SEQ_F32) return norm_launch1<WHAT, float>(a, vec, groups, st);
