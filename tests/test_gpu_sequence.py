@@ -408,6 +408,42 @@ def test_rms_norm_fp8_next_to_every_border(S, channels):
     assert torch.equal(q.double().cpu(), want["q"])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("channels", [5, 67, 257, 1027, 4611, 9001, 16390])
+def test_rms_norm_rows_of_any_start_and_length(S, dtype, channels):
+    """Rows inside wider arrays that start at any element: results as those of packed rows, and nothing written beside them."""
+    gen, dt, rows, pad = torch.Generator().manual_seed(channels), DTYPES[dtype], 5, 3
+    code, wide = {"f32": 0, "bf16": 1, "f16": 2}[dtype], channels + pad
+    inner = lambda: torch.full((rows, wide), 7.0, device="cuda", dtype=dt)
+    x, res, dy, ds = (inner() for _ in range(4))
+    for t in (x, res, dy, ds):
+        t[:, 1:1 + channels] = rnd(gen, rows, channels, dtype=dt)
+    w = rnd(gen, channels)
+    total, y, dh = inner(), inner(), inner()
+    q = torch.full((rows, wide), 9, device="cuda", dtype=torch.uint8)
+    scale, dw = torch.empty(rows, device="cuda"), torch.empty(channels, device="cuda")
+    at = lambda t: t.data_ptr() + t.element_size()
+    stream = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(S._bytes("eventad_rms_norm_workspace", rows, channels), device="cuda", dtype=torch.uint8)
+    S._call("eventad_rms_norm_fwd", at(x), wide, at(res), wide, w.data_ptr(), at(total), wide, at(y), wide, rows, channels, 1e-6, code, stream)
+    S._call("eventad_rms_norm_bwd", at(total), wide, w.data_ptr(), at(dy), wide, at(ds), wide, at(dh), wide, dw.data_ptr(), ws.data_ptr(), ws.numel(),
+            rows, channels, 1e-6, code, stream)
+    kept = total.clone()
+    S._call("eventad_rms_norm_fp8", at(x), wide, at(res), wide, w.data_ptr(), at(total), wide, at(q), wide, scale.data_ptr(), rows, channels, 1e-6, code, stream)
+    assert torch.equal(total, kept)
+    mine = lambda t: t[:, 1:1 + channels]
+    for t, fill in ((total, 7), (y, 7), (dh, 7), (q, 9)):
+        assert bool((t[:, 0] == fill).all()) and bool((t[:, 1 + channels:] == fill).all())
+    want = R.norm(mine(x).cpu(), w, mine(res).cpu(), 1e-6, mine(dy).cpu(), mine(ds).cpu())
+    assert torch.equal(mine(total).double().cpu(), want["sum"][0])
+    assert torch.equal(mine(q).contiguous().view(torch.float8_e4m3fn).double().cpu(), want["q"])
+    units = 2 * (channels / 16 + 24)
+    close("y", mine(y), want["y"][0], units * want["y"][1])
+    close("scale", scale, want["scale"][0], units * want["scale"][0])
+    close("dh", mine(dh), want["h"][0], units * want["h"][1])
+    close("dw", dw, want["weight"][0], (units + rows) * want["weight"][1])
+
+
 def test_rms_norm_takes_any_number_as_eps(S):
     import numpy as np
     x, w = rnd(torch.Generator().manual_seed(8), 5, 24), torch.ones(24, device="cuda")
