@@ -14,8 +14,8 @@
 // a group ahead; a group that meets a clip's or the chunk's border goes row by row instead, reading again what it needs.
 // Four channels and not the eight that 16 bytes of a 16-bit type hold: weights and windows of eight are 128 registers, and the
 // waves that fit beside them do not cover the memory's latency.
-// WAVE: with 64 columns or more a wave has one chunk, and the walk over the clips is scalar; narrower arrays put several chunks
-// into a wave.
+// WAVE: with 64 columns or more a wave has one chunk, and the walk over the clips is scalar (17,920 x 1024 bf16 forward 22 us, without
+// it 24; 400,000 x 256 with gradient 250 and 264); narrower arrays put several chunks into a wave.
 #include "seq.h"
 
 #define CONV_MAX_TAPS 8
@@ -37,7 +37,7 @@ struct ConvArgs {
 };
 
 // The kernels are built for K = 2, 3, 4 and 8 taps; K = 8 serves every other number: its first K - taps window entries are zero
-// and stay out of the sums.
+// and stay out of the sums.  (Four taps, 17,920 x 1024 bf16: 21 us and 61 with the gradient; by the kernels for eight 31 and 118.)
 template <int K> __device__ __forceinline__ int conv_skip(const ConvArgs& a) { return K == 8 ? K - a.taps : 0; }
 
 template <bool WAVE> __device__ __forceinline__ int conv_same(int v) { return WAVE ? __builtin_amdgcn_readfirstlane(v) : v; }
@@ -418,6 +418,7 @@ __global__ __launch_bounds__(256) void k_seq_colsum(const float* __restrict__ in
 
 int seq_colsum(const float* in, int64_t rows, int64_t cols, float* out, float* scratch, hipStream_t st) {
     // one launch while a workgroup has at most 64 rows to add; beyond that the rows are shared out so that ~2048 workgroups run
+    // (gradients with such sums behind them, bf16: norm of 4096 x 256 18 us, in one launch 36; convolution of 100,000 x 64 45, 161)
     const int64_t blocks = (cols + 63) / 64;
     int64_t parts = rows <= 64 ? 1 : (rows + 31) / 32;
     const int64_t fill = (2048 + blocks - 1) / blocks;
@@ -455,6 +456,8 @@ template <int WHAT, typename T, int V> static int conv_launch2(const ConvArgs& a
         default: return conv_launch3<WHAT, T, V, 8>(a, st);
     }
 }
+// Four channels to a thread where rows are whole aligned groups of four (17,920 x 1024 bf16 forward 21 us, with gradient 62), otherwise
+// one (x 1023: 27 and 74; groups with a last one of three, element by element, 35 and 125).
 template <int WHAT, typename T> static int conv_launch1(ConvArgs& a, bool vec, hipStream_t st) {
     const bool four = vec && a.channels % 4 == 0;
     a.cols = four ? a.channels / 4 : a.channels;

@@ -139,6 +139,44 @@ def test_causal_conv_over_long_chunks(S, dtype, rows, channels, taps):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("channels", [1, 6, 67, 259, 1023])
+@pytest.mark.parametrize("taps", [4, 7])
+def test_causal_conv_rows_of_any_start_and_length(S, dtype, channels, taps):
+    """Rows inside wider arrays that start at any element: results as those of packed rows, and nothing written beside them."""
+    gen, dt, rows, wide = torch.Generator().manual_seed(channels + taps), DTYPES[dtype], 77, channels + 3
+    code, bounds = {"f32": 0, "bf16": 1, "f16": 2}[dtype], [2, 31, 31, 32, 75]
+    starts, clips = starts_of(bounds), len(bounds) - 1
+    inner = lambda: torch.full((rows, wide), 7.0, device="cuda", dtype=dt)
+    x, dy, y, dx = (inner() for _ in range(4))
+    mine, at = (lambda t: t[:, 1:1 + channels]), (lambda t: t.data_ptr() + t.element_size())
+    for t in (x, dy):
+        mine(t).copy_(rnd(gen, rows, channels, dtype=dt))
+    w, b = rnd(gen, channels, taps), rnd(gen, channels)
+    st, df = rnd(gen, clips, taps - 1, channels, dtype=dt), rnd(gen, clips, taps - 1, channels, dtype=dt)
+    guard = lambda: torch.full((clips * (taps - 1) * channels + 8,), 7.0, device="cuda", dtype=dt)
+    final, dst = guard(), guard()
+    dp = torch.empty(channels * (taps + 1), device="cuda")
+    ws = torch.empty(S._bytes("eventad_causal_conv_workspace", rows, channels, taps), device="cuda", dtype=torch.uint8)
+    stream = torch.cuda.current_stream().cuda_stream
+    S._call("eventad_causal_conv_fwd", at(x), wide, w.data_ptr(), b.data_ptr(), starts.data_ptr(), clips, st.data_ptr(), final.data_ptr(), at(y), wide,
+            rows, channels, taps, 1, code, stream)
+    S._call("eventad_causal_conv_bwd", at(x), wide, w.data_ptr(), b.data_ptr(), starts.data_ptr(), clips, st.data_ptr(), at(dy), wide, df.data_ptr(),
+            at(dx), wide, dst.data_ptr(), dp.data_ptr(), ws.data_ptr(), ws.numel(), rows, channels, taps, 1, code, stream)
+    for t in (y, dx):
+        assert bool((t[:, 0] == 7).all()) and bool((t[:, 1 + channels:] == 7).all())
+    for t in (final, dst):
+        assert bool((t[-8:] == 7).all())
+    want = R.conv(mine(x).cpu(), w, b, bounds, st, True, mine(dy).cpu(), df)
+    row_units, sum_units = conv_units(taps, rows)
+    close("y", mine(y), want["y"][0], row_units * want["y"][1])
+    close("final", final[:-8].view(clips, taps - 1, channels), want["final"][0], 0)
+    close("dx", mine(dx), want["x"][0], row_units * want["x"][1])
+    close("dstate", dst[:-8].view(clips, taps - 1, channels), want["state"][0], row_units * want["state"][1])
+    close("dweight", dp[:channels * taps].view(channels, taps), want["weight"][0], sum_units * want["weight"][1])
+    close("dbias", dp[channels * taps:], want["bias"][0], sum_units * want["bias"][1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("clips,channels,taps", [(1, 1, 1), (1, 8, 4), (6, 256, 4), (5, 13, 3), (33, 40, 8), (3, 16, 2)])
 def test_causal_conv_step(S, dtype, clips, channels, taps):
     gen, dt = torch.Generator().manual_seed(clips), DTYPES[dtype]
