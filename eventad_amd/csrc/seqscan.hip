@@ -798,9 +798,9 @@ __global__ __launch_bounds__(256) void k_scan_bc(const float* __restrict__ part,
 // One token per clip, bound by the bytes of the states: 4 N in and 4 N out per channel (2048 x 1024 x 16: 285 MB in 50 us,
 // 5.7 TB/s; 6 x 256 x 16: 3.6 us).  A lane owns four states of a channel (16 bytes each way) and goes over four clips at a
 // time, so that four states are requested before the first is used and the lanes of a quad form the step and the gate of one
-// clip each (one clip at a time: 100 us).  VEC: rows of A, B, C and the states are whole and aligned groups
-// of four; otherwise they are read entry by entry (2048 x 1024 x 16 121 us instead of 48).  state_out may be the state itself: a lane reads its entries before it
-// writes them and nobody else needs them.
+// clip each (one clip at a time: 100 us).  VEC: rows of A, B, C and the states are whole and aligned groups of four; otherwise
+// they are read entry by entry (2048 x 1024 x 16 121 us instead of 48).  state_out may be the state itself: a lane reads its
+// entries before it writes them and nobody else needs them.
 template <typename T, bool VEC> __device__ __forceinline__ void step_load4(const T* __restrict__ row, int j, int N, float (&v)[4]) {
     if constexpr (VEC) {
         typename SeqVec<T, 4>::type w = {};
