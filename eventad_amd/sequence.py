@@ -29,6 +29,9 @@ _MAX_LD = 1 << 24               # row strides above this are taken by copying th
 
 # A single-token call is bound by this file: the checks below compare identities and device numbers, read each attribute once
 # and pass plain integers to the library.
+#
+# A backward pass checks its saved tensors like a call's arguments and takes their strides anew: what a saved-tensor hook gives back
+# (torch.autograd.graph.save_on_cpu, say) need not be laid out as what it was given.
 
 
 def _fail(msg, *args):
@@ -183,24 +186,26 @@ class _ConvFn(torch.autograd.Function):
     def forward(ctx, x, w, bias, state, ldx, starts, clips, act, want_state):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, w, bias, state, starts)
-        ctx.ldx, ctx.clips, ctx.act = ldx, clips, act
+        ctx.act = act
         return _conv_fwd(x, ldx, w, bias, starts, clips, state, act, want_state)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
         x, w, bias, state, starts = ctx.saved_tensors
-        rows, D = x.shape
-        K = w.shape[1]
-        with _on(x.get_device()):
+        index = _device(x)
+        with _on(index):
+            starts, clips = _clips(starts, index)
+            x, ldx, w, bias, state, K = _conv_args(x, w, bias, state, None, clips, index)
+            rows, D = x.shape
             dy, ldy = _gradient(dy, x)
-            dfinal = None if dfinal is None else dfinal.contiguous()
+            dfinal = _tensor("the final state's gradient", dfinal, (clips, K - 1, D), x.dtype, index)
             dx = x.new_empty((rows, D))
             dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
             dp = w.new_empty(D * (K + 1))
             ws = _workspace(_bytes("eventad_causal_conv_workspace", rows, D, K), x)
-            _call("eventad_causal_conv_bwd", _p(x), ctx.ldx, _p(w), _p(bias), _p(starts), ctx.clips, _p(state), _p(dy), ldy, _p(dfinal),
-                  _p(dx), D, _p(dstate), _p(dp), _p(ws), ws.numel(), rows, D, K, ctx.act, _DTYPE[x.dtype], _stream(x.get_device()))
+            _call("eventad_causal_conv_bwd", _p(x), ldx, _p(w), _p(bias), _p(starts), clips, _p(state), _p(dy), ldy, _p(dfinal),
+                  _p(dx), D, _p(dstate), _p(dp), _p(ws), ws.numel(), rows, D, K, ctx.act, _DTYPE[x.dtype], _stream(index))
         return dx, dp.as_strided((D, K), (K, 1)), dp.as_strided((D,), (1,), D * K) if bias is not None else None, dstate, None, None, None, None, None
 
 
@@ -287,27 +292,30 @@ class _ScanFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         y, final, ckpt = _scan_fwd(u, delta, A, B, C, D, z, bias, state, lds, starts, clips, softplus, want_state, True)
         ctx.save_for_backward(u, delta, A, B, C, D, z, bias, state, starts, ckpt)
-        ctx.lds, ctx.clips, ctx.softplus = lds, clips, softplus
+        ctx.softplus = softplus
         return y, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
-        u, delta, A, B, C, D, z, bias, state, starts, ckpt = ctx.saved_tensors
-        rows, ch = u.shape
-        N = A.shape[1]
-        ldu, ldd, ldb, ldc, ldz = ctx.lds
-        with _on(u.get_device()):
+        *t, starts, ckpt = ctx.saved_tensors
+        index = _device(t[0])
+        with _on(index):
+            starts, clips = _clips(starts, index)
+            (u, delta, A, B, C, D, z, bias, state), (ldu, ldd, ldb, ldc, ldz) = _scan_args(*t, clips, index)
+            rows, ch = u.shape
+            N = A.shape[1]
+            ckpt = _tensor("the checkpoint", ckpt, (max(16, _bytes("eventad_selective_scan_checkpoint", rows, ch, N)),), torch.uint8, index)
             dy, ldy = _gradient(dy, u)
-            dfinal = None if dfinal is None else dfinal.contiguous()
+            dfinal = _tensor("the final state's gradient", dfinal, (clips, ch, N), _F32, index)
             new = lambda n: u.new_empty((rows, n))
             du, dd, dB, dC, dz = new(ch), new(ch), new(N), new(N), new(ch) if z is not None else None
             dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[8] else None
             dp = A.new_empty(ch * (N + 2))
             ws = _workspace(_bytes("eventad_selective_scan_workspace", rows, ch, N, 1), u)
             _call("eventad_selective_scan_bwd", _p(u), ldu, _p(delta), ldd, _p(A), _p(B), ldb, _p(C), ldc, _p(D), _p(z), ldz, _p(bias), _p(starts),
-                  ctx.clips, _p(state), _p(ckpt), _p(dy), ldy, _p(dfinal), _p(du), ch, _p(dd), ch, _p(dB), N, _p(dC), N, _p(dz), ch,
-                  _p(dstate), _p(dp), _p(ws), ws.numel(), rows, ch, N, ctx.softplus, _DTYPE[u.dtype], _stream(u.get_device()))
+                  clips, _p(state), _p(ckpt), _p(dy), ldy, _p(dfinal), _p(du), ch, _p(dd), ch, _p(dB), N, _p(dC), N, _p(dz), ch,
+                  _p(dstate), _p(dp), _p(ws), ws.numel(), rows, ch, N, ctx.softplus, _DTYPE[u.dtype], _stream(index))
         return (du, dd, dp.as_strided((ch, N), (N, 1)), dB, dC, dp.as_strided((ch,), (1,), ch * N) if D is not None else None, dz,
                 dp.as_strided((ch,), (1,), ch * (N + 1)) if bias is not None else None, dstate, None, None, None, None, None)
 
@@ -393,22 +401,24 @@ class _NormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         y, total = _norm_fwd(x, ldx, weight, residual, ldr, eps)
         ctx.save_for_backward(x if total is None else total, weight)
-        ctx.ldh, ctx.eps = ldx if total is None else x.shape[1], eps
+        ctx.eps = eps
         return y, total
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dtotal):
         h, weight = ctx.saved_tensors
-        rows, D = h.shape
-        with _on(h.get_device()):
+        index = _device(h)
+        with _on(index):
+            h, ldh, weight, _, _, eps = _norm_args(h, weight, None, ctx.eps, index)
+            rows, D = h.shape
             dy, ldy = _gradient(dy, h)
             dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h)
             dh = h.new_empty((rows, D))
             dw = weight.new_empty(D)
             ws = _workspace(_bytes("eventad_rms_norm_workspace", rows, D), h)
-            _call("eventad_rms_norm_bwd", _p(h), ctx.ldh, _p(weight), _p(dy), ldy, _p(dtotal), ldt, _p(dh), D, _p(dw), _p(ws), ws.numel(), rows,
-                  D, ctx.eps, _DTYPE[h.dtype], _stream(h.get_device()))
+            _call("eventad_rms_norm_bwd", _p(h), ldh, _p(weight), _p(dy), ldy, _p(dtotal), ldt, _p(dh), D, _p(dw), _p(ws), ws.numel(), rows,
+                  D, eps, _DTYPE[h.dtype], _stream(index))
         return dh, dw, dh if ctx.needs_input_grad[2] else None, None, None, None
 
 

@@ -790,3 +790,35 @@ def test_refusals(S):
         S.selective_scan_step(x, x, A, Bm, Bm, s1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_gradients_under_saved_tensor_hooks(S):
+    """Offloading packs the slices that were saved, another hook spreads them out: the gradients are bit for bit those of calls
+    on arrays that are laid out so from the start."""
+    gen = torch.Generator().manual_seed(21)
+    rows, ch, N, b = 75, 24, 16, [0, 30, 30, 71]
+    packed = lambda t: t.contiguous().clone()
+    spread = lambda t: torch.cat([t, torch.full_like(t[:, :1], float("nan")).expand(-1, 9)], 1)[:, :t.shape[1]]
+    slices = lambda t: t if t.is_contiguous() else spread(t)     # (the norm's own sum, which it saves, stays packed)
+    plain, on_cpu = torch.autograd.graph.saved_tensors_hooks, torch.autograd.graph.save_on_cpu
+    for dt in DTYPES.values():
+        wide = rnd(gen, rows, 4 * ch + 2 * N + 3, dtype=dt)
+        at = lambda c, n: wide[:, c:c + n]
+        acts = [at(0, ch), at(ch + 1, ch), at(4 * ch, N), at(4 * ch + N, N), at(2 * ch, ch), at(3, ch), at(5, ch), at(7, ch), at(ch, ch)]
+        others = [-torch.exp(rnd(gen, ch, N)), rnd(gen, ch), rnd(gen, ch, 4), rnd(gen, ch), rnd(gen, 3, ch, N), rnd(gen, 3, 3, ch, dtype=dt)]
+        dy, dh, dc = rnd(gen, rows, ch, dtype=dt), rnd(gen, 3, ch, N), rnd(gen, 3, 3, ch, dtype=dt)
+
+        def gradients(hooks, lay=lambda t: t):
+            L = [lay(t).detach().requires_grad_() for t in acts] + [t.detach().requires_grad_() for t in others]
+            u, delta, B, C, z, x, n1, n2, res, A, D, w, bias, h0, c0 = L
+            with hooks:
+                y, h = S.selective_scan(u, delta, A, B, C, D, z, bias, clip_start=starts_of(b), state=h0, return_state=True)
+                v, c = S.causal_conv(x, w, bias, starts_of(b), c0, return_state=True)
+                n = S.rms_norm(n1, D)
+                m, t = S.rms_norm(n2, D, res)
+            return torch.autograd.grad([y, h, v, c, n, m, t], L, [dy, dh, dy, dc, dy, dy, dy])
+
+        for lay, hooks in ((packed, on_cpu()), (packed, on_cpu(pin_memory=True)), (spread, plain(slices, lambda t: t))):
+            want = gradients(plain(lambda t: t, lambda t: t), lay)
+            for i, (p, q) in enumerate(zip(want, gradients(hooks))):
+                assert torch.equal(p, q), (dt, lay is packed, i)

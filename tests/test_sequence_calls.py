@@ -1,0 +1,76 @@
+"""What eventad_amd/sequence.py hands to the library, on the CPU: the library's calls are replaced by a record of their arguments."""
+import pytest
+import torch
+
+from eventad_amd import sequence as S
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The calls made, as (name, arguments); tensors of the CPU pass the checks in the place of a GPU's."""
+    made = []
+    monkeypatch.setattr(S, "_device", lambda t: t.get_device())
+    monkeypatch.setattr(S, "_elsewhere", lambda index: False)
+    monkeypatch.setattr(S, "_stream", lambda index: 0)
+    monkeypatch.setattr(S, "_bytes", lambda name, *shape: 64)
+    monkeypatch.setattr(S, "_call", lambda name, *args: made.append((name, args)))
+    return made
+
+
+ROWS, CH, N, TAPS, CLIPS = 6, 4, 3, 4, 2
+
+
+def run(op, state=True):
+    """One differentiable call on column slices of wider arrays -> (outputs, inputs that need a gradient)"""
+    wide = torch.randn(ROWS, 5 * CH + 2 * N, requires_grad=True)
+    at = lambda c, n: wide[:, c:c + n]
+    starts = torch.tensor([0, 2, ROWS], dtype=torch.int32)
+    x = at(1, CH)
+    if op == "conv":
+        s = torch.randn(CLIPS, TAPS - 1, CH, requires_grad=True) if state else None
+        return S.causal_conv(x, torch.randn(CH, TAPS), torch.randn(CH), starts, s, return_state=True), [t for t in (wide, s) if t is not None]
+    if op == "scan":
+        s = torch.randn(CLIPS, CH, N, requires_grad=True) if state else None
+        return S.selective_scan(x, at(CH, CH), -torch.ones(CH, N), at(3 * CH, N), at(4 * CH, N), torch.ones(CH), at(2 * CH, CH), torch.ones(CH), True,
+                                starts, s, True), [t for t in (wide, s) if t is not None]
+    return (S.rms_norm(x, torch.ones(CH)),), [wide]
+
+
+# (array, row stride) as positions in the arguments of each backward call
+STRIDED = {"conv": [(0, 1), (7, 8)], "scan": [(0, 1), (2, 3), (5, 6), (7, 8), (10, 11), (17, 18)], "norm": [(0, 1), (3, 4)]}
+
+
+@pytest.mark.parametrize("op", ["conv", "scan", "norm"])
+@pytest.mark.parametrize("spread", [False, True])
+def test_backward_takes_the_strides_of_what_saved_tensor_hooks_return(calls, op, spread):
+    """A hook (offloading, say) may give back a packed copy of a slice, or a slice of an array wider still."""
+    back = []
+
+    def unpack(t):
+        if t.dim() == 2 and t.dtype == torch.float32:
+            t = torch.cat([t, torch.zeros(t.shape[0], 7)], 1)[:, :t.shape[1]] if spread else t.clone().contiguous()
+        back.append(t)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        out, leaves = run(op)
+    back.clear()
+    kept = [torch.randn_like(o) for o in out]
+    torch.autograd.grad(out, leaves, kept)
+    name, args = next(c for c in calls if c[0].endswith("_bwd"))
+    strides = {t.data_ptr(): t.stride(0) for t in back + kept if t.dim() == 2}
+    for p, ld in STRIDED[op]:
+        assert args[p] in strides, (name, p)
+        assert args[ld] == strides[args[p]], (name, p, args[ld], strides[args[p]])
+    for t in back:                                               # parameters and states: no strides are passed for them
+        if t.dim() == 3 or (t.dim() == 2 and t.shape[0] == CH):
+            assert t.data_ptr() not in args or t.is_contiguous()
+
+
+@pytest.mark.parametrize("op", ["conv", "scan", "norm"])
+def test_backward_refuses_what_is_no_copy_of_the_saved_tensor(calls, op):
+    for change in (lambda t: t.half() if t.dtype == torch.float32 else t, lambda t: t[:-1], lambda t: t.new_zeros(t.numel())):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            out, leaves = run(op)
+        with pytest.raises(RuntimeError, match="eventad_amd.sequence"):
+            torch.autograd.grad(out, leaves, [torch.randn_like(o) for o in out])
