@@ -144,17 +144,17 @@ template <typename T> struct ScanRows {
 // takes one state of every (256 / N4)th row; rows of no clip and states >= N become zero.
 template <typename T, int N4> struct ScanStage {
     static constexpr int ALL = SCAN_TILE * N4, PER = (ALL + 255) / 256, STEP = 256 / N4;
-    char* p; unsigned step, at; bool in;
+    char* p; unsigned tile, at; bool in;             // tile: bytes from a tile to the next (2^30 at a row stride of 2^24)
     T v[PER];
     __device__ __forceinline__ ScanStage(const void* base, int64_t ld, int t0, int N)
-        : p((char*)base + (int64_t)t0 * ld * (int)sizeof(T)), step(STEP * (unsigned)ld * sizeof(T)), in(threadIdx.x % N4 < N) {
+        : p((char*)base + (int64_t)t0 * ld * (int)sizeof(T)), tile(SCAN_TILE * (unsigned)ld * sizeof(T)), in(threadIdx.x % N4 < N) {
         at = (unsigned)(threadIdx.x / N4 * (int)ld + min((int)threadIdx.x % N4, N - 1)) * sizeof(T);
     }
     __device__ __forceinline__ void load(bool full, int left) {                                  // left: rows of the tile
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             v[i] = (T)0.f;
-            if ((full || (int)threadIdx.x / N4 + i * STEP < left) && (ALL >= 256 || (int)threadIdx.x < ALL)) v[i] = *(const T*)(p + (scan_again(at) + i * step));
+            if ((full || (int)threadIdx.x / N4 + i * STEP < left) && (ALL >= 256 || (int)threadIdx.x < ALL)) v[i] = *(const T*)(p + (scan_again(at) + i * (tile / PER)));
         }
     }
     __device__ __forceinline__ void store(float* __restrict__ s, int t0, int lo, int hi) const {
@@ -166,7 +166,7 @@ template <typename T, int N4> struct ScanStage {
         }
     }
     template <int DIR> __device__ __forceinline__ void move(bool go) {
-        const unsigned by = go ? (STEP > SCAN_TILE ? step / (STEP / SCAN_TILE) : SCAN_TILE / STEP * step) : 0u;
+        const unsigned by = go ? tile : 0u;
         p = DIR > 0 ? p + by : p - by;
     }
 };

@@ -822,3 +822,42 @@ def test_gradients_under_saved_tensor_hooks(S):
             want = gradients(plain(lambda t: t, lambda t: t), lay)
             for i, (p, q) in enumerate(zip(want, gradients(hooks))):
                 assert torch.equal(p, q), (dt, lay is packed, i)
+
+
+@pytest.mark.parametrize("N", [1, 3, 4, 8, 16, 24, 64])
+def test_scan_rows_at_the_largest_stride(S, N):
+    """Every array a slice of rows 2^24 elements apart, the most that is taken without a copy: results are those of packed arrays."""
+    gen, rows, ch, b = torch.Generator().manual_seed(N), 60, 20000, [0, 33, 58]               # (so wide that the rows are one chunk, both ways)
+    held = torch.empty(rows, 1 << 24, device="cuda")             # 4 GB
+    A, D, h0 = -torch.exp(rnd(gen, ch, N)), rnd(gen, ch), rnd(gen, 2, ch, N)
+    dy, dh, views, at = rnd(gen, rows, ch), rnd(gen, 2, ch, N), [], 0
+    for n in (ch, ch, N, N, ch):
+        views.append(held[:, at:at + n].copy_(torch.randn(rows, n, generator=gen)))
+        at += n + 1
+    runs = []
+    for t in (views, [v.contiguous() for v in views]):
+        L = [v.detach().requires_grad_() for v in (*t, A, D, h0)]
+        u, delta, B, C, z, a, d, h = L
+        assert t is not views or B.stride(0) == 1 << 24
+        y, f = S.selective_scan(u, delta, a, B, C, d, z, clip_start=starts_of(b), state=h, return_state=True)
+        runs.append([y, f, *torch.autograd.grad([y, f], L, [dy, dh])])
+        with torch.no_grad():
+            s = torch.ones(rows, ch, N, device="cuda")
+            runs[-1] += [S.selective_scan_step(u, delta, a, B, C, s, d, z), s]
+    for i, (p, q) in enumerate(zip(*runs)):
+        assert torch.equal(p, q), i
+
+
+def test_convolution_and_norm_rows_at_the_largest_stride(S):
+    gen, rows, ch, b = torch.Generator().manual_seed(1), 70, 8, [0, 33, 68]
+    held = torch.empty(rows, 1 << 24, device="cuda")
+    views = [held[:, at:at + ch].copy_(torch.randn(rows, ch, generator=gen)) for at in (0, 8)]
+    w, nw, dy = rnd(gen, ch, 4), rnd(gen, ch), rnd(gen, rows, ch)
+    runs = []
+    for t in (views, [v.contiguous() for v in views]):
+        L = [v.detach().requires_grad_() for v in (*t, w, nw)]
+        out = [S.causal_conv(L[0], L[2], clip_start=starts_of(b)), *S.rms_norm(L[0], L[3], L[1]), S.rms_norm(L[0], L[3])]
+        runs.append([*out, *torch.autograd.grad(out, L, [dy] * 4), *(q.float() for q in S.rms_norm_fp8(t[0], nw, t[1]))])
+        runs[-1].append(S.causal_conv_step(t[0], w, torch.ones(rows, 3, ch, device="cuda")))
+    for i, (p, q) in enumerate(zip(*runs)):
+        assert torch.equal(p, q), i
