@@ -11,12 +11,13 @@ slice of a wider array (any row stride); an array whose channels are not adjacen
 Every function launches on the current stream of its tensors' device, waits for nothing, and can be captured into a graph;
 workspaces come from torch's allocator per call, so captured graphs do not share one.  The functions are differentiable
 (except the single-token and 8-bit forms, which refuse inputs that need a gradient); gradients are not differentiable
-again.  There is no CPU path: tensors must be on a GPU."""
+again, and there are no forward-mode derivatives.  There is no CPU path: tensors must be on a GPU."""
 import contextlib
 import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import NativeError, load
@@ -124,6 +125,10 @@ def _clips(clip_start, index):
 
 
 def _needs_grad(*tensors):
+    if forward_ad._current_level >= 0:                           # (inside forward_ad.dual_level or torch.func.jvp)
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                _fail("there is no forward-mode derivative")
     if torch.is_grad_enabled():
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:

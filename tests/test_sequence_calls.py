@@ -74,3 +74,27 @@ def test_backward_refuses_what_is_no_copy_of_the_saved_tensor(calls, op):
             out, leaves = run(op)
         with pytest.raises(RuntimeError, match="eventad_amd.sequence"):
             torch.autograd.grad(out, leaves, [torch.randn_like(o) for o in out])
+
+
+def every_form():
+    """(name, tensors, call of those tensors): each entry point with every tensor that it takes a derivative of"""
+    r, starts = torch.randn, torch.tensor([0, 2, ROWS], dtype=torch.int32)
+    rows = dict(u=r(ROWS, CH), delta=r(ROWS, CH), A=r(CH, N), B=r(ROWS, N), C=r(ROWS, N), D=r(CH), z=r(ROWS, CH), delta_bias=r(CH))
+    norm = dict(x=r(ROWS, CH), weight=r(CH), residual=r(ROWS, CH))
+    return [("causal_conv", dict(x=r(ROWS, CH), weight=r(CH, TAPS), bias=r(CH), state=r(CLIPS, TAPS - 1, CH)), lambda **t: S.causal_conv(clip_start=starts, **t)),
+            ("causal_conv_step", dict(x=r(ROWS, CH), weight=r(CH, TAPS), state=r(ROWS, TAPS - 1, CH), bias=r(CH)), S.causal_conv_step),
+            ("selective_scan", dict(rows, state=r(CLIPS, CH, N)), lambda **t: S.selective_scan(clip_start=starts, **t)),
+            ("selective_scan_step", dict(rows, state=r(ROWS, CH, N)), S.selective_scan_step), ("rms_norm", norm, S.rms_norm), ("rms_norm_fp8", norm, S.rms_norm_fp8)]
+
+
+def test_forward_mode_derivatives_are_refused(calls):
+    for name, tensors, f in every_form():
+        for dual in tensors:
+            with torch.autograd.forward_ad.dual_level():
+                t = dict(tensors)
+                t[dual] = torch.autograd.forward_ad.make_dual(t[dual], torch.ones_like(t[dual]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(**t)
+        with torch.autograd.forward_ad.dual_level():
+            f(**tensors)                                         # nothing dual among them
+    assert len(calls) == 6
