@@ -9,7 +9,8 @@ Activations are float32, bfloat16 or float16, all of one call alike; parameters 
 slice of a wider array (any row stride); an array whose channels are not adjacent is copied first.
 
 Every function launches on the current stream of its tensors' device, waits for nothing, and can be captured into a graph;
-workspaces come from torch's allocator per call, so captured graphs do not share one.  The functions are differentiable
+workspaces come from torch's allocator per call, so captured graphs do not share one.  torch.jit.trace and make_fx cannot record
+the functions and are refused.  The functions are differentiable
 (except the single-token and 8-bit forms, which refuse inputs that need a gradient); gradients are not differentiable
 again, and there are no forward-mode derivatives.  There is no CPU path: tensors must be on a GPU."""
 import contextlib
@@ -124,7 +125,19 @@ def _clips(clip_start, index):
     return clip_start.contiguous(), clip_start.numel() - 1
 
 
+def _traced():
+    """A tracer records torch's own operations: of these calls the allocation of the result, and nothing that fills it."""
+    if torch._C._is_tracing():
+        return True
+    if torch._C._len_torch_dispatch_stack():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        return get_proxy_mode() is not None
+    return False
+
+
 def _needs_grad(*tensors):
+    if _traced():
+        _fail("the call cannot be recorded by torch.jit.trace or make_fx")
     if forward_ad._current_level >= 0:                           # (inside forward_ad.dual_level or torch.func.jvp)
         for t in tensors:
             if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:

@@ -98,3 +98,19 @@ def test_forward_mode_derivatives_are_refused(calls):
         with torch.autograd.forward_ad.dual_level():
             f(**tensors)                                         # nothing dual among them
     assert len(calls) == 6
+
+
+@pytest.mark.parametrize("pending", [False, True])
+def test_tracers_are_refused(calls, pending):
+    """They would record the result's allocation and nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for name, tensors, f in every_form():
+        if pending and (name.endswith("_step") or name.endswith("_fp8")):
+            continue
+        keys = list(tensors)
+        call = lambda *t: f(**dict(zip(keys, t)))
+        args = tuple(t.clone().requires_grad_(pending) for t in tensors.values())
+        for record in (lambda: torch.jit.trace(call, args, check_trace=False), lambda: make_fx(call)(*args), lambda: make_fx(call, tracing_mode="fake")(*args)):
+            with pytest.raises(RuntimeError, match="recorded by torch.jit.trace or make_fx"):
+                record()
+    assert not calls
