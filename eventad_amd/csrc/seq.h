@@ -4,8 +4,9 @@
 // Rows of a [rows, channels] array are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1 (i32[clips+1], not
 // decreasing, inside 0..rows); rows in front of the first and behind the last clip belong to none.  Without an array all
 // rows are one clip.  The offsets are read on the device only, so no call waits for the GPU and every launch can be
-// captured; whatever they hold, they are only compared with row numbers that the launch made itself, so wrong offsets give
-// wrong numbers, never an access outside an array.
+// captured; whatever they hold, they are only compared with row numbers that the launch made itself: offsets outside 0..rows
+// count as the nearer end, and ones that decrease give wrong numbers (and leave states of clips that no row leads to as they
+// were), never an access outside an array.
 #pragma once
 #include "common.h"
 
@@ -87,7 +88,7 @@ template <int LANES> __device__ __forceinline__ float seq_lane_sum(float v) {
 
 struct SeqClips { const int* start; int n; int rows; };        // start == nullptr: one clip of all rows
 
-__device__ __forceinline__ int seq_start(const SeqClips& c, int s) { return c.start ? c.start[s] : (s ? c.rows : 0); }
+__device__ __forceinline__ int seq_start(const SeqClips& c, int s) { return c.start ? min(max(c.start[s], 0), c.rows) : (s ? c.rows : 0); }
 
 // the last s in 0..n with start[s] <= row, or -1: the clip of the row (n: behind the last clip), empty clips skipped
 __device__ __forceinline__ int seq_find(const SeqClips& c, int row) {

@@ -93,7 +93,7 @@ __device__ __forceinline__ void conv_window(const ConvArgs& a, int c, int s, int
         for (int i = 0; i < V; ++i) win[k][i] = 0.f;
         if (s < 0 || s >= a.clips.n || k < skip) continue;
         float v[V];
-        if (q >= max(first, 0)) seq_load<T, V>((const T*)a.x + (int64_t)q * a.ldx + c, v);
+        if (q >= first) seq_load<T, V>((const T*)a.x + (int64_t)q * a.ldx + c, v);
         else if (a.state && q < first) seq_load<T, V>((const T*)a.state + ((int64_t)s * (a.taps - 1) + (K - 1 - skip + q - first)) * a.channels + c, v);
         else continue;
 #pragma unroll

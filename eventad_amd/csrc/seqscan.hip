@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, LPC > 8 ? 3 : 4) void k_scan_fwd(ScanArgs a) {
     }
     if (c1 <= c0) return;
     // rows that belong to a clip (WHAT 1: to the one that matters)
-    const int lo = WHAT == 1 ? at : max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));
+    const int lo = WHAT == 1 ? at : seq_start(a.clips, 0), hi = min(c1, seq_start(a.clips, n));
     const bool gated = WHAT == 0 && a.z;
     int t0 = at / SCAN_TILE * SCAN_TILE, buf = 0;
     ScanRows<T> fu(a.u, a.ldu, t0, L.q, L.d), fd(a.delta, a.ldd, t0, L.q, L.d), fz(a.z, a.ldz, t0, L.q, L.d), oy(a.y, a.ldy, t0, L.q, L.d);
@@ -590,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     if (s >= 0 && s < n && seq_start(a.clips, s + 1) > c1) {
         if (a.chunks > 1) scan_load(a.carry + ((size_t)chunk * a.channels + L.d) * N4, L.j, N4, g);
     } else entry(s);
-    const int lo = max(0, seq_start(a.clips, 0)), hi = min(c1, seq_start(a.clips, n));            // rows that belong to a clip
+    const int lo = seq_start(a.clips, 0), hi = min(c1, seq_start(a.clips, n));                    // rows that belong to a clip
     float* my_red = red[wave] + (lane >> 5) * N4 + ST * L.j + (ST > 1 ? FOLD * ((lane >> 4) & 1) : 0);               // (its last row takes what no row wants)
     const bool gated = a.z;
     int t0 = (c1 - 1) / SCAN_TILE * SCAN_TILE, buf = 0, end = c1;

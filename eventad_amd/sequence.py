@@ -4,7 +4,8 @@ matrix products.  The reference's temporal part is the GRU of its head (models/E
 there.
 
 Rows are packed: activations are [rows, channels], clip s owns rows clip_start[s] .. clip_start[s+1]-1 (int32 on the device,
-not decreasing, within 0..rows; None = all rows are one clip); rows of no clip give zeros and take no part in a gradient.
+not decreasing; below 0 counts as 0, above rows as rows; None = all rows are one clip); rows of no clip give zeros and take
+no part in a gradient.
 Activations are float32, bfloat16 or float16, all of one call alike; parameters and scan states are float32.  A row may be a
 slice of a wider array (any row stride); an array whose channels are not adjacent is copied first.
 

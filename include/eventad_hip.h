@@ -511,8 +511,10 @@ int eventad_incr_pool0(const float* y2, const float* map_nhwc, int map_h, int ma
  * Arrays of activations are [rows, channels] with a row stride in elements (channels <= ld* <= 2^24; adjacent channels are
  * adjacent in memory), of type dtype = 0 float32, 1 bfloat16, 2 float16, all of one call alike; parameters and scan states are
  * float32, sums are formed in float32.  Rows are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1, clip_start
- * i32[clips+1] on the device, not decreasing, within 0..rows (NULL with clips = 1: all rows are one clip).  Rows of no
- * clip are neither read into a result nor counted in a gradient; their outputs and gradients are written as zeros.
+ * i32[clips+1] on the device, not decreasing (NULL with clips = 1: all rows are one clip); offsets below 0 count as 0 and ones
+ * above rows as rows.  Offsets that decrease give wrong numbers and may leave states unwritten; nothing outside the arrays
+ * is accessed.  Rows of no clip are neither read into a result nor counted in a gradient; their outputs and gradients are
+ * written as zeros.
  * A launch that would need more than 2^32 threads (rows x channels beyond 3e10) is refused with EVENTAD_ERR_TOO_LARGE.
  * Outputs must not overlap inputs unless it says so.  Results are reproducible bit for bit (no float atomics).
  * workspace: 16-byte aligned device memory of at least the bytes that the *_workspace function of the same shape reports

@@ -861,3 +861,29 @@ def test_convolution_and_norm_rows_at_the_largest_stride(S):
         runs[-1].append(S.causal_conv_step(t[0], w, torch.ones(rows, 3, ch, device="cuda")))
     for i, (p, q) in enumerate(zip(*runs)):
         assert torch.equal(p, q), i
+
+
+@pytest.mark.parametrize("rows,taps,N", [(70, 4, 16), (70, 8, 4), (9, 3, 24), (1000, 6, 16), (70, 2, 40)])
+@pytest.mark.parametrize("bounds", [[-5, 30, 75], [-3, -1, 70], [0, 30, 200], [5, 2000, 3000], [80, 90], [-9, -4], [-(1 << 31), (1 << 31) - 1], [-7, -7, 20, 20, 5000, 5000],
+                                    [20, 10, 40, 5, 90], [60, 0, 70], [69, 3, 2]])
+def test_every_entry_is_written_whatever_the_offsets(S, monkeypatch, rows, taps, N, bounds):
+    """Outputs, gradients and workspaces come filled with NaN.  Offsets outside the array count as its nearer end, states included; with
+    offsets that decrease every row is written all the same."""
+    gen, ch, clips = torch.Generator().manual_seed(rows + N), 8, len(bounds) - 1
+    allocate, like = torch.Tensor.new_empty, torch.empty_like
+    spoil = lambda t: t.fill_(255 if t.dtype == torch.uint8 else float("nan"))
+    monkeypatch.setattr(torch.Tensor, "new_empty", lambda self, *a, **k: spoil(allocate(self, *a, **k)))
+    monkeypatch.setattr(torch, "empty_like", lambda *a, **k: spoil(like(*a, **k)))
+    t = [rnd(gen, rows, n) for n in (ch, ch, N, N, ch)] + [rnd(gen, clips, ch, N), rnd(gen, clips, taps - 1, ch)]
+    A, w, dy, dh, dc = -rnd(gen, ch, N).abs(), rnd(gen, ch, taps), rnd(gen, rows, ch), rnd(gen, clips, ch, N), rnd(gen, clips, taps - 1, ch)
+    runs = []
+    for b in (bounds, [min(max(v, 0), rows) for v in bounds]):
+        L = [v.detach().requires_grad_() for v in t]
+        y, h = S.selective_scan(L[0], L[1], A, L[2], L[3], None, L[4], clip_start=starts_of(b), state=L[5], return_state=True)
+        v, c = S.causal_conv(L[0], w, None, starts_of(b), L[6], return_state=True)
+        of_rows = [y, v, *torch.autograd.grad([y, h], L[:5], [dy, dh], retain_graph=True), *torch.autograd.grad([v, c], L[:1], [dy, dc], retain_graph=True)]
+        of_clips = [h, c, *torch.autograd.grad([y, h], L[5:6], [dy, dh]), *torch.autograd.grad([v, c], L[6:], [dy, dc])]
+        runs.append(of_rows + (of_clips if bounds == sorted(bounds) else []))
+    for i, (p, q) in enumerate(zip(*runs)):
+        assert bool(torch.isfinite(p).all()), i
+        assert torch.equal(p, q), i
