@@ -27,6 +27,8 @@ from ._lib import NativeError, load
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACT = {None: 0, "silu": 1}
 _F32, _I32 = torch.float32, torch.int32
+_Tensor = torch.Tensor
+_tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 MAX_TAPS, MAX_STATE = 8, 64
 _MAX_LD = 1 << 24               # row strides above this are taken by copying the array
 
@@ -55,7 +57,7 @@ def _call(name, *args):
 
 def _device(t):
     """The GPU's number."""
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, _Tensor):
         _fail("expected a tensor, got %s", type(t).__name__)
     index = t.get_device() if t.is_cuda else -1
     if index < 0:
@@ -80,11 +82,12 @@ def _stream(index):
 
 def _rows(name, t, rows, width, dtype, index):
     """Checks an array [rows, width] (None: any) -> it with adjacent channels, and its row stride in elements."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+    if not (t.__class__ is _Tensor or isinstance(t, _Tensor)) or t.dtype is not dtype or t.get_device() != index:
         _fail("%s must be a %s tensor on GPU %d", name, dtype, index)
-    if t.dim() != 2:
-        _fail("%s has %d dimensions, expected [rows, channels]", name, t.dim())
-    n, m = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        _fail("%s has %d dimensions, expected [rows, channels]", name, len(shape))
+    n, m = shape
     if (rows is not None and n != rows) or (width is not None and m != width):
         _fail("%s has shape %s, expected %s", name, (n, m), ("*" if rows is None else rows, "*" if width is None else width))
     ld, step = t.stride()
@@ -99,7 +102,7 @@ def _tensor(name, t, shape, dtype, index):
     """Checks a parameter or a state -> it, contiguous (None stays None)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+    if not (t.__class__ is _Tensor or isinstance(t, _Tensor)) or t.dtype is not dtype or t.get_device() != index:
         _fail("%s must be a %s tensor on GPU %d", name, dtype, index)
     if t.shape != shape:
         _fail("%s has shape %s, expected %s", name, tuple(t.shape), shape)
@@ -126,26 +129,22 @@ def _clips(clip_start, index):
     return clip_start.contiguous(), clip_start.numel() - 1
 
 
-def _traced():
-    """A tracer records torch's own operations: of these calls the allocation of the result, and nothing that fills it."""
-    if torch._C._is_tracing():
-        return True
-    if torch._C._len_torch_dispatch_stack():
-        from torch.fx.experimental.proxy_tensor import get_proxy_mode
-        return get_proxy_mode() is not None
-    return False
+def _proxies():
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
 
 
 def _needs_grad(*tensors):
-    if _traced():
+    # A tracer records torch's own operations: of these calls the allocation of the result, and nothing that fills it.
+    if _tracing() or (_modes() and _proxies()):
         _fail("the call cannot be recorded by torch.jit.trace or make_fx")
     if forward_ad._current_level >= 0:                           # (inside forward_ad.dual_level or torch.func.jvp)
         for t in tensors:
-            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
                 _fail("there is no forward-mode derivative")
     if torch.is_grad_enabled():
         for t in tensors:
-            if isinstance(t, torch.Tensor) and t.requires_grad:
+            if t is not None and isinstance(t, _Tensor) and t.requires_grad:
                 return True
     return False
 
