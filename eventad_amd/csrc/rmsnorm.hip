@@ -173,7 +173,8 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
 // y / scale = 448 p / max|p| with p = h w needs no r.  A value next to a border of the 8-bit grid has to fall on the side the
 // definition says, so the quotient is formed in float32 (p, its maximum, 448 / maximum and the product: error below 5 units in the
 // last place) and, where it lies within 8 of a border, again in float64, where p is exact.  One value in 60,000 of ordinary data
-// does.
+// does.  A row with max|p| below 2^-100 is formed in float64 altogether: 448 / max|p| leaves float32 at 1.3e-36, and below 1.2e-38 p
+// has not all its bits.
 
 // v rounded towards the odd neighbour, so that a second rounding to fewer bits is the one rounding of v: e4m3 keeps 4 of the
 // 24 bits of a float
@@ -241,6 +242,7 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
     if (zero) scale = 1.f;
     if (in && lane == 0) a.scale[r] = scale;
     const float by32 = zero ? inv : 448.f / __uint_as_float(most);
+    const bool tiny = !zero && most < 0x0d800000u;               // 2^-100
     // p -> q of a piece; true if a value lies too close to a border
     auto divide = [&](const float (&v)[V], float (&q)[V]) {
         unsigned near = 0xffffffffu, low = 0xffffffffu;
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
             near = min(near, (u << 12) - 0x7fff8000u);           // (borders: the 20 bits that e4m3 has not are 0x80000)
             low = min(low, (u << 1) - 2u);
         }
-        bool close = near <= 0x10000u;
+        bool close = tiny || near <= 0x10000u;
         if (low < 0x79000000u - 2u) {                            // below 2^-6: steps of 2^-9, borders between them
 #pragma unroll
             for (int i = 0; i < V; ++i)

@@ -457,8 +457,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
-    """rms_norm's y in 8 bits for a scaled matrix product: scale float32 [rows] = max|y| / 448 of the row (1 for a row of zeros),
-    q torch.float8_e4m3fn [rows, channels] = y / scale rounded to nearest even.  -> (q, scale), or (q, scale, h) with a residual."""
+    """rms_norm's y in 8 bits for a scaled matrix product: scale float32 [rows] = max|y| / 448 of the row (1 where that is below the
+    smallest normal number, 1.2e-38: a row of zeros comes back as zeros), q torch.float8_e4m3fn [rows, channels] = y / scale
+    rounded to nearest even.  -> (q, scale), or (q, scale, h) with a residual."""
     if _needs_grad(x, weight, residual):
         _fail("the 8-bit form has no gradient: use rms_norm, or torch.no_grad()")
     index = _device(x)

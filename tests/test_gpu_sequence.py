@@ -887,3 +887,21 @@ def test_every_entry_is_written_whatever_the_offsets(S, monkeypatch, rows, taps,
     for i, (p, q) in enumerate(zip(*runs)):
         assert bool(torch.isfinite(p).all()), i
         assert torch.equal(p, q), i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [5, 64, 1030, 2048, 9000, 33000])
+def test_rms_norm_fp8_of_tiny_rows(S, dtype, channels):
+    """Rows of numbers around the smallest normal one, 1.2e-38, and far below 1, zeros among them: the nearest values all the same."""
+    gen, dt = torch.Generator().manual_seed(channels), DTYPES[dtype]
+    size = torch.tensor([1e-20, 1e-30, 1e-35, 1e-36, 3e-37, 1e-37, 3e-38, 1e-38, 1e-39])[:, None]
+    x = torch.randn(len(size), channels, generator=gen)
+    x = (x / x.abs().amax(1, keepdim=True) * size).to(dt)
+    x[:, 1] = 0.0
+    w = torch.randn(channels, generator=gen).abs() + 0.5
+    w[x[-1].abs().argmax()] = 2.0 ** 5                           # (the last row's scale, 32 x 1e-39 x 1000 / 448 = 7e-38, is a normal number)
+    want = R.norm(x, w, None, 1e-6)
+    assert float(want["scale"][0].min()) > 1.2e-38
+    q, scale = S.rms_norm_fp8(x.cuda(), w.cuda())
+    assert torch.equal(q.double().cpu(), want["q"])
+    close("scale", scale, want["scale"][0], (channels / 16 + 28) * want["scale"][0])
