@@ -88,6 +88,13 @@ __device__ __forceinline__ float scan_softplus(float x) {
     return fmaf(2.f * r, p, fmaxf(x, 0.f));
 }
 
+// A as the exponent of 2.  A step of 0 stands for a row that leaves the state as it is, also where A is -inf (a state that forgets
+// at once): the lowest finite number takes its place, with which every step of 1e-36 or more still gives exp(s A) = 0.
+__device__ __forceinline__ float scan_decay(float A) {
+    const float e = A * SEQ_LOG2E;
+    return e < -3.4028235e38f ? -3.4028235e38f : e;              // (NaN stays)
+}
+
 // lane's place in its workgroup
 template <int LPC> struct ScanLane {
     int d, j, q; bool in;                            // channel, lane of the channel, lane of the quad, channel exists
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(256, LPC > 8 ? 3 : 4) void k_scan_fwd(ScanArgs a) {
     for (int m = 0; m < ST; ++m) h[m] = 0.f;
     scan_load(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
-    for (int i = 0; i < ST; ++i) A2[i] *= SEQ_LOG2E;
+    for (int i = 0; i < ST; ++i) A2[i] = scan_decay(A2[i]);
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = WHAT == 0 && a.D ? a.D[L.d] : 0.f;
     auto entry = [&](int s) {                                    // the state in front of clip s
 #pragma unroll
@@ -397,7 +404,7 @@ __global__ __launch_bounds__(16 * G) void k_scan_join(ScanArgs a, int n4) {
     const int col = threadIdx.x & 15, group = threadIdx.x >> 4, one = threadIdx.x / G, lane = threadIdx.x % G;
     const int64_t width = (int64_t)a.channels * n4, place = (int64_t)blockIdx.x * 16 + col, at = place < width ? place : width - 1;
     const int d = (int)(at / n4), i = (int)(at - (int64_t)d * n4);
-    const float A2 = i < a.n_state ? a.A[(size_t)d * a.n_state + i] * SEQ_LOG2E : 0.f;
+    const float A2 = i < a.n_state ? scan_decay(a.A[(size_t)d * a.n_state + i]) : 0.f;
     const int share = (a.chunks + G - 1) / G, first = group * share, mine = min(share, a.chunks - first);
     float own[JOIN_SHARE], e[JOIN_SHARE], in = 0.f, pass = 1.f;
     int alone[JOIN_SHARE];
@@ -455,7 +462,7 @@ __global__ __launch_bounds__(256, LPC > 4 ? 3 : 4) void k_scan_adj(ScanArgs a) {
     for (int m = 0; m < ST; ++m) g[m] = 0.f;
     scan_load(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
-    for (int i = 0; i < ST; ++i) A2[i] *= SEQ_LOG2E;
+    for (int i = 0; i < ST; ++i) A2[i] = scan_decay(A2[i]);
     const float bias = a.bias ? a.bias[L.d] : 0.f;
     const ScanWalk w = scan_walk(a.clips, c0);
     const bool dead = w.s < 0 || w.s >= n || seq_start(a.clips, w.s) >= c0;        // nothing flows out of the chunk
@@ -570,7 +577,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a) {
     for (int m = 0; m < ST; ++m) g[m] = dA[m] = 0.f;
     scan_load(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
-    for (int i = 0; i < ST; ++i) A2[i] *= SEQ_LOG2E;
+    for (int i = 0; i < ST; ++i) A2[i] = scan_decay(A2[i]);
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
     auto entry = [&](int s) {                                     // the gradient of the state behind clip s
 #pragma unroll
@@ -820,7 +827,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
     float A2[4];
     step_load4<float, VEC>(a.A + (size_t)L.d * N, L.j, N, A2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A2[i] *= SEQ_LOG2E;
+    for (int i = 0; i < 4; ++i) A2[i] = scan_decay(A2[i]);
     const float bias = a.bias ? a.bias[L.d] : 0.f, Dd = a.D ? a.D[L.d] : 0.f;
     for (int64_t s0 = blockIdx.y * 4; s0 < a.rows; s0 += gridDim.y * 4) {
         const int64_t mine = min(s0 + L.q, (int64_t)a.rows - 1);           // the clip whose step and output this lane forms

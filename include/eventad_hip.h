@@ -539,7 +539,8 @@ int eventad_causal_conv_step(const void* x, int64_t ldx, const float* w, const f
                              void* y, int64_t ldy, int clips, int channels, int taps, int act, int dtype, void* stream);
 /* s_t = delta_t + delta_bias, through log(1 + exp(.)) if softplus = 1;  h_t = exp(s_t A) h_{t-1} + s_t u_t B_t;
  * y_t = (sum_n C_t[n] h_t[n] + D u_t) * (z ? z_t sigmoid(z_t) : 1).  u, delta, z, y [rows,channels], B, C [rows,n_state]
- * (ldb, ldc >= n_state), A f32[channels,n_state], D, delta_bias f32[channels], n_state 1..64; z, D, delta_bias nullable.
+ * (ldb, ldc >= n_state), A f32[channels,n_state] (-inf counts as -2.36e38: a state that forgets at once), D, delta_bias
+ * f32[channels], n_state 1..64; z, D, delta_bias nullable.
  * state / final_state f32[clips,channels,n_state] (nullable): h in front of each clip's first row / behind its last.
  * checkpoint (nullable, 16-byte aligned): eventad_selective_scan_checkpoint() bytes that the gradient of this call reads. */
 int eventad_selective_scan_workspace(int64_t rows, int channels, int n_state, int backward, int64_t* bytes);

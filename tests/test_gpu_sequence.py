@@ -905,3 +905,28 @@ def test_rms_norm_fp8_of_tiny_rows(S, dtype, channels):
     q, scale = S.rms_norm_fp8(x.cuda(), w.cuda())
     assert torch.equal(q.double().cpu(), want["q"])
     close("scale", scale, want["scale"][0], (channels / 16 + 28) * want["scale"][0])
+
+
+@pytest.mark.parametrize("rows,channels,N,kind", [(200, 9, 3, "tiles"), (140, 67, 7, "gaps"), (400, 20, 16, "empties"), (70, 5, 16, "singles"), (333, 8, 24, "three"), (131, 18, 64, "tiles"),
+                                                  (1300, 65, 4, "one"), (1300, 6, 16, "three")])
+def test_scan_of_states_that_forget_at_once(S, rows, channels, N, kind):
+    """A of -inf, or so low that its multiple leaves float32, wherever clips and chunks end: exp(s A) = 0.  The restatement, which
+    takes finite numbers only, gets -1e9, for which exp(s A) is 0 in 64 bits too."""
+    gen, b = torch.Generator().manual_seed(rows + N), bounds_of(kind, rows)
+    a = scan_inputs(gen, rows, channels, N, torch.float32, 1 if b is None else len(b) - 1)
+    pick = torch.randint(0, 3, (channels, N), generator=gen).cuda()
+    pick[0] = 1
+    a["A"] = torch.where(pick == 0, a["A"], torch.full_like(a["A"], -1e9))
+    dy, df = rnd(gen, rows, channels), torch.randn_like(a["state"])
+    want = R.scan(clip_start=b, dy=dy, dfinal=df, **a)
+    a["A"] = torch.where(pick == 1, torch.full_like(a["A"], float("-inf")), torch.where(pick == 2, torch.full_like(a["A"], -3e38), a["A"]))
+    L = {k: leaf(t) for k, t in a.items()}
+    y, f = S.selective_scan(clip_start=starts_of(b), return_state=True, **L)
+    close("y", y, *want["y"])
+    close("final", f, *want["final"])
+    for k, g in zip(L, torch.autograd.grad([y, f], list(L.values()), [dy, df])):
+        close("d" + k, g, *want[k])
+    with torch.no_grad():
+        one = {k: (t if k in ("A", "D", "delta_bias") else t[:1]) for k, t in a.items()}
+        want = R.scan(**dict(one, A=one["A"].clamp(min=-1e9)))
+        close("y", S.selective_scan_step(**dict(one, state=one["state"].clone())), *want["y"])
