@@ -251,7 +251,7 @@ def causal_conv_step(x, weight, state, bias=None, activation="silu", state_out=N
     """One row per clip: x [clips, channels], state [clips, taps - 1, channels] contiguous.  The state is moved on in place, or
     -- state_out given, a contiguous tensor like it that does not overlap it -- written there and left as it was.  -> y [clips,
     channels]."""
-    if _needs_grad(x, weight, state, bias):
+    if _needs_grad(x, weight, state, bias, state_out):
         _fail("the single-token form has no gradient: use causal_conv, or torch.no_grad()")
     index = _device(x)
     if _elsewhere(index):
@@ -369,7 +369,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     """One row per clip: u, delta, z [clips, channels], B, C [clips, states], state float32 [clips, channels, states] contiguous.
     The state is moved on in place, or -- state_out given, a contiguous tensor like it that does not overlap it -- written there
     and left as it was.  -> y [clips, channels]."""
-    if _needs_grad(u, delta, A, B, C, state, D, z, delta_bias):
+    if _needs_grad(u, delta, A, B, C, state, D, z, delta_bias, state_out):
         _fail("the single-token form has no gradient: use selective_scan, or torch.no_grad()")
     index = _device(u)
     if _elsewhere(index):

@@ -114,3 +114,16 @@ def test_tracers_are_refused(calls, pending):
             with pytest.raises(RuntimeError, match="recorded by torch.jit.trace or make_fx"):
                 record()
     assert not calls
+
+
+def test_state_out_that_needs_a_gradient_is_refused(calls):
+    """Nothing may be written into a leaf, or into a tensor of a graph, behind autograd's back."""
+    for name, tensors, f in every_form():
+        if name.endswith("_step"):
+            out = torch.zeros_like(tensors["state"], requires_grad=True)
+            for t in (out, out * 1.0):
+                with pytest.raises(RuntimeError, match="has no gradient"):
+                    f(state_out=t, **tensors)
+            with torch.no_grad():
+                f(state_out=out, **tensors)
+    assert len(calls) == 2
