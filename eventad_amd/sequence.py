@@ -20,7 +20,6 @@ import functools
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from ._lib import NativeError, load
 
@@ -172,6 +171,29 @@ def _state_out(state, out):
     return out
 
 
+class _Final(torch.autograd.Function):
+    """Gradients as they are; an error where something is differentiated through them."""
+    @staticmethod
+    def forward(ctx, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _fail("gradients are not differentiable again")
+
+
+def _once(backward):
+    """For a backward pass with a graph of its own pending (create_graph): torch's once_differentiable, but its error comes whether or not
+    the incoming gradient needs one, as these gradients depend on the saved inputs too."""
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        return _Final.apply(*(g if g is None else g.detach().requires_grad_() for g in out))
+    return run
+
+
 # ---------------------------------------------------------------------------------------------------- causal convolution
 def _conv_args(x, weight, bias, state, activation, clips, index):
     if activation not in _ACT:
@@ -208,7 +230,7 @@ class _ConvFn(torch.autograd.Function):
         return _conv_fwd(x, ldx, w, bias, starts, clips, state, act, want_state)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dfinal):
         x, w, bias, state, starts = ctx.saved_tensors
         index = _device(x)
@@ -314,7 +336,7 @@ class _ScanFn(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dfinal):
         *t, starts, ckpt = ctx.saved_tensors
         index = _device(t[0])
@@ -424,7 +446,7 @@ class _NormFn(torch.autograd.Function):
         return y, total
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dtotal):
         h, weight = ctx.saved_tensors
         index = _device(h)

@@ -127,3 +127,20 @@ def test_state_out_that_needs_a_gradient_is_refused(calls):
             with torch.no_grad():
                 f(state_out=out, **tensors)
     assert len(calls) == 2
+
+
+@pytest.mark.parametrize("op", ["conv", "scan", "norm"])
+def test_differentiating_twice_is_an_error_and_never_a_silent_zero(calls, op):
+    out, leaves = run(op)
+    loss = sum(o.sum() for o in out)
+    plain = torch.autograd.grad(loss, leaves, retain_graph=True)
+    grads = torch.autograd.grad(loss, leaves, create_graph=True)                # by itself it may be asked for
+    assert all(g.requires_grad for g in grads) and not any(g.requires_grad for g in plain)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        (loss + sum(g.sum() for g in grads)).backward()
+    for t in leaves:
+        t.grad = None
+    out, leaves = run(op)
+    sum(o.sum() for o in out).backward(create_graph=True)
+    with torch.no_grad():
+        torch.nn.utils.clip_grad_norm_(leaves, 1.0)
