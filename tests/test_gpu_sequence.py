@@ -930,3 +930,61 @@ def test_scan_of_states_that_forget_at_once(S, rows, channels, N, kind):
         one = {k: (t if k in ("A", "D", "delta_bias") else t[:1]) for k, t in a.items()}
         want = R.scan(**dict(one, A=one["A"].clamp(min=-1e9)))
         close("y", S.selective_scan_step(**dict(one, state=one["state"].clone())), *want["y"])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("channels,rows,bounds,bad", [(8, 40, [0, 5, 11, 13, 16, 27, 40], 2), (24, 700, [3, 130, 333, 340, 680, 690], 1),
+                                                      (70, 3000, [0, 1000, 1011, 1500, 3000], 1)])
+@pytest.mark.parametrize("N", [1, 4, 7, 24, 64])
+def test_a_clip_does_not_spoil_its_neighbours_with_any_number_of_states(S, value, channels, rows, bounds, bad, N):
+    gen, clips = torch.Generator().manual_seed(rows + N), len(bounds) - 1
+    starts, row = starts_of(bounds), torch.arange(rows, device="cuda")
+    hit = (row >= bounds[bad]) & (row < bounds[bad + 1])
+    others = [i for i in range(clips) if i != bad]
+    a, dy, dh = scan_inputs(gen, rows, channels, N, torch.float32, clips), rnd(gen, rows, channels), rnd(gen, clips, channels, N)
+    per_row, runs = ("u", "delta", "B", "C", "z"), []
+    for spoil in (False, True):
+        t, g, f = {k: v.clone() for k, v in a.items()}, dy.clone(), dh.clone()
+        if spoil:
+            for v in [t[k] for k in per_row] + [g]:
+                v[hit] = value
+            t["state"][bad], f[bad] = value, value
+        L = {k: leaf(v) for k, v in t.items()}
+        y, h = S.selective_scan(clip_start=starts, return_state=True, **L)
+        *d, dstate = torch.autograd.grad([y, h], [L[k] for k in per_row] + [L["state"]], [g, f])
+        runs.append([v[~hit] for v in (y, *d)] + [v[others] for v in (h, dstate)])
+    for i, (p, q) in enumerate(zip(*runs)):
+        assert torch.equal(p, q), i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_captured_single_tokens_move_their_states_on(S, dtype):
+    """A loop over single tokens, captured once and replayed: states and outputs as those of eager calls, step for step."""
+    gen, clips, ch, N, dt = torch.Generator().manual_seed(31), 5, 48, 16, DTYPES[dtype]
+    w, nw, a = rnd(gen, ch, 4), rnd(gen, ch) + 1.0, scan_inputs(gen, clips, ch, N, dt, clips)
+    h0 = a.pop("state")
+    x, conv, scan = a["u"].clone(), rnd(gen, clips, 3, ch, dtype=dt), h0.clone()
+    c2, s2 = conv.clone(), scan.clone()
+
+    def once(x, conv, scan):
+        with torch.no_grad():
+            n, t = S.rms_norm(x, nw, x)
+            v = S.causal_conv_step(n, w, conv)
+            return S.selective_scan_step(v, a["delta"], a["A"], a["B"], a["C"], scan, a["D"], a["z"], a["delta_bias"]), t, *S.rms_norm_fp8(v, nw)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once(x, conv.clone(), scan.clone())
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once(x, conv, scan)
+    conv.copy_(c2)
+    scan.copy_(s2)
+    for it in range(6):
+        x.copy_(rnd(gen, clips, ch, dtype=dt))
+        want = once(x, c2, s2)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip((*out, conv, scan), (*want, c2, s2)):
+            assert torch.equal(p.float(), q.float()), it
