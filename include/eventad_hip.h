@@ -515,7 +515,10 @@ int eventad_incr_pool0(const float* y2, const float* map_nhwc, int map_h, int ma
  * above rows as rows.  Offsets that decrease give wrong numbers and may leave states unwritten; nothing outside the arrays
  * is accessed.  Rows of no clip are neither read into a result nor counted in a gradient; their outputs and gradients are
  * written as zeros.
- * A launch that would need more than 2^32 threads (rows x channels beyond 3e10) is refused with EVENTAD_ERR_TOO_LARGE.
+ * A launch that would need more than 2^32 threads is refused with EVENTAD_ERR_TOO_LARGE: the norm starts 16 to 256 for a row (one
+ * for each 16 bytes of it, rounded up to 16, 32, 64 or 256; 16 up to 16 channels), so it takes 2.6e8 short rows or 1.6e7 long
+ * ones; the convolution of one row per clip starts one for four channels (for one, where rows do not start on a border of
+ * four) and takes 4.2e9 threads, its row form 1.3e11 elements; the scan is not limited by this.
  * Outputs must not overlap inputs unless it says so.  Results are reproducible bit for bit (no float atomics).
  * workspace: 16-byte aligned device memory of at least the bytes that the *_workspace function of the same shape reports
  * (host call, nothing is launched); its contents need not survive the call, and calls that may run at the same time need

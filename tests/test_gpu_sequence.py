@@ -988,3 +988,24 @@ def test_captured_single_tokens_move_their_states_on(S, dtype):
         torch.cuda.synchronize()
         for p, q in zip((*out, conv, scan), (*want, c2, s2)):
             assert torch.equal(p.float(), q.float()), it
+
+
+def test_events_of_a_batch_as_packed_rows(S):
+    """Offsets from a batch's index per event: its clips by one call are its clips one by one."""
+    from eventad_amd import synthetic
+    b = synthetic.make_batch(64, 64, 3000, 3, with_image=False).to("cuda")
+    gen = torch.Generator().manual_seed(1)
+    clip_start = torch.searchsorted(b.batch, torch.arange(b.num_graphs + 1, device=b.batch.device)).int()
+    x = torch.cat([b.x.float().reshape(len(b.batch), -1), b.pos.float()], 1) @ rnd(gen, b.x.float().reshape(len(b.batch), -1).shape[1] + b.pos.shape[1], 24)
+    w, A, B, C = rnd(gen, 24, 4), -torch.exp(rnd(gen, 24, 16)), x[:, :16], x[:, 8:]
+    v = S.causal_conv(x, w, clip_start=clip_start)
+    y = S.selective_scan(v, x, A, B, C, clip_start=clip_start)
+    at = clip_start.tolist()
+    assert at[-1] == len(b.batch)
+    for lo, hi in zip(at, at[1:]):
+        assert bool((b.batch[lo:hi] == b.batch[lo]).all())
+        one = S.causal_conv(x[lo:hi], w)
+        assert torch.equal(v[lo:hi], one)
+        alone = S.selective_scan(one, x[lo:hi], A, B[lo:hi], C[lo:hi])
+        # other chunks: float32 sums over up to 3000 rows joined elsewhere
+        assert float((y[lo:hi] - alone).abs().max()) <= 1e-4 * float(alone.abs().max())

@@ -144,3 +144,28 @@ def test_differentiating_twice_is_an_error_and_never_a_silent_zero(calls, op):
     sum(o.sum() for o in out).backward(create_graph=True)
     with torch.no_grad():
         torch.nn.utils.clip_grad_norm_(leaves, 1.0)
+
+
+def batch_of(sizes):
+    from eventad_amd.batch import EventBatch
+    clip = lambda n: dict(x=torch.zeros(n, 1), pos=torch.rand(n, 2), t=torch.zeros(n), bbox=torch.zeros(1, 5), bbox0=torch.zeros(1, 5), width=64, height=64, time_window=1)
+    return EventBatch.from_clips([clip(n) for n in sizes])
+
+
+def test_offsets_from_a_batch_of_events():
+    """Made from the index per event, empty clips at the ends and in between included."""
+    for sizes in ([3, 5, 1], [0, 4, 0, 0, 2, 0], [7], [0, 0]):
+        b = batch_of(sizes)
+        clip_start = torch.searchsorted(b.batch, torch.arange(b.num_graphs + 1, device=b.batch.device)).int()
+        assert clip_start.tolist() == [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+
+
+def test_launches_past_the_stated_sizes_are_refused():
+    import ctypes
+    from eventad_amd import _lib
+    lib, buf = _lib.load(), ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)     # only ever compared with NULL
+    norm = lambda rows, ch: lib.eventad_rms_norm_fwd(buf, ch, None, 0, buf, None, 0, buf, ch, rows, ch, 1e-6, 0, None)
+    for rows, ch in ((268435441, 1), (268435441, 64), (16777216, 4096)):
+        assert norm(rows, ch) == -3
+    step = lambda clips, ch: lib.eventad_causal_conv_step(buf, ch, buf, None, buf, buf, buf, ch, clips, ch, 4, 1, 0, None)
+    assert step(4294967296 // 31 + 1, 31) == -3 and step(4294967296 // 8 + 1, 32) == -3
