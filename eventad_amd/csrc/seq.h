@@ -100,6 +100,7 @@ __device__ __forceinline__ int seq_find(const SeqClips& c, int row) {
     return lo;
 }
 
+#define SEQ_MOST_CLIPS ((1 << 30) - 1)         // (seq_find adds two of their numbers)
 #define SEQ_MOST_THREADS 0xffffff00LL          // of one launch (threads are numbered in 32 bits)
 
 static inline bool seq_aligned(const void* p, int64_t row_bytes) { return (((uintptr_t)p | (uintptr_t)row_bytes) & 15) == 0; }

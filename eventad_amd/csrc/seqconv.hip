@@ -501,7 +501,7 @@ extern "C" int eventad_causal_conv_workspace(int64_t rows, int channels, int tap
 extern "C" int eventad_causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bias, const int32_t* clip_start,
                                        int clips, const void* state, void* final_state, void* y, int64_t ldy, int64_t rows,
                                        int channels, int taps, int act, int dtype, void* stream) {
-    if (!conv_shape_ok(rows, channels, taps, dtype) || !w || clips < 1 || (!clip_start && clips != 1) || act < 0 || act > 1 ||
+    if (!conv_shape_ok(rows, channels, taps, dtype) || !w || clips < 1 || clips > SEQ_MOST_CLIPS || (!clip_start && clips != 1) || act < 0 || act > 1 ||
         (rows && (!x || !y || ldx < channels || ldy < channels))) return EVAD_ERR_ARG;
     ConvArgs a = {};
     a.clips = SeqClips{clip_start, clips, (int)rows};
@@ -520,7 +520,7 @@ extern "C" int eventad_causal_conv_bwd(const void* x, int64_t ldx, const float* 
                                        int64_t rows, int channels, int taps, int act, int dtype, void* stream) {
     int64_t need = 0;
     if (eventad_causal_conv_workspace(rows, channels, taps, &need) != EVAD_OK) return EVAD_ERR_ARG;
-    if (!conv_shape_ok(rows, channels, taps, dtype) || !w || clips < 1 || (!clip_start && clips != 1) || act < 0 || act > 1 ||
+    if (!conv_shape_ok(rows, channels, taps, dtype) || !w || clips < 1 || clips > SEQ_MOST_CLIPS || (!clip_start && clips != 1) || act < 0 || act > 1 ||
         !dparams || !workspace || workspace_bytes < need || (rows && (!x || !dy || !dx || ldx < channels || lddy < channels || lddx < channels)))
         return EVAD_ERR_ARG;
     ConvArgs a = {};

@@ -1002,7 +1002,7 @@ extern "C" int eventad_selective_scan_fwd(const void* u, int64_t ldu, const void
     ScanArgs a = {};
     int64_t need = 0;
     if (!scan_common(a, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, delta_bias, rows, channels, n_state, softplus, dtype) ||
-        clips < 1 || (!clip_start && clips != 1) || (rows && (!y || !scan_ld_ok(ldy, channels))) || ((uintptr_t)checkpoint & 15) ||
+        clips < 1 || clips > SEQ_MOST_CLIPS || (!clip_start && clips != 1) || (rows && (!y || !scan_ld_ok(ldy, channels))) || ((uintptr_t)checkpoint & 15) ||
         eventad_selective_scan_workspace(rows, channels, n_state, 0, &need) != EVAD_OK || !workspace || workspace_bytes < need ||
         ((uintptr_t)workspace & 15)) return EVAD_ERR_ARG;
     a.clips = SeqClips{clip_start, clips, (int)rows};
@@ -1030,7 +1030,7 @@ extern "C" int eventad_selective_scan_bwd(const void* u, int64_t ldu, const void
     ScanArgs a = {};
     int64_t need = 0;
     if (!scan_common(a, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, delta_bias, rows, channels, n_state, softplus, dtype) ||
-        clips < 1 || (!clip_start && clips != 1) || !dparams || ((uintptr_t)checkpoint & 15) ||
+        clips < 1 || clips > SEQ_MOST_CLIPS || (!clip_start && clips != 1) || !dparams || ((uintptr_t)checkpoint & 15) ||
         (rows && (!dy || !du || !ddelta || !dB || !dC || !checkpoint || !scan_ld_ok(lddy, channels) || !scan_ld_ok(lddu, channels) ||
                   !scan_ld_ok(lddd, channels) || lddb < n_state || lddc < n_state || (z && (!dz || !scan_ld_ok(lddz, channels))))) ||
         eventad_selective_scan_workspace(rows, channels, n_state, 1, &need) != EVAD_OK || !workspace || workspace_bytes < need ||

@@ -7,7 +7,8 @@ Rows are packed: activations are [rows, channels], clip s owns rows clip_start[s
 not decreasing; below 0 counts as 0, above rows as rows; None = all rows are one clip); rows of no clip give zeros and take
 no part in a gradient.
 Activations are float32, bfloat16 or float16, all of one call alike; parameters and scan states are float32.  A row may be a
-slice of a wider array (any row stride); an array whose channels are not adjacent is copied first.
+slice of a wider array (any row stride); an array whose channels are not adjacent is copied first.  Up to 2^20 channels (the
+norm: 2^24), 2^31 rows and 2^30 clips.
 
 Every function launches on the current stream of its tensors' device, waits for nothing, and can be captured into a graph;
 workspaces come from torch's allocator per call, so captured graphs do not share one.  torch.jit.trace and make_fx cannot record
@@ -29,7 +30,8 @@ _F32, _I32 = torch.float32, torch.int32
 _Tensor = torch.Tensor
 _tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 MAX_TAPS, MAX_STATE = 8, 64
-_MAX_LD = 1 << 24               # row strides above this are taken by copying the array
+_MAX_LD = 1 << 24               # row strides above this are taken by copying the array; no more channels than that
+_MAX_CLIPS = (1 << 30) - 1      # (the library numbers clips, and bisects their offsets, in 32 bits)
 
 # A single-token call is bound by this file: the checks below compare identities and device numbers, read each attribute once
 # and pass plain integers to the library.
@@ -92,6 +94,8 @@ def _rows(name, t, rows, width, dtype, index):
     ld, step = t.stride()
     if step == 1 and m <= ld <= _MAX_LD:
         return t, ld
+    if m > _MAX_LD:
+        _fail("%s has %d channels, more than 2^24", name, m)
     if n <= 1 and (step == 1 or m <= 1):                         # (one row: any stride)
         return t, m
     return t.contiguous(), m
@@ -123,8 +127,8 @@ def _clips(clip_start, index):
     if clip_start is None:
         return None, 1
     if not isinstance(clip_start, torch.Tensor) or clip_start.dtype is not _I32 or clip_start.get_device() != index or \
-            clip_start.dim() != 1 or clip_start.numel() < 2:
-        _fail("clip_start must be int32[clips + 1] on GPU %d", index)
+            clip_start.dim() != 1 or not 2 <= clip_start.numel() <= _MAX_CLIPS + 1:
+        _fail("clip_start must be int32[clips + 1] on GPU %d, with 1..%d clips", index, _MAX_CLIPS)
     return clip_start.contiguous(), clip_start.numel() - 1
 
 
@@ -284,6 +288,8 @@ def causal_conv_step(x, weight, state, bias=None, activation="silu", state_out=N
         _fail("state must be contiguous, of x's type, [clips, taps - 1, channels]")
     out = _state_out(state, state_out)
     clips, D = x.shape
+    if clips > _MAX_CLIPS:
+        _fail("%d clips, more than %d", clips, _MAX_CLIPS)
     y = x.new_empty((clips, D))
     _call("eventad_causal_conv_step", x.data_ptr(), ldx, weight.data_ptr(), _p(bias), state.data_ptr(), out.data_ptr(), y.data_ptr(), D, clips,
           D, taps, _ACT[activation], _DTYPE[x.dtype], _stream(index))
@@ -403,6 +409,8 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
         _fail("state must be contiguous float32 [clips, channels, states]")
     out = _state_out(state, state_out)
     clips, ch = u.shape
+    if clips > _MAX_CLIPS:
+        _fail("%d clips, more than %d", clips, _MAX_CLIPS)
     y = u.new_empty((clips, ch))
     _call("eventad_selective_scan_step", u.data_ptr(), ldu, delta.data_ptr(), ldd, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc, _p(D),
           _p(z), ldz, _p(delta_bias), state.data_ptr(), out.data_ptr(), y.data_ptr(), ch, clips, ch, A.shape[1], 1 if delta_softplus else 0,

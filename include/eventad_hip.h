@@ -510,7 +510,8 @@ int eventad_incr_pool0(const float* y2, const float* map_nhwc, int map_h, int ma
  * pass and the event-by-event update of groups (B)-(K), for a recurrence over the rows themselves).
  * Arrays of activations are [rows, channels] with a row stride in elements (channels <= ld* <= 2^24; adjacent channels are
  * adjacent in memory), of type dtype = 0 float32, 1 bfloat16, 2 float16, all of one call alike; parameters and scan states are
- * float32, sums are formed in float32.  Rows are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1, clip_start
+ * float32, sums are formed in float32.  At most 2^20 channels (the norm: 2^24), 2^31 - 256 rows and 2^30 - 1 clips.
+ * Rows are packed: clip s owns rows clip_start[s] .. clip_start[s+1]-1, clip_start
  * i32[clips+1] on the device, not decreasing (NULL with clips = 1: all rows are one clip); offsets below 0 count as 0 and ones
  * above rows as rows.  Offsets that decrease give wrong numbers and may leave states unwritten; nothing outside the arrays
  * is accessed.  Rows of no clip are neither read into a result nor counted in a gradient; their outputs and gradients are

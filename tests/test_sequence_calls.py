@@ -169,3 +169,34 @@ def test_launches_past_the_stated_sizes_are_refused():
         assert norm(rows, ch) == -3
     step = lambda clips, ch: lib.eventad_causal_conv_step(buf, ch, buf, None, buf, buf, buf, ch, clips, ch, 4, 1, 0, None)
     assert step(4294967296 // 31 + 1, 31) == -3 and step(4294967296 // 8 + 1, 32) == -3
+
+
+def test_sizes_past_32_bits_are_refused_and_not_cut_short(calls):
+    """ctypes passes the low 32 bits of an int.  The arrays are one element each, repeated."""
+    r, big = lambda *s: torch.zeros(1).expand(*s), (1 << 32) + 2
+    clips = torch.zeros(1, dtype=torch.int32).expand(big + 1)
+    x, w, A, B = r(6, CH), r(CH, TAPS), r(CH, N), r(6, N)
+    for f in (lambda: S.rms_norm(r(1, big), r(big)), lambda: S.rms_norm_fp8(r(1, big), r(big)), lambda: S.causal_conv(r(1, big), r(big, TAPS)),
+              lambda: S.causal_conv(x, w, clip_start=clips), lambda: S.selective_scan(x, x, A, B, B, clip_start=clips)):
+        with pytest.raises(RuntimeError, match="more than 2\\^24|1\\.\\.1073741823 clips"):
+            f()
+
+    many = 1 << 30                                               # rows of a single-token call; memory that nobody touches
+    u, h = torch.empty(many, 1, dtype=torch.bfloat16), torch.empty(many, 1, 1)
+    for f in (lambda: S.causal_conv_step(u, r(1, 1), torch.empty(many, 0, 1, dtype=torch.bfloat16)), lambda: S.selective_scan_step(u, u, r(1, 1), u, u, h)):
+        with pytest.raises(RuntimeError, match="1073741824 clips"):
+            f()
+    assert not calls
+
+
+def test_more_clips_than_can_be_bisected_are_refused_by_the_library():
+    import ctypes
+    from eventad_amd import _lib
+    lib, buf = _lib.load(), ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)     # only ever compared with NULL
+    for clips in (1 << 30, (1 << 31) - 1):
+        assert lib.eventad_causal_conv_fwd(buf, 8, buf, None, buf, clips, None, None, buf, 8, 4, 8, 4, 1, 0, None) == -1
+        assert lib.eventad_causal_conv_bwd(buf, 8, buf, None, buf, clips, None, buf, 8, None, buf, 8, None, buf, buf, 1 << 20, 4, 8, 4, 1, 0, None) == -1
+        assert lib.eventad_selective_scan_fwd(buf, 8, buf, 8, buf, buf, 16, buf, 16, None, None, 0, None, buf, clips, None, None, buf, 8, None, buf, 1 << 16, 4, 8, 16, 1,
+                                              0, None) == -1
+        assert lib.eventad_selective_scan_bwd(buf, 8, buf, 8, buf, buf, 16, buf, 16, None, None, 0, None, buf, clips, None, buf, buf, 8, None, buf, 8, buf, 8, buf, 16,
+                                              buf, 16, None, 0, None, buf, buf, 1 << 20, 4, 8, 16, 1, 0, None) == -1
