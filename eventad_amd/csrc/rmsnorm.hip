@@ -27,7 +27,8 @@ struct NormArgs {
 };
 
 // A piece of a row: V elements from column c on.  U: rows start anywhere and end inside a piece; whole pieces are still one access
-// each (global memory takes any address), the last one goes element by element.
+// each (global memory takes any address), the last one goes element by element.  (12,000 x 8191 bf16: forward 193 us, with gradient 600; x 8192
+// 150 and 294.  The gradient then takes 258 registers, one wave per SIMD.)
 template <typename T, int V> struct NormAny { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T, int V, bool U> __device__ __forceinline__ typename SeqRaw<T, V>::type norm_raw(const T* __restrict__ row, int c, int D) {
     if constexpr (!U) return seq_raw<T, V>(row + min(c, D - V));
@@ -465,7 +466,9 @@ template <int WHAT, typename T, int V, bool U, int LANES, int ITERS, bool LOOP> 
 // pieces per lane (65,536 x 1024: 101 us, gradient 109; with four waves 103 and 175).  Up to four pieces the gradient, which
 // keeps dw and the next row in registers too, still does better with a wave per row (65,536 x 1280: 153 us against 184), the
 // forward forms with four waves (100,000 x 2048: 276 us against 302).  From there on four waves (16,384 x 4096: 103 us, a wave 117), up to
-// eight pieces per lane (12,000 x 8192 f32: 290 us, gradient 338, read again for every pass over the row 369 and 438).
+// eight pieces per lane (12,000 x 8192 f32: 288 us, with gradient 564, read again for every pass over the row 360 and 762; x 12,288 bf16
+// 228 and 513 against 269 and 710).  The gradient's eight pieces of eight 16-bit elements take 390 registers, one wave per SIMD,
+// and unaligned ones all 512 and scratch beside them; that is still the faster side (x 12,287 bf16 with gradient: 889 us against 1295).
 template <int WHAT, typename T, int V, bool U> static int norm_launch2(const NormArgs& a, int groups, hipStream_t st) {
     const int pieces = (a.channels + V - 1) / V;
     if (pieces <= 16) return norm_launch3<WHAT, T, V, U, 16, 1, false>(a, groups, st);

@@ -7,7 +7,7 @@
 // d_t = dy_t act'(pre_t):  dx_t = sum_k w[:,k] d_{t+(K-1)-k} inside the clip,  dw[:,k] = sum_t d_t x_{t-(K-1)+k},
 // dbias = sum_t d_t.
 //
-// All of it is bound by bytes (2K + 4 operations per element that is read and written once): K = 4, 400,000 x 256 f32 819 MB in
+// Up to four taps it is bound by bytes (2K + 4 operations per element that is read and written once): K = 4, 400,000 x 256 f32 819 MB in
 // 153 us (5.4 TB/s), its gradient 1229 MB in 280 us (4.4 TB/s; a copy of 4 GiB runs at 4.75), 17,920 x 1024 f16 73 MB in 19 us.  A thread owns four adjacent
 // channels (one, where rows are not aligned to four) of a chunk of rows and slides down it with the K-1 inputs before the current
 // row in registers, so a row is read once plus (K-1) / chunk for the chunk's start.  Rows go by in groups of four, requested
@@ -37,7 +37,9 @@ struct ConvArgs {
 };
 
 // The kernels are built for K = 2, 3, 4 and 8 taps; K = 8 serves every other number: its first K - taps window entries are zero
-// and stay out of the sums.  (Four taps, 17,920 x 1024 bf16: 21 us and 61 with the gradient; by the kernels for eight 31 and 118.)
+// and stay out of the sums.  (17,920 x 1024 bf16, forward and with the gradient: four taps 18 and 60 us, by the kernels for eight 31 and
+// 118; five 26 and 119, six 32 and 134, eight 41 and 158.  The gradient's 244 to 295 registers leave one or two waves per SIMD, and it
+// reads seven rows behind every chunk.)
 template <int K> __device__ __forceinline__ int conv_skip(const ConvArgs& a) { return K == 8 ? K - a.taps : 0; }
 
 template <bool WAVE> __device__ __forceinline__ int conv_same(int v) { return WAVE ? __builtin_amdgcn_readfirstlane(v) : v; }
@@ -203,7 +205,8 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a) {
 }
 
 // One pass down the chunk and the K-1 rows behind it: d_p is formed once per row, and a row's dx is complete K-1 rows later.
-// acc[k] = what position p-(K-1)+k of the clip has collected when row p is reached.
+// acc[k] = what position p-(K-1)+k of the clip has collected when row p is reached.  (Three workgroups per CU: with four taps and fewer than
+// 64 columns that spills 3 to 13 registers; 100,000 x 64 bf16 with the forward 44 us, where its bytes take 14.)
 template <typename T, int V, int K, bool WAVE>
 __global__ __launch_bounds__(256, K == 8 ? 1 : 3) void k_conv_bwd(ConvArgs a) {
     ConvLane<T, V, K, WAVE> L;

@@ -211,8 +211,8 @@ __device__ __forceinline__ ScanWalk scan_walk(const SeqClips& c, int row) {
 }
 
 // WHAT 0: outputs.  WHAT 1: the chunk's end state for the chunks behind it.  Four workgroups per CU; with 16 lanes per channel three,
-// as their staging registers would be spilled at four (16384 x 1024 x 64 bf16: 690 us against 710; with 8 lanes three cost more than the
-// spills, x 24: 322 against 311).
+// as their staging registers would be spilled at four (16384 x 1024 x 64 bf16: 690 us against 710).  With fewer lanes three cost more than
+// the spills of the first pass (two registers with 4 lanes, six with 8): x 16 160 us against 153, x 24 315 against 307.
 //
 // A chunk is walked in pieces, the rows that a tile and a clip have in common.  A piece runs through all 16 rows of its
 // tile as straight-line code, with step and input 0 for rows outside it, which leave the state as it is: the usual tile is one
@@ -806,8 +806,8 @@ __global__ __launch_bounds__(256) void k_scan_bc(const float* __restrict__ part,
 // 5.7 TB/s; 6 x 256 x 16: 3.6 us).  A lane owns four states of a channel (16 bytes each way) and goes over four clips at a
 // time, so that four states are requested before the first is used and the lanes of a quad form the step and the gate of one
 // clip each (one clip at a time: 100 us).  VEC: rows of A, B, C and the states are whole and aligned groups of four; otherwise
-// they are read entry by entry (2048 x 1024 x 16 121 us instead of 48).  state_out may be the state itself: a lane reads its
-// entries before it writes them and nobody else needs them.
+// they are read entry by entry, the states too (2048 x 1024 x 16 with B and C off a border of four: 147 us instead of 55).
+// state_out may be the state itself: a lane reads its entries before it writes them and nobody else needs them.
 template <typename T, bool VEC> __device__ __forceinline__ void step_load4(const T* __restrict__ row, int j, int N, float (&v)[4]) {
     if constexpr (VEC) {
         typename SeqVec<T, 4>::type w = {};

@@ -378,7 +378,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
 
     Every clip's end inside a group of 16 rows costs that group another turn: a batch whose clips are all a row or two long is
     better served by selective_scan_step.  With a gradient pending, the call keeps 2 x channels x (states, rounded up to a power of
-    two from 4 to 64) bytes per 4 rows."""
+    two from 4 to 64) bytes per 4 rows, and the backward pass takes 2 bytes per row and channel up to 16 states (8 up to 32, 32 up to
+    64) for as long as it runs."""
     index = _device(u)
     if _elsewhere(index):
         with torch.cuda.device(index):

@@ -1009,3 +1009,24 @@ def test_events_of_a_batch_as_packed_rows(S):
         alone = S.selective_scan(one, x[lo:hi], A, B[lo:hi], C[lo:hi])
         # other chunks: float32 sums over up to 3000 rows joined elsewhere
         assert float((y[lo:hi] - alone).abs().max()) <= 1e-4 * float(alone.abs().max())
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_block_has_the_same_gradients(S, reentrant):
+    """torch.utils.checkpoint forms a block's saved tensors again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    gen = torch.Generator().manual_seed(41)
+    p = {k: leaf(v) for k, v in block_weights(gen, 24, 40, 16, 4, 5).items()}
+    x, res, b = rnd(gen, 137, 24), rnd(gen, 137, 24), starts_of([0, 50, 50, 130])
+    dy, dr = rnd(gen, 137, 24), rnd(gen, 137, 24)
+    results = []
+    for again in (False, True):
+        L = [leaf(x), leaf(res)]
+        f = lambda x, res, *w: block(S, dict(zip(p, w)), x, res, b)[:2]
+        out = checkpoint(f, *L, *p.values(), use_reentrant=reentrant) if again else f(*L, *p.values())
+        for t in p.values():
+            t.grad = None
+        torch.autograd.backward(out, [dy, dr])
+        results.append([*(o.detach() for o in out), *(t.grad.clone() for t in (*L, *p.values()))])
+    for i, (s, t) in enumerate(zip(*results)):
+        assert torch.equal(s, t), i
