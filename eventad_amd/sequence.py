@@ -112,11 +112,11 @@ def _tensor(name, t, shape, dtype, index):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _gradient(g, like):
-    """An incoming gradient as an array [rows, channels] of like's type, zeros for None; with its row stride."""
+def _gradient(g, like, rows, width, index):
+    """An incoming gradient as an array [rows, width] of like's type, zeros for None; with its row stride."""
     if g is None:
         g = torch.zeros_like(like, memory_format=torch.contiguous_format)
-    return _rows("the gradient", g, like.shape[0], like.shape[1], like.dtype, like.get_device())
+    return _rows("the gradient", g, rows, width, like.dtype, index)
 
 
 def _p(t):
@@ -190,10 +190,10 @@ def _once(backward):
     """For a backward pass with a graph of its own pending (create_graph): torch's once_differentiable, but its error comes whether or not
     the incoming gradient needs one, as these gradients depend on the saved inputs too."""
     def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
         with torch.no_grad():
             out = backward(ctx, *grads)
-        if not torch.is_grad_enabled():
-            return out
         return _Final.apply(*(g if g is None else g.detach().requires_grad_() for g in out))
     return run
 
@@ -242,7 +242,7 @@ class _ConvFn(torch.autograd.Function):
             starts, clips = _clips(starts, index)
             x, ldx, w, bias, state, K = _conv_args(x, w, bias, state, None, clips, index)
             rows, D = x.shape
-            dy, ldy = _gradient(dy, x)
+            dy, ldy = _gradient(dy, x, rows, D, index)
             dfinal = _tensor("the final state's gradient", dfinal, (clips, K - 1, D), x.dtype, index)
             dx = x.new_empty((rows, D))
             dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
@@ -352,7 +352,7 @@ class _ScanFn(torch.autograd.Function):
             rows, ch = u.shape
             N = A.shape[1]
             ckpt = _tensor("the checkpoint", ckpt, (max(16, _bytes("eventad_selective_scan_checkpoint", rows, ch, N)),), torch.uint8, index)
-            dy, ldy = _gradient(dy, u)
+            dy, ldy = _gradient(dy, u, rows, ch, index)
             dfinal = _tensor("the final state's gradient", dfinal, (clips, ch, N), _F32, index)
             new = lambda n: u.new_empty((rows, n))
             du, dd, dB, dC, dz = new(ch), new(ch), new(N), new(N), new(ch) if z is not None else None
@@ -462,8 +462,8 @@ class _NormFn(torch.autograd.Function):
         with _on(index):
             h, ldh, weight, _, _, eps = _norm_args(h, weight, None, ctx.eps, index)
             rows, D = h.shape
-            dy, ldy = _gradient(dy, h)
-            dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h)
+            dy, ldy = _gradient(dy, h, rows, D, index)
+            dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h, rows, D, index)
             dh = h.new_empty((rows, D))
             dw = weight.new_empty(D)
             ws = _workspace(_bytes("eventad_rms_norm_workspace", rows, D), h)
