@@ -81,16 +81,17 @@ def _stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _rows(name, t, rows, width, dtype, index):
-    """Checks an array [rows, width] (None: any) -> it with adjacent channels, and its row stride in elements."""
+def _rows(name, t, shape, dtype, index):
+    """Checks an array [rows, channels] (shape None: any) -> it with adjacent channels, and its row stride in elements."""
     if not (t.__class__ is _Tensor or isinstance(t, _Tensor)) or t.dtype is not dtype or t.get_device() != index:
         _fail("%s must be a %s tensor on GPU %d", name, dtype, index)
-    shape = t.shape
-    if len(shape) != 2:
-        _fail("%s has %d dimensions, expected [rows, channels]", name, len(shape))
+    if shape is None:
+        shape = t.shape
+        if len(shape) != 2:
+            _fail("%s has %d dimensions, expected [rows, channels]", name, len(shape))
+    elif t.shape != shape:
+        _fail("%s has shape %s, expected %s", name, tuple(t.shape), shape)
     n, m = shape
-    if (rows is not None and n != rows) or (width is not None and m != width):
-        _fail("%s has shape %s, expected %s", name, (n, m), ("*" if rows is None else rows, "*" if width is None else width))
     ld, step = t.stride()
     if step == 1 and m <= ld <= _MAX_LD:
         return t, ld
@@ -112,11 +113,11 @@ def _tensor(name, t, shape, dtype, index):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _gradient(g, like, rows, width, index):
-    """An incoming gradient as an array [rows, width] of like's type, zeros for None; with its row stride."""
+def _gradient(g, like, shape, index):
+    """An incoming gradient as an array [rows, channels] of like's type, zeros for None; with its row stride."""
     if g is None:
         g = torch.zeros_like(like, memory_format=torch.contiguous_format)
-    return _rows("the gradient", g, rows, width, like.dtype, index)
+    return _rows("the gradient", g, shape, like.dtype, index)
 
 
 def _p(t):
@@ -204,7 +205,7 @@ def _conv_args(x, weight, bias, state, activation, clips, index):
         _fail("activation must be None or 'silu', not %r", activation)
     if x.dtype not in _DTYPE:
         _fail("x must be float32, bfloat16 or float16, not %s", x.dtype)
-    x, ldx = _rows("x", x, None, None, x.dtype, index)
+    x, ldx = _rows("x", x, None, x.dtype, index)
     D = x.shape[1]
     taps = weight.shape[1] if isinstance(weight, torch.Tensor) and weight.dim() == 2 else 0
     if D < 1 or not 1 <= taps <= MAX_TAPS:
@@ -242,7 +243,7 @@ class _ConvFn(torch.autograd.Function):
             starts, clips = _clips(starts, index)
             x, ldx, w, bias, state, K = _conv_args(x, w, bias, state, None, clips, index)
             rows, D = x.shape
-            dy, ldy = _gradient(dy, x, rows, D, index)
+            dy, ldy = _gradient(dy, x, (rows, D), index)
             dfinal = _tensor("the final state's gradient", dfinal, (clips, K - 1, D), x.dtype, index)
             dx = x.new_empty((rows, D))
             dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
@@ -303,17 +304,17 @@ def _scan_args(u, delta, A, B, C, D, z, bias, state, clips, index):
     dt = u.dtype
     if dt not in _DTYPE:
         _fail("u must be float32, bfloat16 or float16, not %s", dt)
-    u, ldu = _rows("u", u, None, None, dt, index)
-    rows, ch = u.shape
+    u, ldu = _rows("u", u, None, dt, index)
+    wide = rows, ch = u.shape
     N = A.shape[1] if isinstance(A, torch.Tensor) and A.dim() == 2 else 0
     if ch < 1 or not 1 <= N <= MAX_STATE:
         _fail("A must be [channels, states] with 1..%d states, u [rows, channels] with at least one channel", MAX_STATE)
-    delta, ldd = _rows("delta", delta, rows, ch, dt, index)
+    delta, ldd = _rows("delta", delta, wide, dt, index)
     A = _tensor("A", A, (ch, N), _F32, index)
-    B, ldb = _rows("B", B, rows, N, dt, index)
-    C, ldc = _rows("C", C, rows, N, dt, index)
+    B, ldb = _rows("B", B, (rows, N), dt, index)
+    C, ldc = _rows("C", C, (rows, N), dt, index)
     D = _tensor("D", D, (ch,), _F32, index)
-    z, ldz = (None, 0) if z is None else _rows("z", z, rows, ch, dt, index)
+    z, ldz = (None, 0) if z is None else _rows("z", z, wide, dt, index)
     bias = _tensor("delta_bias", bias, (ch,), _F32, index)
     state = _tensor("state", state, (clips, ch, N), _F32, index)
     return (u, delta, A, B, C, D, z, bias, state), (ldu, ldd, ldb, ldc, ldz)
@@ -352,7 +353,7 @@ class _ScanFn(torch.autograd.Function):
             rows, ch = u.shape
             N = A.shape[1]
             ckpt = _tensor("the checkpoint", ckpt, (max(16, _bytes("eventad_selective_scan_checkpoint", rows, ch, N)),), torch.uint8, index)
-            dy, ldy = _gradient(dy, u, rows, ch, index)
+            dy, ldy = _gradient(dy, u, (rows, ch), index)
             dfinal = _tensor("the final state's gradient", dfinal, (clips, ch, N), _F32, index)
             new = lambda n: u.new_empty((rows, n))
             du, dd, dB, dC, dz = new(ch), new(ch), new(N), new(N), new(ch) if z is not None else None
@@ -424,7 +425,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
 def _norm_args(x, weight, residual, eps, index):
     if x.dtype not in _DTYPE:
         _fail("x must be float32, bfloat16 or float16, not %s", x.dtype)
-    x, ldx = _rows("x", x, None, None, x.dtype, index)
+    x, ldx = _rows("x", x, None, x.dtype, index)
     rows, D = x.shape
     if D < 1 or weight is None:
         _fail("x must have at least one channel, and weight must be a float32 tensor")
@@ -432,7 +433,7 @@ def _norm_args(x, weight, residual, eps, index):
     if not eps >= 0.0:
         _fail("eps must not be negative")
     weight = _tensor("weight", weight, (D,), _F32, index)
-    residual, ldr = (None, 0) if residual is None else _rows("residual", residual, rows, D, x.dtype, index)
+    residual, ldr = (None, 0) if residual is None else _rows("residual", residual, (rows, D), x.dtype, index)
     return x, ldx, weight, residual, ldr, eps
 
 
@@ -462,8 +463,8 @@ class _NormFn(torch.autograd.Function):
         with _on(index):
             h, ldh, weight, _, _, eps = _norm_args(h, weight, None, ctx.eps, index)
             rows, D = h.shape
-            dy, ldy = _gradient(dy, h, rows, D, index)
-            dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h, rows, D, index)
+            dy, ldy = _gradient(dy, h, (rows, D), index)
+            dtotal, ldt = (None, 0) if dtotal is None else _gradient(dtotal, h, (rows, D), index)
             dh = h.new_empty((rows, D))
             dw = weight.new_empty(D)
             ws = _workspace(_bytes("eventad_rms_norm_workspace", rows, D), h)
