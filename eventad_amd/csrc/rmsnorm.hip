@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void k_norm_fwd(NormArgs a) {
 // definition says, so the quotient is formed in float32 (p, its maximum, 448 / maximum and the product: error below 5 units in the
 // last place) and, where it lies within 8 of a border, again in float64, where p is exact.  One value in 60,000 of ordinary data
 // does.  A row with max|p| below 2^-100 is formed in float64 altogether: 448 / max|p| leaves float32 at 1.3e-36, and below 1.2e-38 p
-// has not all its bits.
+// has not all its bits; so is its scale.
 
 // v rounded towards the odd neighbour, so that a second rounding to fewer bits is the one rounding of v: e4m3 keeps 4 of the
 // 24 bits of a float
@@ -241,7 +241,6 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
     float scale = __uint_as_float(most) * inv / 448.f;
     const bool zero = !(scale >= 1.17549435e-38f) && scale == scale;             // a row of zeros (or next to it)
     if (zero) scale = 1.f;
-    if (in && lane == 0) a.scale[r] = scale;
     const float by32 = zero ? inv : 448.f / __uint_as_float(most);
     const bool tiny = !zero && most < 0x0d800000u;               // 2^-100
     // p -> q of a piece; true if a value lies too close to a border
@@ -294,7 +293,9 @@ __global__ __launch_bounds__(256) void k_norm_fp8(NormArgs a) {
             exact = max(max(s_exact[0], s_exact[1]), max(s_exact[2], s_exact[3]));
         }
         by = most > 0x7f800000u ? (double)__builtin_nanf("") : zero ? (double)inv : 448.0 / __longlong_as_double(exact);
+        if (tiny) scale = (float)(__longlong_as_double(exact) * (double)inv / 448.0);
     }
+    if (in && lane == 0) a.scale[r] = scale;
     if (!in) return;
     auto finish = [&](int c, float (&q)[V], bool again) {
         if (again) {

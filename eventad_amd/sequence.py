@@ -374,7 +374,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     u, delta, z [rows, channels]; B, C [rows, states], shared by the channels; A float32 [channels, states], states 1..64;
     D, delta_bias float32 [channels].  D, z and delta_bias may be None; delta_softplus=False takes delta + delta_bias as the step
     itself.  An A of -inf is a state that forgets at once: it counts as -2.36e38, which every step of 1e-36 or more takes to
-    exp(s A) = 0; a step of 0 leaves the state as it is.  state float32 [clips, channels, states] = h in front of each clip's first row (None: zeros).
+    exp(s A) = 0; a step of 0 leaves the state as it is.  state float32 [clips, channels, states] = h in front of each clip's
+    first row (None: zeros).
     -> y, or (y, final_state) with return_state: h behind each clip's last row (an empty clip keeps its state).
 
     Every clip's end inside a group of 16 rows costs that group another turn: a batch whose clips are all a row or two long is

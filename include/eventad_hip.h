@@ -573,7 +573,8 @@ int eventad_selective_scan_step(const void* u, int64_t ldu, const void* delta, i
 int eventad_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, void* sum, int64_t lds,
                          void* y, int64_t ldy, int64_t rows, int channels, float eps, int dtype, void* stream);
 /* The same row y as 8-bit values (e4m3: 3 fraction bits, largest 448): scale[row] = max|y| / 448 (1 where that is below the
- * smallest normal number, as for a row of zeros), q = y / scale rounded to nearest even.  q u8[rows,channels] with row stride ldq, scale f32[rows]. */
+ * smallest normal number, as for a row of zeros), q = y / scale rounded to nearest even.  q u8[rows,channels] with row stride
+ * ldq, scale f32[rows]. */
 int eventad_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, void* sum, int64_t lds,
                          uint8_t* q, int64_t ldq, float* scale, int64_t rows, int channels, float eps, int dtype, void* stream);
 int eventad_rms_norm_workspace(int64_t rows, int channels, int64_t* bytes);

@@ -1030,3 +1030,19 @@ def test_checkpointed_block_has_the_same_gradients(S, reentrant):
         results.append([*(o.detach() for o in out), *(t.grad.clone() for t in (*L, *p.values()))])
     for i, (s, t) in enumerate(zip(*results)):
         assert torch.equal(s, t), i
+
+
+@pytest.mark.parametrize("channels", [40, 2048, 9000])
+def test_rms_norm_fp8_scale_of_subnormal_products(S, channels):
+    """With a small eps a row of subnormal numbers has a scale in the normal range: it keeps all its bits."""
+    gen = torch.Generator().manual_seed(channels)
+    size = torch.tensor([1e-38, 1e-39, 1e-41, 1e-43])[:, None]
+    x = torch.randn(len(size), channels, generator=gen)
+    x = x / x.abs().amax(1, keepdim=True) * size
+    w = torch.rand(channels, generator=gen) + 0.5
+    want = R.norm(x, w, None, 2.0 ** -100)                       # y = h w 2^50: the squares of h vanish beside eps
+    q, scale = S.rms_norm_fp8(x.cuda(), w.cuda(), eps=2.0 ** -100)
+    assert torch.equal(q.double().cpu(), want["q"])
+    got = scale.double().cpu()
+    # the quotient's root, its reciprocal (2 units each) and one rounding
+    assert bool(((got - want["scale"][0]).abs() <= 6 * UNIT * want["scale"][0]).all())
